@@ -40,7 +40,8 @@ enum {
   GR_DEV_BAD_LENGTH = 2,  /* length beyond the block-table row capacity */
   GR_DEV_BAD_PARENT = 4,  /* parent index outside [0, beam width) */
   GR_DEV_SUFFIX_FULL = 8, /* append past the row capacity (token dropped) */
-  GR_DEV_BAD_NODE = 16    /* catalog node id or child range outside the trie */
+  GR_DEV_BAD_NODE = 16,   /* catalog node id or child range outside the trie */
+  GR_DEV_BAD_EXPERT = 32  /* expert id >= the number of experts */
 };
 
 enum { GR_DTYPE_F32 = 0, GR_DTYPE_F16 = 1, GR_DTYPE_BF16 = 2,

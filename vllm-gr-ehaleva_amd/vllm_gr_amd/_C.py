@@ -1,5 +1,5 @@
-"""ctypes binding of libgr_beam.so (declared in include/gr_beam.h and
-include/gr_decoder.h).
+"""ctypes binding of libgr_beam.so (declared in include/gr_beam.h,
+include/gr_decoder.h and include/gr_experts.h).
 
 The library is the product: there is no Python or CPU fallback.  Loading
 fails loudly with an ImportError-like RuntimeError when the shared object is
@@ -25,13 +25,14 @@ GR_DEV_BAD_LENGTH = 2
 GR_DEV_BAD_PARENT = 4
 GR_DEV_SUFFIX_FULL = 8
 GR_DEV_BAD_NODE = 16
+GR_DEV_BAD_EXPERT = 32
 
 GR_PRUNE_SCRATCH_BYTES = 16 << 20  # static scratch of gr_beam_prune_topk_noalloc
 
 GR_DTYPE_F32 = 0
 GR_DTYPE_F16 = 1
 GR_DTYPE_BF16 = 2
-GR_DTYPE_FP8_E4M3 = 3  # KV-cache element type only
+GR_DTYPE_FP8_E4M3 = 3  # KV caches and block-scaled operands
 
 _P = ctypes.c_void_p
 _I = ctypes.c_int
@@ -47,7 +48,10 @@ class AttnOptions(ctypes.Structure):
                 ("kv_dtype", ctypes.c_int), ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p)]
 
 
-# name -> (restype, argtypes); mirrors include/gr_beam.h and include/gr_decoder.h one to one
+GR_SCORE_SOFTMAX = 0
+GR_SCORE_SIGMOID = 1
+
+# name -> (restype, argtypes); mirrors the headers in include/ one to one
 SIGNATURES = {
     "gr_status_string": (ctypes.c_char_p, [_I]),
     "gr_version": (_I, []),
@@ -99,6 +103,25 @@ SIGNATURES = {
     ]),
     "gr_linear": (_I, [_P, _L, _P, _L, _P, _L, _I, _I, _I, _I, _I, _I, _P]),
     "gr_linear_tile": (_I, [_I, _I, _I, _I]),
+    "gr_quant_fp8": (_I, [_P, _L, _P, _L, _L, _P, _L, _I, _I, _I, _P]),
+    "gr_linear_fp8": (_I, [
+        _P, _L, _P, _L, _L,             # out, out_stride, out_scale and its row / group strides
+        _P, _L, _P, _L, _L,             # x, x_stride, x_scale and its row / group strides
+        _P, _L, _P,                     # w, w_stride, w_scale
+        _I, _I, _I, _I, _I, _P,         # tokens, out_features, in_features, swiglu, out_dtype, stream
+    ]),
+    "gr_route_experts": (_I, [
+        _P, _P, _P, _L, _P,             # weights, ids, logits, logits_stride, bias
+        _I, _I, _I, _I, _I, _I, _I,     # tokens, experts, top_k, score, num_groups, top_groups, renormalize
+        _F, _I, _P,                     # scale, dtype, stream
+    ]),
+    "gr_expert_mlp_workspace_size": (_SZ, [_I, _I, _I, _I, _I, _I]),
+    "gr_expert_mlp": (_I, [
+        _P, _L, _P, _L, _P, _P, _P, _P, # out, out_stride, x, x_stride, gate_up, its scale, down, its scale
+        _P, _P,                         # weights, ids
+        _I, _I, _I, _I, _I, _I,         # tokens, top_k, experts, hidden, ffn, dtype
+        _P, _SZ, _P, _P,                # workspace, bytes, dev_status, stream
+    ]),
     "gr_silu_mul": (_I, [_P, _L, _P, _L, _I, _I, _I, _P]),
     "gr_reshape_and_cache": (_I, [
         _P, _L, _P, _L, _P, _P, _L, _L, _L, _L, _P, _I, _I, _I, _I, _I, _P, _P,

@@ -1,5 +1,5 @@
 """torch-tensor entry points over the C ABI (include/gr_beam.h,
-include/gr_decoder.h).
+include/gr_decoder.h, include/gr_experts.h).
 
 Each function validates shapes/devices on the host, allocates outputs with
 the torch caching allocator when the caller passes none, and launches on
@@ -9,6 +9,7 @@ the HIP library every call raises.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import weakref
 
@@ -103,7 +104,8 @@ def check_status(status: torch.Tensor) -> None:
                                 (_C.GR_DEV_BAD_LENGTH, "length beyond table capacity"),
                                 (_C.GR_DEV_BAD_PARENT, "parent index out of range"),
                                 (_C.GR_DEV_SUFFIX_FULL, "suffix full"),
-                                (_C.GR_DEV_BAD_NODE, "catalog node out of range")) if bits & b]
+                                (_C.GR_DEV_BAD_NODE, "catalog node out of range"),
+                                (_C.GR_DEV_BAD_EXPERT, "expert id out of range")) if bits & b]
         raise ValueError("device tables rejected: " + ", ".join(names))
 
 
@@ -726,3 +728,193 @@ def silu_mul(x: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
                                 _dtype_code(x), _stream(dev))
     _C.check("gr_silu_mul", code)
     return out
+
+
+# ---- 8-bit block-scaled projections and routed experts (include/gr_experts.h) ----
+
+#: features of a row of activations, and rows and features of a weight block, that share a scale
+FP8_BLOCK = 128
+
+
+def _blocks(n: int) -> int:
+    return -(-n // FP8_BLOCK)
+
+
+def _row_stride(t: torch.Tensor) -> int:
+    """Elements from row to row; of a single row, whose stride means nothing, its length."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _on(dev: torch.device):
+    """Launches go to ``dev``, also while another device is the current one."""
+    return contextlib.nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+
+def _row_scales(name: str, t: torch.Tensor, rows: int, features: int) -> None:
+    if t.dtype != torch.float32 or t.shape != (rows, _blocks(features)):
+        raise ValueError(f"{name} must be a float32 [tokens, ceil(features / 128)] tensor")
+
+
+def _new_row_scales(rows: int, features: int, dev) -> torch.Tensor:
+    """Scales of quantised rows, a group's scales of all rows side by side (the
+    order in which the product reads them)."""
+    return torch.empty((_blocks(features), rows), dtype=torch.float32, device=dev).t()
+
+
+def quant_fp8(x: torch.Tensor, *, out: torch.Tensor | None = None, scale: torch.Tensor | None = None):
+    """Rows ``x [T, K]`` (float32, fp16 or bf16) as e4m3 with one float32 scale
+    for each 128 features: ``(out [T, K] float8_e4m3fn, scale [T, ceil(K / 128)])``,
+    the value being ``out * scale``; see ``gr_quant_fp8`` in gr_experts.h.  ``K`` is
+    a multiple of 16 and rows are 16-byte aligned; ``scale`` may have any strides."""
+    dev = _need_cuda(x, out, scale)
+    _rows("x", x)
+    T, K = x.shape
+    if out is None:
+        out = torch.empty((T, K), dtype=torch.float8_e4m3fn, device=dev)
+    _rows("out", out)
+    if out.shape != x.shape or out.dtype != torch.float8_e4m3fn:
+        raise ValueError("out must be a float8_e4m3fn tensor of x's shape")
+    if scale is None:
+        scale = _new_row_scales(T, K, dev)
+    _row_scales("scale", scale, T, K)
+    with _on(dev):
+        code = _C.lib().gr_quant_fp8(out.data_ptr(), _row_stride(out), scale.data_ptr(), scale.stride(0), scale.stride(1),
+                                     x.data_ptr(), _row_stride(x), T, K, _dtype_code(x), _stream(dev))
+    _C.check("gr_quant_fp8", code)
+    return out, scale
+
+
+def linear_fp8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, *,
+               swiglu: bool = False, quantized: bool = False, out_dtype: torch.dtype = torch.bfloat16,
+               out: torch.Tensor | None = None, out_scale: torch.Tensor | None = None):
+    """``x [T, K] @ w[N, K].T`` of e4m3 operands (float8_e4m3fn) with float32 sums:
+    ``x_scale [T, ceil(K / 128)]`` of any strides as ``quant_fp8`` gives them,
+    ``w_scale [ceil(N / 128), ceil(K / 128)]`` contiguous; see ``gr_linear_fp8`` in
+    gr_experts.h.  ``swiglu``: ``silu(gate) * up`` of the two halves of ``w``'s
+    rows, whose block scales stand one half's after the other's.  Returns ``[T, N]``
+    of ``out_dtype`` (float32, fp16, bf16), or with ``quantized`` the pair
+    ``quant_fp8`` would give of the float32 results."""
+    dev = _need_cuda(x, x_scale, w, w_scale, out, out_scale)
+    _rows("x", x)
+    _rows("w", w)
+    if x.dtype != torch.float8_e4m3fn or w.dtype != torch.float8_e4m3fn:
+        raise ValueError("x and w must be float8_e4m3fn")
+    T, K = x.shape
+    rows = w.shape[0]
+    if w.shape[1] != K or (swiglu and rows % 2):
+        raise ValueError("w must be [out_features, in_features] (twice the rows with swiglu)")
+    N = rows // 2 if swiglu else rows
+    _row_scales("x_scale", x_scale, T, K)
+    if (w_scale.dtype != torch.float32 or w_scale.shape != (_blocks(N) * (2 if swiglu else 1), _blocks(K))
+            or not w_scale.is_contiguous()):
+        raise ValueError("w_scale must be a contiguous float32 [blocks of rows, blocks of features] tensor")
+    odt = torch.float8_e4m3fn if quantized else out_dtype
+    if out is None:
+        out = torch.empty((T, N), dtype=odt, device=dev)
+    _rows("out", out)
+    if out.shape != (T, N) or out.dtype != odt:
+        raise ValueError("out must be [tokens, out_features] of the result's type")
+    if quantized and out_scale is None:
+        out_scale = _new_row_scales(T, N, dev)
+    if out_scale is not None:
+        if not quantized:
+            raise ValueError("out_scale goes with quantized=True")
+        _row_scales("out_scale", out_scale, T, N)
+    with _on(dev):
+        code = _C.lib().gr_linear_fp8(
+            out.data_ptr(), _row_stride(out), _ptr(out_scale), *(out_scale.stride() if quantized else (0, 0)),
+            x.data_ptr(), _row_stride(x), x_scale.data_ptr(), x_scale.stride(0), x_scale.stride(1), w.data_ptr(),
+            _row_stride(w), w_scale.data_ptr(), T, N, K, int(swiglu),
+            _C.GR_DTYPE_FP8_E4M3 if quantized else _dtype_code(out), _stream(dev))
+    _C.check("gr_linear_fp8", code)
+    return (out, out_scale) if quantized else out
+
+
+_SCORES = {"softmax": _C.GR_SCORE_SOFTMAX, "sigmoid": _C.GR_SCORE_SIGMOID}
+
+
+def route_experts(logits: torch.Tensor, top_k: int, *, score: str = "softmax", bias: torch.Tensor | None = None,
+                  num_groups: int = 1, top_groups: int = 1, renormalize: bool = True, scale: float = 1.0):
+    """Each token's ``top_k`` experts from its router logits ``[T, E]`` (float32,
+    fp16 or bf16; row stride free): ``(weights [T, top_k] float32, ids [T, top_k]
+    int32)``, best first; see ``gr_route_experts`` in gr_experts.h.  ``score`` is
+    'softmax' or 'sigmoid'; ``bias [E]`` (float32) is added for the choice only;
+    with ``num_groups`` the choice is among the experts of the ``top_groups`` best."""
+    dev = _need_cuda(logits, bias)
+    _rows("logits", logits)
+    T, E = logits.shape
+    if score not in _SCORES:
+        raise ValueError("score must be 'softmax' or 'sigmoid'")
+    if bias is not None and (bias.shape != (E,) or bias.dtype != torch.float32 or not bias.is_contiguous()):
+        raise ValueError("bias must be a contiguous float32 [experts] tensor")
+    top_k = int(top_k)
+    if top_k < 1:
+        raise ValueError("top_k must be at least 1")
+    weights = torch.empty((T, top_k), dtype=torch.float32, device=dev)
+    ids = torch.empty((T, top_k), dtype=torch.int32, device=dev)
+    with _on(dev):
+        code = _C.lib().gr_route_experts(
+            weights.data_ptr(), ids.data_ptr(), logits.data_ptr(), _row_stride(logits), _ptr(bias), T, E, top_k,
+            _SCORES[score], int(num_groups), int(top_groups), int(bool(renormalize)), float(scale), _dtype_code(logits),
+            _stream(dev))
+    _C.check("gr_route_experts", code)
+    return weights, ids
+
+
+def expert_mlp(x: torch.Tensor, gate_up: torch.Tensor, down: torch.Tensor, weights: torch.Tensor, ids: torch.Tensor,
+               *, gate_up_scale: torch.Tensor | None = None, down_scale: torch.Tensor | None = None,
+               out: torch.Tensor | None = None, workspace: torch.Tensor | None = None,
+               status: torch.Tensor | None = None) -> torch.Tensor:
+    """``out[t] = sum_j weights[t, j] * down[e] @ (silu(gate[e] @ x[t]) * (up[e] @ x[t]))``
+    with ``e = ids[t, j]``, for ``x [T, H]`` (fp16 or bf16), ``gate_up [E, 2 F, H]``
+    (gate | up), ``down [E, H, F]`` and what ``route_experts`` gives; see
+    ``gr_expert_mlp`` in gr_experts.h.  Weights are of ``x``'s type, or
+    float8_e4m3fn with ``gate_up_scale [E, 2 ceil(F / 128), ceil(H / 128)]`` and
+    ``down_scale [E, ceil(H / 128), ceil(F / 128)]``.  An id below 0 adds nothing;
+    one of E or more adds nothing and is flagged in ``status``.  ``workspace``: uint8,
+    ``expert_mlp_workspace_bytes`` of it (allocated when None)."""
+    dev = _need_cuda(x, gate_up, down, weights, ids, gate_up_scale, down_scale, out, workspace, status)
+    _rows("x", x)
+    T, H = x.shape
+    if gate_up.dim() != 3 or down.dim() != 3 or gate_up.shape[1] % 2:
+        raise ValueError("gate_up must be [E, 2 F, H] and down [E, H, F]")
+    E, F = gate_up.shape[0], gate_up.shape[1] // 2
+    if gate_up.shape[2] != H or down.shape != (E, H, F) or not gate_up.is_contiguous() or not down.is_contiguous():
+        raise ValueError("gate_up must be a contiguous [E, 2 F, H] tensor and down a contiguous [E, H, F] one")
+    if ids.dim() != 2 or ids.shape[0] != T or ids.dtype != torch.int32 or not ids.is_contiguous():
+        raise ValueError("ids must be a contiguous int32 [tokens, top_k] tensor")
+    if weights.shape != ids.shape or weights.dtype != torch.float32 or not weights.is_contiguous():
+        raise ValueError("weights must be a contiguous float32 [tokens, top_k] tensor")
+    fp8 = gate_up_scale is not None or down_scale is not None
+    if fp8:
+        if gate_up.dtype != torch.float8_e4m3fn or down.dtype != torch.float8_e4m3fn:
+            raise ValueError("scales go with float8_e4m3fn weights")
+        for name, t, shape in (("gate_up_scale", gate_up_scale, (E, 2 * _blocks(F), _blocks(H))),
+                               ("down_scale", down_scale, (E, _blocks(H), _blocks(F)))):
+            if t is None or t.dtype != torch.float32 or t.shape != shape or not t.is_contiguous():
+                raise ValueError(f"{name} must be a contiguous float32 {list(shape)} tensor")
+    elif gate_up.dtype != x.dtype or down.dtype != x.dtype:
+        raise ValueError("the weights must have x's dtype, or be float8_e4m3fn with their scales")
+    k = ids.shape[1]
+    if k < 1:
+        raise ValueError("ids must name at least one expert a token")
+    if out is None:
+        out = torch.empty((T, H), dtype=x.dtype, device=dev)
+    _rows("out", out)
+    if out.shape != x.shape or out.dtype != x.dtype:
+        raise ValueError("out must match x")
+    need = expert_mlp_workspace_bytes(T, k, E, H, F, fp8)
+    if workspace is None:
+        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+    with _on(dev):
+        code = _C.lib().gr_expert_mlp(
+            out.data_ptr(), _row_stride(out), x.data_ptr(), _row_stride(x), gate_up.data_ptr(), _ptr(gate_up_scale),
+            down.data_ptr(), _ptr(down_scale), weights.data_ptr(), ids.data_ptr(), T, k, E, H, F, _dtype_code(x),
+            workspace.data_ptr(), workspace.numel() * workspace.element_size(), _ptr(status), _stream(dev))
+    _C.check("gr_expert_mlp", code)
+    return out
+
+
+def expert_mlp_workspace_bytes(num_tokens: int, top_k: int, num_experts: int, hidden: int, ffn: int, fp8: bool) -> int:
+    """Workspace of ``expert_mlp``."""
+    return int(_C.lib().gr_expert_mlp_workspace_size(num_tokens, top_k, num_experts, hidden, ffn, int(fp8)))

@@ -48,7 +48,7 @@ gr_status_t gr_quant_fp8(void* out, int64_t out_stride, float* scale, int64_t sc
  * matrix core adds the e4m3 products, in groups of 8 whose members are cut off
  * below 2^-13 of the largest (about 1.5e-5 of an ordinary result); the groups'
  * sums are float32.
- * in_features % 16 == 0; x and w rows 16-byte aligned.
+ * in_features % 16 == 0; x and w rows 16-byte aligned, at most 4 MB apart.
  */
 gr_status_t gr_linear_fp8(void* out, int64_t out_stride, float* out_scale, int64_t out_scale_row,
                           int64_t out_scale_group, const void* x, int64_t x_stride, const float* x_scale,
@@ -91,7 +91,7 @@ gr_status_t gr_route_experts(float* weights, int32_t* ids, const void* logits, i
  * ceil(ffn / 128)] they are e4m3, and x and the gated products are quantised as
  * gr_quant_fp8 does.  Everything else is float32, out is rounded once.
  * hidden % 16 == 0, ffn % 16 == 0; rows of x, and weights, 16-byte aligned; out
- * rows 8-byte aligned.  num_experts <= 1024.  workspace: gr_expert_mlp_workspace_size
+ * rows 8-byte aligned.  num_experts <= 1024, x spans less than 2 GB.  workspace: gr_expert_mlp_workspace_size
  * bytes, 256-byte aligned, no initial contents; calls that may overlap need one each.
  */
 size_t gr_expert_mlp_workspace_size(int num_tokens, int top_k, int num_experts, int hidden, int ffn, int fp8);

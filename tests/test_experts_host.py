@@ -38,7 +38,7 @@ def test_linear_refusals(built_lib):
     for o in (dict(K=248), dict(swiglu=1, N=120), dict(odt=3, os=A, N=100), dict(x=A + 8), dict(w=A + 8),
               dict(xstr=264), dict(wstr=264), dict(out=A + 2), dict(odt=0, out=A + 8), dict(odt=3, os=A, ostr=130),
               dict(xs=A + 2), dict(ws=A + 1), dict(N=2 ** 28 + 16, ostr=2 ** 28 + 16),
-              dict(T=2 ** 28, N=2 ** 27, ostr=2 ** 27)):
+              dict(T=2 ** 28, N=2 ** 27, ostr=2 ** 27), dict(xstr=2 ** 22 + 16), dict(wstr=2 ** 22 + 16)):
         assert f(**o) == UNSUPPORTED, o
 
 
@@ -67,7 +67,8 @@ def test_expert_mlp_refusals(built_lib):
               dict(dns=A)):
         assert f(**o) == BAD, o
     for o in (dict(dtype=0), dict(H=248), dict(F=120), dict(E=1025), dict(x=A + 8), dict(xstr=260), dict(gu=A + 8),
-              dict(dn=A + 8), dict(out=A + 4), dict(ostr=258), dict(T=2 ** 26, k=2), dict(gus=A + 2, dns=A)):
+              dict(dn=A + 8), dict(out=A + 4), dict(ostr=258), dict(T=2 ** 26, k=2), dict(gus=A + 2, dns=A),
+              dict(T=2 ** 19, xstr=2048), dict(H=2 ** 21 + 16, xstr=2 ** 22, ostr=2 ** 22), dict(F=2 ** 21 + 16)):
         assert f(**o) == UNSUPPORTED, o
     for o in (dict(ws=None), dict(ws=A + 128), dict(bytes=need - 1)):
         assert f(**o) == _C.GR_ERR_WORKSPACE, o

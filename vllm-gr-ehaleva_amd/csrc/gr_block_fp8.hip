@@ -50,10 +50,68 @@ __global__ __launch_bounds__(QT_THREADS) void quant_fp8_k(QuantArgs a) {
   if (l == 0) a.scale[t * a.scale_row + g * a.scale_grp] = s;
 }
 
+// The tile with the least estimated time, over the workgroups of the XCD that gets
+// the most of them (its 32 CUs take one or two each): a round costs a fixed part
+// (launch, first stages, stores) and its stages, `one` ns each alone on a CU, `two`
+// with a neighbour.  From 512 to 12288 columns and 64 to 2048 rows of 2048 and 6144
+// features (weights cold; measured, us, the picked tile's and the next best one's):
+//   64 x 4096 (2048 in)   64 x 64    8.5,  64 x 128 10.3
+//   512 x 8192            64 x 128  17.5, 128 x 128 18.5
+//   1000 x 12288         256 x 256  33.9, 128 x 128 39.9
+//   2048 x 12288         256 x 256  67.4, 128 x 128 63.7  (the estimate is within 6 %)
+//   1000 x 2048 (6144 in) 64 x 128  27.4,  64 x 64  30.0
+// A float32 result's stages convert their operands and take longer; 256 x 256 has no
+// registers for that.
+struct MmChoice { int bm, bn, per_cu, fixed, one, two; };
+constexpr MmChoice kFast[] = {{64, 64, 2, 2300, 400, 570}, {64, 128, 2, 2500, 510, 820}, {128, 128, 2, 1500, 900, 1260},
+                              {128, 256, 1, 2000, 1100, 0}, {256, 256, 1, 4000, 1600, 0}};
+constexpr MmChoice kExact[] = {{64, 64, 2, 2300, 500, 860}, {64, 128, 2, 2500, 750, 1310}, {128, 128, 2, 1500, 1150, 2000},
+                               {128, 256, 1, 2000, 1750, 0}};
+
+template <int N> int pick_tile(const MmChoice (&all)[N], int M, int rows_w, int stages) {
+  int best = 0;
+  int64_t least = INT64_MAX;
+  for (int i = 0; i < N; ++i) {
+    const MmChoice& c = all[i];
+    const int64_t tiles = ((int64_t)((M + c.bm - 1) / c.bm) * ((rows_w + c.bn - 1) / c.bn) + 7) / 8;
+    const int64_t one = c.fixed + (int64_t)stages * c.one, two = c.fixed + (int64_t)stages * c.two;
+    const int64_t round = 32 * c.per_cu, left = tiles % round;
+    const int64_t cost = tiles / round * (c.per_cu == 2 ? two : one) + (left == 0 ? 0 : left <= 32 ? one : two);
+    if (cost < least) {
+      least = cost;
+      best = i;
+    }
+  }
+  return best;
+}
+
 template <int MODE, bool EXACT>
 void launch_linear_fp8(const MmArgs& a, hipStream_t stream) {
-  constexpr int BN = MODE == MM_PLAIN_Q ? 128 : 256;
-  launch_mm<GR_DTYPE_FP8_E4M3, 64, BN, 2, 4, 3, MODE, false, EXACT>(a, (a.M + 63) / 64, stream);
+  constexpr int T = GR_DTYPE_FP8_E4M3;
+  constexpr bool GATED = MODE == MM_SWIGLU || MODE == MM_SWIGLU_Q;
+  const int M = a.M, rows_w = GATED ? 2 * a.N : a.N, stages = (a.kbytes + 127) / 128;
+  if constexpr (MODE == MM_PLAIN_Q) {
+    launch_mm<T, 64, 128, 2, 4, 3, MODE, false, EXACT>(a, (M + 63) / 64, stream);
+  } else if constexpr (MODE == MM_SWIGLU_Q) {
+    // a group of 128 results is 256 weight rows of one workgroup, which leaves little choice
+    const int64_t cols = (a.N + 127) / 128;
+    if ((M + 63) / 64 * cols <= 256) launch_mm<T, 64, 256, 2, 4, 3, MODE, false, EXACT>(a, (M + 63) / 64, stream);
+    else launch_mm<T, 128, 256, 2, 4, 3, MODE, false, EXACT>(a, (M + 127) / 128, stream);
+  } else {
+    // as long as two workgroups a CU hold them all (8 rows x 4096 columns 4.8 us, by 64 x 64 tiles 8.7; 64 x 4096
+    // 8.5; 64 x 8192, twice that many, 14.5 against 9.5)
+    const int64_t cols = (a.N + 15) / 16, few = (M + 15) / 16 * cols, few2 = (M + 31) / 32 * cols;
+    if (few <= 256 || (M <= 16 && few <= 512)) return launch_few<T, 1, 8, MODE, false>(a, (M + 15) / 16, stream);
+    if (few2 <= 512) return launch_few<T, 2, 8, MODE, false>(a, (M + 31) / 32, stream);
+    switch (EXACT ? pick_tile(kExact, M, rows_w, stages) : pick_tile(kFast, M, rows_w, stages)) {
+      case 0: launch_mm<T, 64, 64, 2, 2, 4, MODE, false, EXACT>(a, (M + 63) / 64, stream); break;
+      case 1: launch_mm<T, 64, 128, 2, 2, 3, MODE, false, EXACT>(a, (M + 63) / 64, stream); break;
+      case 2: launch_mm<T, 128, 128, 2, 2, 2, MODE, false, EXACT>(a, (M + 127) / 128, stream); break;
+      case 3: launch_mm<T, 128, 256, 2, 4, 3, MODE, false, EXACT>(a, (M + 127) / 128, stream); break;
+      default:
+        if constexpr (!EXACT) launch_mm<T, 256, 256, 2, 4, 2, MODE, false, EXACT>(a, (M + 255) / 256, stream);
+    }
+  }
 }
 
 }  // namespace
@@ -108,7 +166,7 @@ extern "C" gr_status_t gr_linear_fp8(void* out, int64_t out_stride, float* out_s
       (quant && (!out_scale || out_scale_row < 0 || out_scale_group < 0)))
     return GR_ERR_INVALID_ARG;
   if (in_features % 16 != 0 || ((swiglu || quant) && out_features % 16 != 0) || out_features > (1 << 28) ||
-      num_tokens > (1 << 28) || !aligned(x, 16) || x_stride % 16 != 0 || !aligned(w, 16) || w_stride % 16 != 0 ||
+      num_tokens > (1 << 28) || x_stride > (1 << 22) || w_stride > (1 << 22) || !aligned(x, 16) || x_stride % 16 != 0 || !aligned(w, 16) || w_stride % 16 != 0 ||
       !aligned(out, out_dtype == GR_DTYPE_F32 ? 16 : quant ? 4 : 8) || (quant && out_stride % 4 != 0) ||
       !aligned(x_scale, 4) || !aligned(w_scale, 4) || (quant && !aligned(out_scale, 4)) ||
       ((int64_t)num_tokens + 15) / 16 * ((out_features + 15) / 16) > INT32_MAX - 8)

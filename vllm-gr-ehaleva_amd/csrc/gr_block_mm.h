@@ -97,29 +97,13 @@ template <int DT> __device__ inline mm4_t mm_mma(u32x4_t a, u32x4_t b, mm4_t c) 
                                                   0, 0);
 }
 
-// cnt neighbouring results in the output's type; vec: all four, aligned
-__device__ inline void mm_store(void* out, int type, int64_t at, const float (&v)[4], int cnt, bool vec) {
-  if (type == GR_DTYPE_F32) {
-    float* o = static_cast<float*>(out) + at;
-    if (vec) *reinterpret_cast<mm4_t*>(o) = mm4_t{v[0], v[1], v[2], v[3]};
-    else
-#pragma unroll
-      for (int u = 0; u < 4; ++u)
-        if (u < cnt) o[u] = v[u];
-    return;
-  }
-  const bool bf = type == GR_DTYPE_BF16;
-  const uint32_t lo = bf ? Mma<GR_DTYPE_BF16>::pack2(v[0], v[1]) : Mma<GR_DTYPE_F16>::pack2(v[0], v[1]);
-  const uint32_t hi = bf ? Mma<GR_DTYPE_BF16>::pack2(v[2], v[3]) : Mma<GR_DTYPE_F16>::pack2(v[2], v[3]);
-  uint16_t* o = static_cast<uint16_t*>(out) + at;
-  if (vec) {
-    *reinterpret_cast<u32x2_t*>(o) = u32x2_t{lo, hi};
-    return;
-  }
-  const uint32_t p[2] = {lo, hi};
-#pragma unroll
-  for (int u = 0; u < 4; ++u)
-    if (u < cnt) o[u] = (uint16_t)(p[u >> 1] >> (16 * (u & 1)));
+// four neighbouring results in the output's type
+template <int OT> __device__ __forceinline__ void mm_store(void* out, int64_t at, const float (&v)[4]) {
+  if constexpr (OT == GR_DTYPE_F32)
+    *reinterpret_cast<mm4_t*>(static_cast<float*>(out) + at) = mm4_t{v[0], v[1], v[2], v[3]};
+  else
+    *reinterpret_cast<u32x2_t*>(static_cast<uint16_t*>(out) + at) =
+        u32x2_t{Mma<OT>::pack2(v[0], v[1]), Mma<OT>::pack2(v[2], v[3])};
 }
 
 // One dword per lane from global memory into LDS: lane i's lands at lds + 4 i.
@@ -152,172 +136,239 @@ __device__ inline bool mm_tile(const MmArgs& a, int tiles_m, int& mt, int& nt) {
   return true;
 }
 
+// One 16-byte chunk per lane of a buffer (base and length in d) into LDS: lane i's,
+// from byte off + soff, lands at lds + 16 i; zeros where off is past the length.  (M0
+// is no value's home for the compiler: it sets it where an instruction of its own reads it.)
+__device__ __forceinline__ void dma_b(uint32_t lds, u32x4_t d, uint32_t off, uint32_t soff) {
+  __asm__ volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+                   : : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(off), "s"(d), "s"(__builtin_amdgcn_readfirstlane(soff))
+               : "memory");
+}
+// A buffer of 2 GB from p on: offsets of MM_NOWHERE and more read zeros.
+constexpr uint32_t MM_NOWHERE = 0x80000000u;
+__device__ inline u32x4_t mm_buffer(const void* p) {
+  const uint64_t b = reinterpret_cast<uint64_t>(p);
+  return u32x4_t{(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)b),
+                 (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(b >> 32)) & 0xFFFFu, MM_NOWHERE, 0x00027000u};
+}
+
+// What a tile's workgroup knows about it.
+struct MmTile {
+  int mt, nt, m0, m_end, n0;
+  const uint8_t* w;
+  const float* ws;
+};
+
 // XT: element type of both operands.  WM x WN waves over a BM x BN tile (BN weight
 // rows; with SwiGLU 16 gate rows and the 16 up rows of the same columns alternate).
-template <int XT, int BM, int BN, int WM, int WN, int ST, int MODE, bool EXPERTS, bool EXACT>
-__global__ __launch_bounds__(64 * WM * WN) void block_mm(MmArgs a) {
-  constexpr bool F8 = XT == GR_DTYPE_FP8_E4M3;
+template <int XT, int BM, int BN, int WM, int WN, int MODE, bool EXPERTS, bool EXACT>
+struct Mm {
+  static constexpr bool F8 = XT == GR_DTYPE_FP8_E4M3;
+  static constexpr bool GATED = MODE == MM_SWIGLU || MODE == MM_SWIGLU_Q;
+  static constexpr bool QUANT = MODE == MM_SWIGLU_Q || MODE == MM_PLAIN_Q;
+  static constexpr int NW = WM * WN;
+  static constexpr int TILE = (BM + BN) * 128;              // bytes of a stage
+  static constexpr int SCALES = F8 ? NW * 256 : 0;          // and of its scales
+  static constexpr int LPS = (BM + BN) / 8 / NW;            // transfers per wave and stage, 8 rows each
+  static constexpr int OPS = LPS + (F8 ? 1 : 0);
+  static constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
+  static constexpr int OC = GATED ? BN / 2 : BN;            // output columns of the tile
+  static constexpr int WBLOCKS = (OC + 127) / 128 * (GATED ? 2 : 1);  // weight blocks of the tile
   static_assert(F8 || !EXACT, "16-bit sums are exact as they are");
-  constexpr bool GATED = MODE == MM_SWIGLU || MODE == MM_SWIGLU_Q;
-  constexpr bool QUANT = MODE == MM_SWIGLU_Q || MODE == MM_PLAIN_Q;
-  constexpr int NW = WM * WN;
-  constexpr int TILE = (BM + BN) * 128;                 // bytes of a stage
-  constexpr int STAGE = TILE + (F8 ? NW * 256 : 0);     // and the row scales
-  constexpr int LPS = (BM + BN) / 8 / NW;               // transfers per wave and stage, 8 rows each
-  constexpr int OPS = LPS + (F8 ? 1 : 0);
-  constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
-  constexpr int OC = GATED ? BN / 2 : BN;               // output columns of the tile
-  static_assert((BM + BN) % (8 * NW) == 0 && BM <= NW * 64, "whole transfers");
   static_assert(BM % (16 * WM) == 0 && BN % (16 * WN) == 0 && (!GATED || FN % 2 == 0), "whole fragments");
-  static_assert(OC / WN <= 128 && 128 % (OC / WN) == 0, "a wave's columns share a weight block");
+  static_assert(OC / WN <= 128 && 128 % (OC / WN) == 0 && (OC / WN) % 16 == 0, "a wave's columns share a weight block");
   static_assert(!QUANT || OC == 128, "a tile's columns are one group of the result");
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[ST * STAGE];
 
-  const int tiles_m = EXPERTS ? __builtin_amdgcn_readfirstlane(*a.num_tiles) : a.tiles_m;
-  int mt, nt;
-  if (!mm_tile(a, tiles_m, mt, nt)) return;
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wm = wave / WN, wn = wave % WN;
-  int m0 = mt * BM, m_end = a.M;
-  const uint8_t* w = a.w;
-  const float* ws = a.ws;
-  if constexpr (EXPERTS) {
-    const int4 t = a.tiles[mt];
-    const int e = __builtin_amdgcn_readfirstlane(t.x);
-    m0 = __builtin_amdgcn_readfirstlane(t.y);
-    m_end = m0 + __builtin_amdgcn_readfirstlane(t.z);
-    w += e * a.w_expert;
-    if constexpr (F8) ws += e * a.ws_expert;
-  }
-  const int n0 = nt * OC;
+  using Acc = mm4_t[FN][FM];
 
   // Transfer i of a stage moves LDS rows 8 (wave + NW i) .. + 7 (x rows, then w
   // rows); lane l lands on row l >> 3, chunk l & 7 of them and fetches the logical
   // chunk (l & 7) ^ (row & 7).  Rows past the tile's last repeat it (their results
-  // are not stored).
-  const int ch = ((lane & 7) ^ (lane >> 3)) * 16;
-  auto x_row = [&](int r) -> int64_t {
-    const int p = min(m0 + r, m_end - 1);
+  // are not stored).  One more transfer, of a dword a lane, moves the scales.
+  struct Source {
+    u32x4_t buf[LPS];   // wave-uniform
+    uint32_t off[LPS];
+    const float* scale;
+    int scale_step;
+    uint32_t ch;        // this lane's byte within a stage of a row
+  };
+
+  __device__ static __forceinline__ bool tile(const MmArgs& a, MmTile& t) {
+    const int tiles_m = EXPERTS ? __builtin_amdgcn_readfirstlane(*a.num_tiles) : a.tiles_m;
+    if (!mm_tile(a, tiles_m, t.mt, t.nt)) return false;
+    t.m0 = t.mt * BM;
+    t.m_end = a.M;
+    t.w = a.w;
+    t.ws = a.ws;
+    if constexpr (EXPERTS) {
+      const int4 e = a.tiles[t.mt];
+      const int id = __builtin_amdgcn_readfirstlane(e.x);
+      t.m0 = __builtin_amdgcn_readfirstlane(e.y);
+      t.m_end = t.m0 + __builtin_amdgcn_readfirstlane(e.z);
+      t.w += id * a.w_expert;
+      if constexpr (F8) t.ws += id * a.ws_expert;
+    }
+    t.n0 = t.nt * OC;
+    return true;
+  }
+
+  __device__ static __forceinline__ int x_row(const MmArgs& a, const MmTile& t, int r) {
+    const int p = min(t.m0 + r, t.m_end - 1);
     if constexpr (EXPERTS) return a.gather ? a.slot[p] / a.gather : p;
     else return p;
-  };
-  const uint8_t* src[LPS];
-#pragma unroll
-  for (int i = 0; i < LPS; ++i) {
-    const int row = 8 * (wave + NW * i) + (lane >> 3);
-    if (row < BM) {
-      src[i] = a.x + x_row(row) * a.x_stride + ch;
-    } else {
-      const int b = row - BM;
-      const int64_t n = GATED ? min(n0 + (b >> 5) * 16 + (b & 15), a.N - 1) + (int64_t)((b >> 4) & 1) * a.N
-                              : min(n0 + b, a.N - 1);
-      src[i] = w + n * a.w_stride + ch;
-    }
   }
-  const float* xsrc = F8 ? a.xs + x_row(min(wave * 64 + lane, BM - 1)) * a.xs_row : nullptr;
-  const uint32_t lds0 = (uint32_t)reinterpret_cast<uintptr_t>(lds);
-  const int n = (a.kbytes + 127) >> 7;
-  auto fetch = [&](int s, int buf) __attribute__((always_inline)) {
-    const bool part = (s + 1) * 128 > a.kbytes;  // a short last stage: zeros behind its end
+
+  __device__ static __forceinline__ void source(const MmArgs& a, const MmTile& t, int wave, int lane, Source& s) {
+    s.ch = ((lane & 7) ^ (lane >> 3)) * 16;
+    // x rows are addressed from the tile's first one, gathered ones from the tensor's
+    const int first = EXPERTS && a.gather ? 0 : t.m0;
+    const u32x4_t xb = mm_buffer(a.x + (int64_t)first * a.x_stride);
+    const u32x4_t wb = mm_buffer(t.w + (int64_t)t.n0 * a.w_stride);
+    const u32x4_t ub = GATED ? mm_buffer(t.w + (int64_t)(t.n0 + a.N) * a.w_stride) : wb;
 #pragma unroll
     for (int i = 0; i < LPS; ++i) {
-      const uint8_t* p = src[i] + (int64_t)s * 128;
-      if (part && s * 128 + ch >= a.kbytes) p = reinterpret_cast<const uint8_t*>(g_zero16);
-      dma_v(lds0 + (uint32_t)(buf * STAGE + (wave + NW * i) * 1024), p);
-    }
-    if constexpr (F8) dma_v1(lds0 + (uint32_t)(buf * STAGE + TILE + wave * 256), xsrc + s * a.xs_grp);
-  };
-
-  const int r16 = lane & 15, q = lane >> 4;
-  const int fch[2] = {(q ^ (r16 & 7)) * 16, ((4 + q) ^ (r16 & 7)) * 16};
-  const int xo = (wm * (BM / WM) + r16) * 128, wo = (BM + wn * (BN / WN) + r16) * 128;
-  mm4_t acc[FN][FM];
-#pragma unroll
-  for (int i = 0; i < FN; ++i)
-#pragma unroll
-    for (int j = 0; j < FM; ++j) acc[i][j] = mm4_t{0.f, 0.f, 0.f, 0.f};
-  // scales of this wave's weight block(s): gate's and up's with SwiGLU
-  const int kb = n, nb0 = (n0 + wn * (OC / WN)) >> 7;
-  const int nb_last = ((a.N + 127) >> 7) - 1;
-  const float* ws0 = F8 ? ws + (int64_t)min(nb0, nb_last) * kb : nullptr;
-  const float* ws1 = F8 && GATED ? ws0 + (int64_t)(nb_last + 1) * kb : ws0;
-
-  auto stage = [&](int s, int buf) __attribute__((always_inline)) {
-    const uint8_t* p = lds + buf * STAGE;
-    u32x4_t wf[2][FN];
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int i = 0; i < FN; ++i) wf[h][i] = *reinterpret_cast<const u32x4_t*>(p + wo + fch[h] + i * 2048);
-    u32x4_t wh[EXACT ? 4 : 1][FN];  // as fp16
-    if constexpr (EXACT)
-#pragma unroll
-      for (int i = 0; i < FN; ++i)
-#pragma unroll
-        for (int z = 0; z < 4; ++z)
-          wh[z][i] = Fp8Cvt<GR_DTYPE_F16>::x8(wf[z >> 1][i][2 * (z & 1)], wf[z >> 1][i][2 * (z & 1) + 1]);
-    float s0 = 0.f, s1 = 0.f;
-    if constexpr (F8) {
-      s0 = ws0[s];
-      if constexpr (GATED) s1 = ws1[s];
-    }
-#pragma unroll
-    for (int j = 0; j < FM; ++j) {
-      const u32x4_t x0 = *reinterpret_cast<const u32x4_t*>(p + xo + fch[0] + j * 2048);
-      const u32x4_t x1 = *reinterpret_cast<const u32x4_t*>(p + xo + fch[1] + j * 2048);
-      if constexpr (F8) {
-        const float xs = *reinterpret_cast<const float*>(p + TILE + (wm * (BM / WM) + j * 16 + r16) * 4);
-        const float c0 = xs * s0, c1 = GATED ? xs * s1 : c0;
-        if constexpr (EXACT) {
-          const u32x4_t xh[4] = {Fp8Cvt<GR_DTYPE_F16>::x8(x0[0], x0[1]), Fp8Cvt<GR_DTYPE_F16>::x8(x0[2], x0[3]),
-                                 Fp8Cvt<GR_DTYPE_F16>::x8(x1[0], x1[1]), Fp8Cvt<GR_DTYPE_F16>::x8(x1[2], x1[3])};
-#pragma unroll
-          for (int i = 0; i < FN; ++i) {
-            mm4_t t = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int z = 0; z < 4; ++z) t = mm_mma<GR_DTYPE_F16>(wh[z][i], xh[z], t);
-            const float c = GATED && (i & 1) ? c1 : c0;
-#pragma unroll
-            for (int u = 0; u < 4; ++u) acc[i][j][u] = fmaf(t[u], c, acc[i][j][u]);
-          }
-          continue;
-        }
-        const mm8i_t xv = __builtin_shufflevector(__builtin_bit_cast(mm4i_t, x0), __builtin_bit_cast(mm4i_t, x1), 0, 1, 2, 3, 4, 5, 6, 7);
-#pragma unroll
-        for (int i = 0; i < FN; ++i) {
-          const mm8i_t wv = __builtin_shufflevector(__builtin_bit_cast(mm4i_t, wf[0][i]), __builtin_bit_cast(mm4i_t, wf[1][i]), 0, 1, 2, 3, 4, 5, 6, 7);
-          const mm4_t t = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wv, xv, mm4_t{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
-          const float c = GATED && (i & 1) ? c1 : c0;
-#pragma unroll
-          for (int u = 0; u < 4; ++u) acc[i][j][u] = fmaf(t[u], c, acc[i][j][u]);
-        }
+      const int r8 = 8 * (wave + NW * i), row = r8 + (lane >> 3);
+      if (r8 < BM) {
+        s.buf[i] = xb;
+        s.off[i] = (uint32_t)((x_row(a, t, row) - first) * (uint32_t)a.x_stride) + s.ch;
       } else {
-#pragma unroll
-        for (int i = 0; i < FN; ++i) acc[i][j] = mm_mma<XT>(wf[0][i], x0, acc[i][j]);
-#pragma unroll
-        for (int i = 0; i < FN; ++i) acc[i][j] = mm_mma<XT>(wf[1][i], x1, acc[i][j]);
+        const int b = row - BM, n = GATED ? (b >> 5) * 16 + (b & 15) : b;
+        s.buf[i] = GATED && ((r8 - BM) >> 4 & 1) ? ub : wb;
+        s.off[i] = (uint32_t)(min(n, a.N - 1 - t.n0) * (uint32_t)a.w_stride) + s.ch;
       }
     }
-  };
+    if constexpr (F8) {
+      // entries: the tile's rows, then its weight blocks (with SwiGLU gate's, then up's)
+      const int e = wave * 64 + lane, kb = (a.kbytes + 127) >> 7, nb = (a.N + 127) >> 7;
+      if (e < BM || e >= BM + WBLOCKS) {
+        s.scale = a.xs + x_row(a, t, min(e, BM - 1)) * a.xs_row;
+        s.scale_step = (int)a.xs_grp;
+      } else {
+        constexpr int HALF = WBLOCKS / (GATED ? 2 : 1);
+        const int up = GATED ? (e - BM) / HALF : 0;
+        s.scale = t.ws + (int64_t)(up * nb + min((t.n0 >> 7) + (e - BM) % HALF, nb - 1)) * kb;
+        s.scale_step = 1;
+      }
+    }
+  }
 
-  // stage s has landed when all but the ST - 2 younger ones' transfers have; past
-  // its barrier nobody reads stage s - 1, whose buffer takes stage s + ST - 1
+  // Stage k of a tile into the buffer at LDS byte `lds`, its scales to `sc`.
+  __device__ static __forceinline__ void fetch(const MmArgs& a, const Source& s, int k, uint32_t lds, uint32_t sc, int wave) {
+    if ((k + 1) * 128 <= a.kbytes) {
 #pragma unroll
-  for (int s = 0; s < ST - 1; ++s)
-    if (s < n) fetch(s, s);
-  int buf = 0;
-  for (int s = 0; s < n; ++s) {
-    if (s + ST - 1 <= n) mm_wait_barrier<(ST - 2) * OPS>();
-    else mm_wait_barrier<0>();
-    if (s + ST - 1 < n) fetch(s + ST - 1, buf == 0 ? ST - 1 : buf - 1);
-    stage(s, buf);
-    buf = buf + 1 == ST ? 0 : buf + 1;
+      for (int i = 0; i < LPS; ++i) dma_b(lds + (uint32_t)(wave + NW * i) * 1024, s.buf[i], s.off[i], (uint32_t)k * 128);
+    } else {  // a short last stage: zeros behind its end
+      const bool in = k * 128 + (int)s.ch < a.kbytes;
+#pragma unroll
+      for (int i = 0; i < LPS; ++i)
+        dma_b(lds + (uint32_t)(wave + NW * i) * 1024, s.buf[i], in ? s.off[i] : MM_NOWHERE, (uint32_t)k * 128);
+    }
+    if constexpr (F8) dma_v1(sc + wave * 256, s.scale + (int64_t)k * s.scale_step);
+  }
+
+  struct Lane {
+    int xo, wo, fch[2], so, wso[GATED ? 2 : 1];
+  };
+  __device__ static __forceinline__ Lane lane_of(int wm, int wn, int lane) {
+    const int r16 = lane & 15, q = lane >> 4;
+    Lane l;
+    l.fch[0] = (q ^ (r16 & 7)) * 16;
+    l.fch[1] = ((4 + q) ^ (r16 & 7)) * 16;
+    l.xo = (wm * (BM / WM) + r16) * 128;
+    l.wo = (BM + wn * (BN / WN) + r16) * 128;
+    l.so = (wm * (BM / WM) + r16) * 4;
+    l.wso[0] = (BM + (wn * (OC / WN)) / 128) * 4;
+    if constexpr (GATED) l.wso[1] = l.wso[0] + WBLOCKS / 2 * 4;
+    return l;
+  }
+  // a lane's 32 bytes of a fragment of 16 rows: one 8-bit operand, or two 16-bit ones
+  __device__ static __forceinline__ mm8i_t read(const uint8_t* p, const Lane& l) {
+    const mm4i_t a = *reinterpret_cast<const mm4i_t*>(p + l.fch[0]), b = *reinterpret_cast<const mm4i_t*>(p + l.fch[1]);
+    return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+  }
+  // the wave's weight fragments and their blocks' scales
+  __device__ static __forceinline__ void read_w(const uint8_t* p, const uint8_t* sc, const Lane& l, mm8i_t (&w)[FN],
+                                                float (&ws)[2]) {
+#pragma unroll
+    for (int i = 0; i < FN; ++i) w[i] = read(p + l.wo + i * 2048, l);
+    ws[0] = ws[1] = 0.f;
+    if constexpr (F8) {
+      ws[0] = *reinterpret_cast<const float*>(sc + l.wso[0]);
+      if constexpr (GATED) ws[1] = *reinterpret_cast<const float*>(sc + l.wso[1]);
+    }
+  }
+  __device__ static __forceinline__ u32x4_t half(mm8i_t v, int h) {
+    return __builtin_bit_cast(u32x4_t, h ? __builtin_shufflevector(v, v, 4, 5, 6, 7) : __builtin_shufflevector(v, v, 0, 1, 2, 3));
+  }
+  // fragment bytes 8 z .. + 7 as fp16
+  __device__ static __forceinline__ u32x4_t fp16(mm8i_t v, int z) {
+    return Fp8Cvt<GR_DTYPE_F16>::x8((uint32_t)v[2 * z], (uint32_t)v[2 * z + 1]);
+  }
+  __device__ static __forceinline__ void convert(const mm8i_t (&w)[FN], u32x4_t (&wh)[4][FN]) {
+#pragma unroll
+    for (int i = 0; i < FN; ++i)
+#pragma unroll
+      for (int z = 0; z < 4; ++z) wh[z][i] = fp16(w[i], z);
+  }
+  // products of fragment row j; xs, ws0, ws1: the row's scale and the weight blocks'
+  __device__ static __forceinline__ void mul(const mm8i_t (&w)[FN], mm8i_t x, int j, float xs, float ws0, float ws1, Acc& acc) {
+    if constexpr (F8 && !EXACT) {
+      const float c0 = xs * ws0, c1 = GATED ? xs * ws1 : c0;
+#pragma unroll
+      for (int i = 0; i < FN; ++i) {
+        const mm4_t t = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w[i], x, mm4_t{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
+        const float c = GATED && (i & 1) ? c1 : c0;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) acc[i][j][u] = fmaf(t[u], c, acc[i][j][u]);
+      }
+    } else {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < FN; ++i) acc[i][j] = mm_mma<XT>(half(w[i], h), half(x, h), acc[i][j]);
+    }
+  }
+  // the same with the operands converted to fp16; wh: fragment bytes 8 z .. + 7 of the weights
+  __device__ static __forceinline__ void mul_exact(const u32x4_t (&wh)[4][FN], mm8i_t x, int j, float xs, float ws0,
+                                                   float ws1, Acc& acc) {
+    const float c0 = xs * ws0, c1 = GATED ? xs * ws1 : c0;
+    u32x4_t xh[4];
+#pragma unroll
+    for (int z = 0; z < 4; ++z) xh[z] = fp16(x, z);
+    mm4_t t[FN];
+#pragma unroll
+    for (int i = 0; i < FN; ++i) t[i] = mm4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int z = 0; z < 4; ++z)
+#pragma unroll
+      for (int i = 0; i < FN; ++i) t[i] = mm_mma<GR_DTYPE_F16>(wh[z][i], xh[z], t[i]);
+#pragma unroll
+    for (int i = 0; i < FN; ++i)
+#pragma unroll
+      for (int u = 0; u < 4; ++u) acc[i][j][u] = fmaf(t[i][u], GATED && (i & 1) ? c1 : c0, acc[i][j][u]);
+  }
+
+  // a stage's operands in registers
+  struct Frags {
+    mm8i_t w[FN], x[FM];
+    float ws[2], xs[FM];
+  };
+  __device__ static __forceinline__ void read_all(const uint8_t* p, const uint8_t* sc, const Lane& l, Frags& f) {
+    read_w(p, sc, l, f.w, f.ws);
+#pragma unroll
+    for (int j = 0; j < FM; ++j) {
+      f.x[j] = read(p + l.xo + j * 2048, l);
+      f.xs[j] = F8 ? *reinterpret_cast<const float*>(sc + l.so + j * 64) : 0.f;
+    }
+  }
+  __device__ static __forceinline__ void mul_all(const Frags& f, Acc& acc) {
+#pragma unroll
+    for (int j = 0; j < FM; ++j) mul(f.w, f.x[j], j, f.xs[j], f.ws[0], f.ws[1], acc);
   }
 
   // fragment (i, j), register u: column 16 i + 4 (lane / 16) + u, row 16 j + lane % 16
-  constexpr int STEP = GATED ? 2 : 1, FO = FN / STEP;  // output fragments
-  auto value = [&](int i, int j, float (&v)[4]) __attribute__((always_inline)) {
+  static constexpr int FO = FN / (GATED ? 2 : 1);  // output fragments
+  __device__ static __forceinline__ void value(const Acc& acc, int i, int j, float (&v)[4]) {
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       if constexpr (GATED) {
@@ -327,76 +378,329 @@ __global__ __launch_bounds__(64 * WM * WN) void block_mm(MmArgs a) {
         v[u] = acc[i][j][u];
       }
     }
-  };
-  const int c0 = n0 + wn * (OC / WN) + 4 * q;
-  auto out_row = [&](int r) -> int64_t {
-    if constexpr (EXPERTS) return a.scatter ? a.slot[m0 + r] : m0 + r;
-    else return m0 + r;
-  };
-  if constexpr (QUANT) {
-    // the group's largest value: over the lane's columns, the four lanes of the
-    // row, then the waves of the row through LDS
-    uint32_t* part = reinterpret_cast<uint32_t*>(lds);  // [WN][BM]
-    __syncthreads();
-    float v[FO][FM][4];
-    uint32_t am[FM];
+  }
+  __device__ static __forceinline__ int64_t out_row(const MmArgs& a, const MmTile& t, int r) {
+    if constexpr (EXPERTS) return a.scatter ? a.slot[t.m0 + r] : t.m0 + r;
+    else return t.m0 + r;
+  }
+
+  // Results of one wave: through LDS (its own part, a fragment row at a time), so that
+  // whole lines are written instead of 16 pieces of 32 bytes each -- 8192 x 8192 bf16
+  // results of 2048 features, 142 us against 157; float32, 248 against 281.
+  template <int OT>
+  __device__ static __forceinline__ void store(const MmArgs& a, const MmTile& t, const Acc& acc, int wave, int wm, int wn,
+                                               int lane, uint8_t* lds) {
+    using S = typename Elem<OT>::storage;
+    constexpr int COLS = OC / WN, PITCH = COLS * sizeof(S) + 16;  // (16: rows start on different banks)
+    constexpr int PER = 16 / sizeof(S), LANES = COLS / PER;      // results a lane stores, lanes a row
+    const int r16 = lane & 15, q = lane >> 4, c0 = t.n0 + wn * COLS;
+    const bool wide = a.out_stride % PER == 0 && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0;
+    uint8_t* mine = lds + wave * 16 * PITCH;
 #pragma unroll
     for (int j = 0; j < FM; ++j) {
-      am[j] = 0;
+      const int r0 = wm * (BM / WM) + j * 16;
+      if (t.m0 + r0 >= t.m_end) break;
 #pragma unroll
       for (int i = 0; i < FO; ++i) {
-        value(i, j, v[i][j]);
-        if (c0 + 16 * i < a.N)
-#pragma unroll
-          for (int u = 0; u < 4; ++u) am[j] = max(am[j], __builtin_bit_cast(uint32_t, v[i][j][u]) & 0x7FFFFFFFu);
+        float v[4];
+        value(acc, i, j, v);
+        S* o = reinterpret_cast<S*>(mine + r16 * PITCH) + 16 * i + 4 * q;
+        if constexpr (OT == GR_DTYPE_F32) *reinterpret_cast<mm4_t*>(o) = mm4_t{v[0], v[1], v[2], v[3]};
+        else *reinterpret_cast<u32x2_t*>(o) = u32x2_t{Mma<OT>::pack2(v[0], v[1]), Mma<OT>::pack2(v[2], v[3])};
       }
-      am[j] = max(am[j], (uint32_t)__shfl_xor((int)am[j], 16, 64));
-      am[j] = max(am[j], (uint32_t)__shfl_xor((int)am[j], 32, 64));
-      if (q == 0) part[wn * BM + wm * (BM / WM) + j * 16 + r16] = am[j];
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int e = 0; e < 16 * LANES; e += 64) {
+        const int r = (e + lane) / LANES, col = (e + lane) % LANES * PER;
+        if (16 * LANES < 64 && lane >= 16 * LANES) continue;
+        const u32x4_t d = *reinterpret_cast<const u32x4_t*>(mine + r * PITCH + col * sizeof(S));
+        if (t.m0 + r0 + r >= t.m_end || c0 + col >= a.N) continue;
+        S* o = static_cast<S*>(a.out) + out_row(a, t, r0 + r) * a.out_stride + c0 + col;
+        if (wide && c0 + col + PER <= a.N) {
+          *reinterpret_cast<u32x4_t*>(o) = d;
+        } else {
+          struct { S e[PER]; } p = __builtin_bit_cast(decltype(p), d);
+#pragma unroll
+          for (int u = 0; u < PER; ++u)
+            if (c0 + col + u < a.N) o[u] = p.e[u];
+        }
+      }
+      __builtin_amdgcn_wave_barrier();
     }
+  }
+
+  // The results; `lds` may be overwritten once every wave is here.
+  __device__ static __forceinline__ void finish(const MmArgs& a, const MmTile& t, const Acc& acc, int wave, int wm, int wn,
+                                                int lane, uint8_t* lds) {
     __syncthreads();
+    if constexpr (QUANT) {
+      // the group's largest value: over the lane's columns, the four lanes of the
+      // row, then the waves of the row through LDS
+      constexpr int PITCH = 128 + 16;
+      const int r16 = lane & 15, q = lane >> 4, c0 = wn * (OC / WN) + 4 * q;
+      uint32_t* part = reinterpret_cast<uint32_t*>(lds);  // [WN][BM]
+      uint8_t* rows = lds + WN * BM * 4;                  // [BM][PITCH]
 #pragma unroll
-    for (int j = 0; j < FM; ++j) {
-      const int r = wm * (BM / WM) + j * 16 + r16;
-      uint32_t m = 0;
+      for (int j = 0; j < FM; ++j) {
+        uint32_t m = 0;
 #pragma unroll
-      for (int k = 0; k < WN; ++k) m = max(m, part[k * BM + r]);
-      if (m0 + r >= m_end) continue;
-      const float s = quant_scale(m), rs = 1.0f / s;
-      const int64_t orow = out_row(r);
-      if (wn == 0 && q == 0) a.out_scale[orow * a.os_row + nt * a.os_grp] = s;
-      uint8_t* o = static_cast<uint8_t*>(a.out) + orow * a.out_stride;
+        for (int i = 0; i < FO; ++i) {
+          float v[4];
+          value(acc, i, j, v);
+          if (t.n0 + c0 + 16 * i < a.N)
 #pragma unroll
-      for (int i = 0; i < FO; ++i)
-        if (c0 + 16 * i < a.N) *reinterpret_cast<uint32_t*>(o + c0 + 16 * i) = quant_pack4(v[i][j], s, rs);
+            for (int u = 0; u < 4; ++u) m = max(m, __builtin_bit_cast(uint32_t, v[u]) & 0x7FFFFFFFu);
+        }
+        m = max(m, (uint32_t)__shfl_xor((int)m, 16, 64));
+        m = max(m, (uint32_t)__shfl_xor((int)m, 32, 64));
+        if (q == 0) part[wn * BM + wm * (BM / WM) + j * 16 + r16] = m;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < FM; ++j) {
+        const int r = wm * (BM / WM) + j * 16 + r16;
+        uint32_t m = 0;
+#pragma unroll
+        for (int k = 0; k < WN; ++k) m = max(m, part[k * BM + r]);
+        const float s = quant_scale(m), rs = 1.0f / s;
+        if (wn == 0 && q == 0 && t.m0 + r < t.m_end) a.out_scale[out_row(a, t, r) * a.os_row + t.nt * a.os_grp] = s;
+#pragma unroll
+        for (int i = 0; i < FO; ++i) {
+          float v[4];
+          value(acc, i, j, v);
+          *reinterpret_cast<uint32_t*>(rows + r * PITCH + c0 + 16 * i) = quant_pack4(v, s, rs);
+        }
+      }
+      __syncthreads();
+      // whole rows of 128 bytes
+      const bool wide = a.out_stride % 16 == 0 && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0;
+      const int ch = (lane & 7) * 16;
+      for (int r = wave * 8 + (lane >> 3); r < BM; r += NW * 8) {
+        if (t.m0 + r >= t.m_end || t.n0 + ch >= a.N) continue;  // (N is a multiple of 16)
+        const u32x4_t d = *reinterpret_cast<const u32x4_t*>(rows + r * PITCH + ch);
+        uint8_t* o = static_cast<uint8_t*>(a.out) + out_row(a, t, r) * a.out_stride + t.n0 + ch;
+        if (wide) {
+          *reinterpret_cast<u32x4_t*>(o) = d;
+        } else {
+#pragma unroll
+          for (int u = 0; u < 4; ++u) reinterpret_cast<uint32_t*>(o)[u] = d[u];
+        }
+      }
+    } else {
+      store_any(a, t, acc, wave, wm, wn, lane, lds);
+    }
+  }
+  __device__ static __forceinline__ void store_any(const MmArgs& a, const MmTile& t, const Acc& acc, int wave, int wm, int wn,
+                                                   int lane, uint8_t* lds) {
+    if (a.out_type == GR_DTYPE_BF16) store<GR_DTYPE_BF16>(a, t, acc, wave, wm, wn, lane, lds);
+    else if (a.out_type == GR_DTYPE_F16) store<GR_DTYPE_F16>(a, t, acc, wave, wm, wn, lane, lds);
+    else store<GR_DTYPE_F32>(a, t, acc, wave, wm, wn, lane, lds);
+  }
+};
+
+// One barrier a stage: each wave reads a stage's fragments and multiplies, ST - 1
+// stages on their way.  AHEAD (64 x 64 tiles): a stage's fragments are read while the
+// one before multiplies, from registers, and all ST buffers are on their way: 5 to 9 %
+// there (64 x 4096 by 2048 features 8.5 us against 9.0), nothing or less on larger
+// tiles, whose two sets of fragments crowd the registers.
+template <int XT, int BM, int BN, int WM, int WN, int ST, int MODE, bool EXPERTS, bool EXACT, bool AHEAD>
+__global__ __launch_bounds__(64 * WM * WN, 2) void block_mm(MmArgs a) {
+  using M = Mm<XT, BM, BN, WM, WN, MODE, EXPERTS, EXACT>;
+  static_assert((BM + BN) % (8 * M::NW) == 0 && BM + M::WBLOCKS <= M::NW * 64, "whole transfers");
+  static_assert(!M::QUANT || WN * BM * 4 + BM * 144 <= ST * M::TILE, "the epilogue's rows fit");
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[ST * (M::TILE + M::SCALES)];
+  MmTile t;
+  if (!M::tile(a, t)) return;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave / WN, wn = wave % WN;
+  typename M::Source src;
+  M::source(a, t, wave, lane, src);
+  const typename M::Lane l = M::lane_of(wm, wn, lane);
+  const uint32_t lds0 = (uint32_t)reinterpret_cast<uintptr_t>(lds);
+  const int n = __builtin_amdgcn_readfirstlane((a.kbytes + 127) >> 7);
+  auto fetch = [&](int s, int buf) __attribute__((always_inline)) {
+    M::fetch(a, src, s, lds0 + buf * M::TILE, lds0 + ST * M::TILE + buf * M::SCALES, wave);
+  };
+  typename M::Acc acc;
+#pragma unroll
+  for (int i = 0; i < M::FN; ++i)
+#pragma unroll
+    for (int j = 0; j < M::FM; ++j) acc[i][j] = mm4_t{0.f, 0.f, 0.f, 0.f};
+  if constexpr (AHEAD) {
+#pragma unroll
+    for (int s = 0; s < ST; ++s)
+      if (s < n) fetch(s, s);
+    if (ST <= n) mm_wait_barrier<(ST - 1) * M::OPS>();
+    else mm_wait_barrier<0>();
+    typename M::Frags f0, f1;
+    M::read_all(lds, lds + ST * M::TILE, l, f0);
+    int buf = 0;
+    // stage s is in registers; past the barrier its buffer is free, stage s + 1 has
+    // landed, and stages s + 2 .. s + ST - 1 may be on their way
+    auto step = [&](int s, const typename M::Frags& cur, typename M::Frags& nxt) __attribute__((always_inline)) {
+      const int next = buf + 1 == ST ? 0 : buf + 1;
+      if (s + 1 < n) {
+        if (s + ST <= n) mm_wait_barrier<(ST - 2) * M::OPS>();
+        else mm_wait_barrier<0>();
+        M::read_all(lds + next * M::TILE, lds + ST * M::TILE + next * M::SCALES, l, nxt);
+        if (s + ST < n) fetch(s + ST, buf);
+      }
+      buf = next;
+      M::mul_all(cur, acc);
+    };
+    for (int s = 0; s < n; s += 2) {
+      step(s, f0, f1);
+      if (s + 1 < n) step(s + 1, f1, f0);
     }
   } else {
-    const bool vec = a.N % 4 == 0 && a.out_stride % 4 == 0;  // whole groups of four columns, each aligned
+    // stage s has landed when all but the ST - 2 younger ones' transfers have; past
+    // its barrier nobody reads stage s - 1, whose buffer takes stage s + ST - 1
 #pragma unroll
-    for (int j = 0; j < FM; ++j) {
-      const int r = wm * (BM / WM) + j * 16 + r16;
-      if (m0 + r >= m_end) continue;
-      const int64_t o0 = out_row(r) * a.out_stride;
+    for (int s = 0; s < ST - 1; ++s)
+      if (s < n) fetch(s, s);
+    int buf = 0;
+    for (int s = 0; s < n; ++s) {
+      if (s + ST - 1 <= n) mm_wait_barrier<(ST - 2) * M::OPS>();
+      else mm_wait_barrier<0>();
+      if (s + ST - 1 < n) fetch(s + ST - 1, buf == 0 ? ST - 1 : buf - 1);
+      const uint8_t *p = lds + buf * M::TILE, *sc = lds + ST * M::TILE + buf * M::SCALES;
+      mm8i_t w[M::FN];
+      u32x4_t wh[4][EXACT ? M::FN : 1];
+      float ws[2];
+      M::read_w(p, sc, l, w, ws);
+      if constexpr (EXACT) M::convert(w, wh);
 #pragma unroll
-      for (int i = 0; i < FO; ++i) {
-        const int col = c0 + 16 * i;
-        if (col >= a.N) continue;
-        float v[4];
-        value(i, j, v);
-        mm_store(a.out, a.out_type, o0 + col, v, vec ? 4 : min(4, a.N - col), vec);
+      for (int j = 0; j < M::FM; ++j) {
+        const float xs = M::F8 ? *reinterpret_cast<const float*>(sc + l.so + j * 64) : 0.f;
+        const mm8i_t x = M::read(p + l.xo + j * 2048, l);
+        if constexpr (EXACT) M::mul_exact(wh, x, j, xs, ws[0], ws[1], acc);
+        else M::mul(w, x, j, xs, ws[0], ws[1], acc);
       }
+      buf = buf + 1 == ST ? 0 : buf + 1;
+    }
+  }
+  M::finish(a, t, acc, wave, wm, wn, lane, lds);
+}
+
+// Few rows: BM = 16 FM.  What bounds this is the weights' way from memory (or, for a
+// single projection, one round trip), so nothing is shared through LDS: every weight
+// is loaded once, by the one wave that multiplies it, straight into the registers of
+// the operand, U stages at a time, and the eight waves split the depth WK ways (wave
+// k takes stages k, k + WK, ...) and the columns 8 / WK ways, 16 columns a wave.  The
+// partial sums of the depth meet in LDS.  The rows are read by every workgroup, from L2.
+template <int XT, int FM, int WK, int MODE, bool EXPERTS>
+__global__ __launch_bounds__(512) void few_mm(MmArgs a) {
+  constexpr bool F8 = XT == GR_DTYPE_FP8_E4M3;
+  constexpr bool GATED = MODE == MM_SWIGLU || MODE == MM_SWIGLU_Q, QUANT = MODE == MM_SWIGLU_Q || MODE == MM_PLAIN_Q;
+  constexpr int WN = 8 / WK, FN = GATED ? 2 : 1, U = FM == 1 ? 4 : 2;
+  using M = Mm<XT, 16 * FM, 16 * FN * WN, 1, WN, MODE, EXPERTS, F8>;
+  using M1 = Mm<XT, 16, 16 * FN * WN, 1, WN, MODE, EXPERTS, F8>;  // one fragment row
+  static_assert(!QUANT || WK == 1, "a tile's columns are one group of the result");
+  constexpr int LDS = QUANT ? WN * 16 * FM * 4 + 16 * FM * 144 : WK * WN * FM * FN * 1024 + 8 * 16 * 80;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[LDS];
+  MmTile t;
+  if (!M::tile(a, t)) return;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wk = wave / WN, wn = wave % WN, r16 = lane & 15, q = lane >> 4;
+  const int n = (a.kbytes + 127) >> 7, nb = (a.N + 127) >> 7;
+  const int col = min(t.n0 + wn * 16 + r16, a.N - 1);
+  const uint8_t* w0 = t.w + (int64_t)col * a.w_stride + q * 16;
+  const int64_t up = (int64_t)a.N * a.w_stride;
+  const float* ws = F8 ? t.ws + (int64_t)min((t.n0 + wn * 16) >> 7, nb - 1) * n : nullptr;
+  const uint8_t* x0[FM];
+  const float* xs[FM];
+#pragma unroll
+  for (int j = 0; j < FM; ++j) {
+    const int64_t r = M::x_row(a, t, 16 * j + r16);
+    x0[j] = a.x + r * a.x_stride + q * 16;
+    xs[j] = F8 ? a.xs + r * a.xs_row : nullptr;
+  }
+  auto load = [&](const uint8_t* p, int s) __attribute__((always_inline)) {
+    mm4i_t lo = {0, 0, 0, 0}, hi = {0, 0, 0, 0};
+    if (s * 128 + q * 16 < a.kbytes) lo = *reinterpret_cast<const mm4i_t*>(p + (int64_t)s * 128);
+    if (s * 128 + 64 + q * 16 < a.kbytes) hi = *reinterpret_cast<const mm4i_t*>(p + (int64_t)s * 128 + 64);
+    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+  };
+  typename M::Acc acc;
+#pragma unroll
+  for (int i = 0; i < FN; ++i)
+#pragma unroll
+    for (int j = 0; j < FM; ++j) acc[i][j] = mm4_t{0.f, 0.f, 0.f, 0.f};
+  for (int s0 = wk; s0 < n; s0 += WK * U) {
+    mm8i_t w[U][FN], x[U][FM];
+    float sx[U][FM], sw[U][FN];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int s = s0 + u * WK;  // (past the last: zeros)
+#pragma unroll
+      for (int i = 0; i < FN; ++i) {
+        w[u][i] = load(w0 + i * up, s);
+        sw[u][i] = F8 && s < n ? ws[(int64_t)i * nb * n + s] : 0.f;
+      }
+#pragma unroll
+      for (int j = 0; j < FM; ++j) {
+        x[u][j] = load(x0[j], s);
+        sx[u][j] = F8 && s < n ? xs[j][(int64_t)s * a.xs_grp] : 0.f;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (u && s0 + u * WK >= n) break;
+      u32x4_t wh[4][F8 ? FN : 1];
+      if constexpr (F8) M::convert(w[u], wh);
+#pragma unroll
+      for (int j = 0; j < FM; ++j)
+        if constexpr (F8) M::mul_exact(wh, x[u][j], j, sx[u][j], sw[u][0], sw[u][FN - 1], acc);
+        else M::mul(w[u], x[u][j], j, 0.f, 0.f, 0.f, acc);
+    }
+  }
+  if constexpr (QUANT) {
+    M::finish(a, t, acc, wave, 0, wn, lane, lds);
+  } else {
+    mm4_t* part = reinterpret_cast<mm4_t*>(lds);  // [wave][FM][FN][64]
+#pragma unroll
+    for (int j = 0; j < FM; ++j)
+#pragma unroll
+      for (int i = 0; i < FN; ++i) part[((wave * FM + j) * FN + i) * 64 + lane] = acc[i][j];
+    __syncthreads();
+    // wave (k, n) finishes fragment rows k, k + WK, ... of column fragment n
+    for (int j = wk; j < FM; j += WK) {
+      typename M1::Acc sum;
+#pragma unroll
+      for (int i = 0; i < FN; ++i) {
+        sum[i][0] = part[((wn * FM + j) * FN + i) * 64 + lane];
+#pragma unroll
+        for (int k = 1; k < WK; ++k) {
+          const mm4_t v = part[(((k * WN + wn) * FM + j) * FN + i) * 64 + lane];
+#pragma unroll
+          for (int u = 0; u < 4; ++u) sum[i][0][u] += v[u];
+        }
+      }
+      MmTile tj = t;
+      tj.m0 += 16 * j;
+      if (tj.m0 < tj.m_end) M1::store_any(a, tj, sum, wave, 0, wn, lane, lds + WK * WN * FM * FN * 1024);
     }
   }
 }
 
 template <int XT, int BM, int BN, int WM, int WN, int ST, int MODE, bool EXPERTS, bool EXACT>
 void launch_mm(MmArgs a, int tiles_m, hipStream_t stream) {
-  constexpr int OC = MODE == MM_SWIGLU || MODE == MM_SWIGLU_Q ? BN / 2 : BN;
+  using M = Mm<XT, BM, BN, WM, WN, MODE, EXPERTS, EXACT>;
+  constexpr bool AHEAD = !EXACT && M::FM * M::FN <= 4;
+  a.tiles_m = tiles_m;
+  a.tiles_n = (a.N + M::OC - 1) / M::OC;
+  const int64_t total = (int64_t)tiles_m * a.tiles_n;
+  hipLaunchKernelGGL((block_mm<XT, BM, BN, WM, WN, ST, MODE, EXPERTS, EXACT, AHEAD>), dim3((unsigned)((total + 7) / 8 * 8)),
+                     dim3(64 * WM * WN), 0, stream, a);
+}
+
+template <int XT, int FM, int WK, int MODE, bool EXPERTS>
+void launch_few(MmArgs a, int tiles_m, hipStream_t stream) {
+  constexpr int OC = 16 * (8 / WK);
   a.tiles_m = tiles_m;
   a.tiles_n = (a.N + OC - 1) / OC;
   const int64_t total = (int64_t)tiles_m * a.tiles_n;
-  hipLaunchKernelGGL((block_mm<XT, BM, BN, WM, WN, ST, MODE, EXPERTS, EXACT>), dim3((unsigned)((total + 7) / 8 * 8)),
-                     dim3(64 * WM * WN), 0, stream, a);
+  hipLaunchKernelGGL((few_mm<XT, FM, WK, MODE, EXPERTS>), dim3((unsigned)((total + 7) / 8 * 8)), dim3(512), 0, stream, a);
 }
 
 }  // namespace

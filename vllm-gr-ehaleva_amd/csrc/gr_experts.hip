@@ -140,7 +140,7 @@ __global__ __launch_bounds__(64 * RT_WAVES) void route_experts_k(RouteArgs a) {
 }
 
 // ---- the experts' rows ---------------------------------------------------------
-constexpr int PLAN_THREADS = 1024;
+constexpr int PLAN_THREADS = 1024;  // >= MAX_EXPERTS
 constexpr int PLAN_ROWS = 8192;  // choices a workgroup sorts
 
 struct PlanArgs {
@@ -152,21 +152,6 @@ struct PlanArgs {
   int32_t* num_tiles;
   int32_t* dev_status;
 };
-
-// choices of each expert in this workgroup's part
-__global__ __launch_bounds__(PLAN_THREADS) void expert_count_k(PlanArgs a) {
-  __shared__ int n[MAX_EXPERTS];
-  if ((int)threadIdx.x < a.E) n[threadIdx.x] = 0;
-  __syncthreads();
-  const int r0 = blockIdx.x * PLAN_ROWS, r1 = min(r0 + PLAN_ROWS, a.rows);
-  for (int r = r0 + threadIdx.x; r < r1; r += PLAN_THREADS) {
-    const int e = a.ids[r];
-    if (e >= 0 && e < a.E) atomicAdd(&n[e], 1);
-    else if (e >= 0) flag_status(a.dev_status, GR_DEV_BAD_EXPERT);
-  }
-  __syncthreads();
-  if ((int)threadIdx.x < a.E) a.hist[(int64_t)blockIdx.x * a.E + threadIdx.x] = n[threadIdx.x];
-}
 
 // exclusive prefix sum over the workgroup's 1024 threads
 __device__ inline int block_excl_scan(int v, int* part) {
@@ -180,6 +165,40 @@ __device__ inline int block_excl_scan(int v, int* part) {
   return before + incl - v;
 }
 
+constexpr int PLAN_PER = PLAN_ROWS / PLAN_THREADS;
+// the workgroup's choices, PLAN_PER a thread; -1: none, or another rank's
+__device__ inline void plan_load(const PlanArgs& a, int (&e)[PLAN_PER], bool flag) {
+  const int r0 = blockIdx.x * PLAN_ROWS + threadIdx.x;
+#pragma unroll
+  for (int i = 0; i < PLAN_PER; ++i) {
+    const int r = r0 + i * PLAN_THREADS;
+    e[i] = r < a.rows ? a.ids[r] : -1;
+  }
+#pragma unroll
+  for (int i = 0; i < PLAN_PER; ++i)
+    if (e[i] >= a.E) {
+      if (flag) flag_status(a.dev_status, GR_DEV_BAD_EXPERT);
+      e[i] = -1;
+    }
+}
+__device__ inline void plan_count(const PlanArgs& a, const int (&e)[PLAN_PER], int* n) {
+  n[threadIdx.x] = 0;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < PLAN_PER; ++i)
+    if (e[i] >= 0) atomicAdd(&n[e[i]], 1);
+  __syncthreads();
+}
+
+// more choices than one workgroup sorts: how many of each expert every one of them has
+__global__ __launch_bounds__(PLAN_THREADS) void expert_count_k(PlanArgs a) {
+  __shared__ int n[MAX_EXPERTS];
+  int e[PLAN_PER];
+  plan_load(a, e, true);
+  plan_count(a, e, n);
+  if ((int)threadIdx.x < a.E) a.hist[(int64_t)blockIdx.x * a.E + threadIdx.x] = n[threadIdx.x];
+}
+
 // Sorts this workgroup's choices by expert into the rows of the experts' tiles.
 // Where a row lands within its expert differs from run to run (an atomic in LDS
 // hands out the places); its result does not.
@@ -187,15 +206,22 @@ __global__ __launch_bounds__(PLAN_THREADS) void expert_plan_k(PlanArgs a) {
   __shared__ int next[MAX_EXPERTS];
   __shared__ int part[PLAN_THREADS / 64];
   const int tid = threadIdx.x;
+  int e[PLAN_PER];
+  plan_load(a, e, a.blocks == 1);
   int total = 0, before = 0;
-  if (tid < a.E)
+  if (a.blocks == 1) {
+    plan_count(a, e, next);
+    total = next[tid];
+    __syncthreads();
+  } else if (tid < a.E) {
     for (int b = 0; b < a.blocks; ++b) {
       const int n = a.hist[(int64_t)b * a.E + tid];
       if (b < (int)blockIdx.x) before += n;
       total += n;
     }
+  }
   const int first = block_excl_scan(total, part);
-  if (tid < a.E) next[tid] = first + before;
+  next[tid] = first + before;
   if (blockIdx.x == 0) {
     const int tiles = (total + a.bm - 1) / a.bm;
     const int t0 = block_excl_scan(tiles, part);
@@ -204,11 +230,9 @@ __global__ __launch_bounds__(PLAN_THREADS) void expert_plan_k(PlanArgs a) {
     if (tid == PLAN_THREADS - 1) *a.num_tiles = t0 + tiles;
   }
   __syncthreads();
-  const int r0 = blockIdx.x * PLAN_ROWS, r1 = min(r0 + PLAN_ROWS, a.rows);
-  for (int r = r0 + tid; r < r1; r += PLAN_THREADS) {
-    const int e = a.ids[r];
-    if (e >= 0 && e < a.E) a.slot[atomicAdd(&next[e], 1)] = r;
-  }
+#pragma unroll
+  for (int i = 0; i < PLAN_PER; ++i)
+    if (e[i] >= 0) a.slot[atomicAdd(&next[e[i]], 1)] = blockIdx.x * PLAN_ROWS + i * PLAN_THREADS + tid;
 }
 
 // ---- out[t] = sum_j weights[t, j] * y[t, j] ---------------------------------------
@@ -236,19 +260,30 @@ __global__ __launch_bounds__(256) void expert_combine_k(CombineArgs a) {
     for (int u = 0; u < 4; ++u) acc[u] = fmaf(w, v[u], acc[u]);
   }
   const float v[4] = {acc[0], acc[1], acc[2], acc[3]};
-  mm_store(a.out, DT, t * a.out_stride + h, v, 4, true);
+  mm_store<DT>(a.out, t * a.out_stride + h, v);
 }
 
 // ---- workspace -----------------------------------------------------------------
-constexpr int EXPERT_BM = 64;
-
 struct Workspace {
   int64_t hist, slot, tiles, num_tiles, x8, xs, act, act_scale, y, bytes;
   int64_t max_tiles;
   int blocks;
 };
 
-Workspace plan_workspace(int T, int k, int E, int H, int F, bool fp8) {
+// Rows of a tile, by the rows an expert gets on average.  Few rows are bound by the
+// weights' way from memory: then more workgroups on a CU count, later the rows a
+// weight is read for.  Measured (64 experts of 768 features, hidden 2048, 8 of them a
+// token; us, by tile rows; 16-bit weights, then e4m3):
+//   rows an expert   1             8              32              64              256             1024
+//   16 / 64        86 / 96      145 / 143      285 / 159        - / 190         - / 432         -
+//   128 / 256     105 / 120     162 / 186      172 / 190       197 / 213       300 / 322     934 / 867
+//   32 / 128       61 / 78       82 / 124      104 / 132       126 / 147      (280 at 128)    - / 920
+int expert_tile_rows(int64_t rows, int E, bool fp8) {
+  if (fp8) return rows <= 112ll * E ? 32 : 128;
+  return rows <= 4ll * E ? 16 : rows <= 80ll * E ? 64 : rows <= 512ll * E ? 128 : 256;
+}
+
+Workspace plan_workspace(int T, int k, int E, int H, int F, bool fp8, int bm) {
   Workspace w{};
   const int64_t rows = (int64_t)T * k;
   auto take = [&](int64_t bytes) {
@@ -257,7 +292,7 @@ Workspace plan_workspace(int T, int k, int E, int H, int F, bool fp8) {
     return at;
   };
   w.blocks = (int)((rows + PLAN_ROWS - 1) / PLAN_ROWS);
-  w.max_tiles = rows / EXPERT_BM + (rows < E ? rows : E);
+  w.max_tiles = rows / bm + (rows < E ? rows : E);
   w.num_tiles = take(4);
   w.hist = take(4ll * w.blocks * E);
   w.slot = take(4 * rows);
@@ -275,11 +310,31 @@ Workspace plan_workspace(int T, int k, int E, int H, int F, bool fp8) {
 }
 
 template <int XT>
-void launch_experts(MmArgs up, MmArgs down, int tiles, hipStream_t stream) {
-  constexpr bool F8 = XT == GR_DTYPE_FP8_E4M3;
-  launch_mm<XT, EXPERT_BM, 256, 2, 4, 3, F8 ? MM_SWIGLU_Q : MM_SWIGLU, true, F8>(up, tiles, stream);
-  // (its float32 results are summed into one of 16 bits)
-  launch_mm<XT, EXPERT_BM, 256, 2, 4, 3, MM_PLAIN, true, false>(down, tiles, stream);
+void launch_experts(const MmArgs& up, const MmArgs& down, int tiles, int bm, hipStream_t stream) {
+  if constexpr (XT == GR_DTYPE_FP8_E4M3) {
+    // (down's float32 results are summed into 16 bits: the 8-bit instruction will do)
+    if (bm == 32) {
+      launch_mm<XT, 32, 256, 1, 4, 2, MM_SWIGLU_Q, true, true>(up, tiles, stream);
+      launch_mm<XT, 32, 128, 1, 4, 3, MM_PLAIN, true, false>(down, tiles, stream);
+    } else {
+      launch_mm<XT, 128, 256, 2, 4, 3, MM_SWIGLU_Q, true, true>(up, tiles, stream);
+      launch_mm<XT, 128, 128, 2, 2, 2, MM_PLAIN, true, false>(down, tiles, stream);
+    }
+  } else {
+    if (bm == 16) {
+      launch_few<XT, 1, 8, MM_SWIGLU, true>(up, tiles, stream);
+      launch_few<XT, 1, 8, MM_PLAIN, true>(down, tiles, stream);
+    } else if (bm == 64) {
+      launch_mm<XT, 64, 64, 2, 2, 4, MM_SWIGLU, true, false>(up, tiles, stream);
+      launch_mm<XT, 64, 64, 2, 2, 4, MM_PLAIN, true, false>(down, tiles, stream);
+    } else if (bm == 128) {
+      launch_mm<XT, 128, 256, 2, 4, 3, MM_SWIGLU, true, false>(up, tiles, stream);
+      launch_mm<XT, 128, 256, 2, 4, 3, MM_PLAIN, true, false>(down, tiles, stream);
+    } else {
+      launch_mm<XT, 256, 256, 2, 4, 2, MM_SWIGLU, true, false>(up, tiles, stream);
+      launch_mm<XT, 256, 256, 2, 4, 2, MM_PLAIN, true, false>(down, tiles, stream);
+    }
+  }
 }
 
 template <int DT>
@@ -319,7 +374,8 @@ extern "C" gr_status_t gr_route_experts(float* weights, int32_t* ids, const void
 extern "C" size_t gr_expert_mlp_workspace_size(int num_tokens, int top_k, int num_experts, int hidden, int ffn,
                                                int fp8) {
   if (num_tokens < 1 || top_k < 1 || num_experts < 1 || hidden < 1 || ffn < 1) return 0;
-  return (size_t)plan_workspace(num_tokens, top_k, num_experts, hidden, ffn, fp8 != 0).bytes;
+  const int bm = expert_tile_rows((int64_t)num_tokens * top_k, num_experts, fp8 != 0);
+  return (size_t)plan_workspace(num_tokens, top_k, num_experts, hidden, ffn, fp8 != 0, bm).bytes;
 }
 
 extern "C" gr_status_t gr_expert_mlp(void* out, int64_t out_stride, const void* x, int64_t x_stride,
@@ -336,22 +392,24 @@ extern "C" gr_status_t gr_expert_mlp(void* out, int64_t out_stride, const void* 
     return GR_ERR_INVALID_ARG;
   const bool fp8 = gate_up_scale != nullptr;
   const int T = num_tokens, H = hidden, F = ffn;
-  if (dtype == GR_DTYPE_F32 || hidden % 16 != 0 || ffn % 16 != 0 || hidden > (1 << 24) || ffn > (1 << 24) ||
+  if (dtype == GR_DTYPE_F32 || hidden % 16 != 0 || ffn % 16 != 0 || hidden > (1 << 21) || ffn > (1 << 21) ||
       num_experts > MAX_EXPERTS || (int64_t)T * top_k > (1 << 26) || !aligned(x, 16) || x_stride % 8 != 0 ||
       !aligned(gate_up, 16) || !aligned(down, 16) || !aligned(out, 8) || out_stride % 4 != 0 ||
-      (fp8 && (!aligned(gate_up_scale, 4) || !aligned(down_scale, 4))))
+      (fp8 && (!aligned(gate_up_scale, 4) || !aligned(down_scale, 4))) || (int64_t)T * x_stride > (1 << 30) - (1 << 24) ||
+      (fp8 && (int64_t)T * H > (1ll << 31) - (1 << 24)))
     return GR_ERR_UNSUPPORTED;
-  const Workspace l = plan_workspace(T, top_k, num_experts, H, F, fp8);
+  const int bm = expert_tile_rows((int64_t)T * top_k, num_experts, fp8);
+  const Workspace l = plan_workspace(T, top_k, num_experts, H, F, fp8, bm);
   if (l.max_tiles * ((2ll * F + 15) / 16) > INT32_MAX - 8 || l.max_tiles * ((H + 15) / 16) > INT32_MAX - 8)
     return GR_ERR_UNSUPPORTED;
   if (!workspace || !aligned(workspace, 256) || workspace_bytes < (size_t)l.bytes) return GR_ERR_WORKSPACE;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   const int rows = T * top_k, hb = (H + 127) / 128, fb = (F + 127) / 128;
 
-  PlanArgs p{ids, rows, num_experts, EXPERT_BM, l.blocks, reinterpret_cast<int32_t*>(ws + l.hist),
+  PlanArgs p{ids, rows, num_experts, bm, l.blocks, reinterpret_cast<int32_t*>(ws + l.hist),
              reinterpret_cast<int32_t*>(ws + l.slot), reinterpret_cast<int4*>(ws + l.tiles),
              reinterpret_cast<int32_t*>(ws + l.num_tiles), dev_status};
-  hipLaunchKernelGGL(expert_count_k, dim3(l.blocks), dim3(PLAN_THREADS), 0, stream, p);
+  if (l.blocks > 1) hipLaunchKernelGGL(expert_count_k, dim3(l.blocks), dim3(PLAN_THREADS), 0, stream, p);
   hipLaunchKernelGGL(expert_plan_k, dim3(l.blocks), dim3(PLAN_THREADS), 0, stream, p);
 
   const int esize = fp8 ? 1 : 2;
@@ -409,9 +467,9 @@ extern "C" gr_status_t gr_expert_mlp(void* out, int64_t out_stride, const void* 
     dn.ws_expert = (int64_t)hb * fb;
   }
   const int tiles = (int)l.max_tiles;
-  if (fp8) launch_experts<GR_DTYPE_FP8_E4M3>(up, dn, tiles, stream);
-  else if (dtype == GR_DTYPE_BF16) launch_experts<GR_DTYPE_BF16>(up, dn, tiles, stream);
-  else launch_experts<GR_DTYPE_F16>(up, dn, tiles, stream);
+  if (fp8) launch_experts<GR_DTYPE_FP8_E4M3>(up, dn, tiles, bm, stream);
+  else if (dtype == GR_DTYPE_BF16) launch_experts<GR_DTYPE_BF16>(up, dn, tiles, bm, stream);
+  else launch_experts<GR_DTYPE_F16>(up, dn, tiles, bm, stream);
 
   const CombineArgs c{out, out_stride, reinterpret_cast<const float*>(ws + l.y), weights, ids, T, top_k,
                       num_experts, H};

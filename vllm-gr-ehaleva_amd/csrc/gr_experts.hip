@@ -23,119 +23,311 @@ struct RouteArgs {
   float scale;
 };
 
-__device__ inline double wave_max_f64(double v) {
+// Reductions over each L neighbouring lanes, the result in all of them: within a row
+// of 16 by DPP moves (the xor of 1 and of 2, then mirrors of 8 and of 16, whose halves
+// agree in themselves by then).
+template <typename F> __device__ __forceinline__ uint32_t seg_step(uint32_t v, int step, F f) {
+  switch (step) {
+    case 1: return f(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xf, 0xf, true));
+    case 2: return f(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xf, 0xf, true));
+    case 4: return f(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xf, 0xf, true));
+    case 8: return f(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x140, 0xf, 0xf, true));
+    default: return f(v, (uint32_t)__shfl_xor((int)v, step, 64));
+  }
+}
+template <int L, typename F> __device__ __forceinline__ uint32_t seg_all(uint32_t v, F f) {
 #pragma unroll
-  for (int off = 32; off > 0; off >>= 1) v = fmax(v, __shfl_xor(v, off, 64));
+  for (int step = 1; step < L; step *= 2) v = seg_step(v, step, f);
   return v;
 }
-__device__ inline double wave_sum_f64(double v) {
+template <int L> __device__ __forceinline__ uint32_t seg_max(uint32_t v) {
+  return seg_all<L>(v, [](uint32_t a, uint32_t b) { return max(a, b); });
+}
+template <int L> __device__ __forceinline__ uint64_t seg_max(uint64_t k) {
+  const uint32_t hi = seg_max<L>((uint32_t)(k >> 32));
+  return (uint64_t)hi << 32 | seg_max<L>((uint32_t)(k >> 32) == hi ? (uint32_t)k : 0u);
+}
+template <int L> __device__ __forceinline__ float seg_sum(float v) {
+  return __uint_as_float(seg_all<L>(__float_as_uint(v), [](uint32_t a, uint32_t b) {
+    return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
+  }));
+}
+template <int L> __device__ __forceinline__ double seg_sum(double v) {
 #pragma unroll
-  for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
+  for (int step = 1; step < L; step *= 2) v += __shfl_xor(v, step, 64);
   return v;
 }
-// (v, i) before (w, j): larger value first, then lower index; a NaN after everything
-__device__ inline bool ranks_before(double v, int i, double w, int j) {
-  const bool vn = v != v, wn = w != w;
-  if (vn || wn) return vn == wn ? i < j : wn;
-  return v > w || (v == w && i < j);
+// Keys that rank as the values do: a NaN's is 1, 0 is left for what cannot be chosen.
+__device__ __forceinline__ uint32_t rank_key(float v) {
+  const uint32_t b = __float_as_uint(v + 0.0f);  // (-0 as 0)
+  return v != v ? 1u : (int32_t)b < 0 ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ uint64_t rank_key(double v) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, v + 0.0);
+  return v != v ? 1u : (int64_t)b < 0 ? ~b : b | (1ull << 63);
+}
+__device__ __forceinline__ float rank_value(uint32_t k) {
+  return k <= 1 ? NAN : __uint_as_float((k >> 31) ? k & 0x7FFFFFFFu : ~k);
+}
+// a before b in rank (a NaN after everything)
+template <typename T> __device__ __forceinline__ bool better(T a, T b) { return a > b || (b != b && a == a); }
+
+__device__ __forceinline__ void wave_sync() {  // LDS written by this wave is read by other lanes of it
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
 }
 
-// Expert i * 64 + lane in slot i of each lane.
-template <int DT, int PER>
+// One row's logits (experts l * PER .. of it in lane l of its L lanes) and what its
+// scores need.
+template <int PER> struct RouteRow {
+  float x[PER];  // -inf past the last
+  float mx;      // softmax: the largest
+  bool nan;      // softmax: every score is NaN (a NaN or +inf among the logits)
+};
+// A wave's room in LDS, by token: c of the experts, the groups' values and whether they
+// are kept, the choices and their scores.
+template <int PER, int L> struct RouteRoom {
+  double c[64 / L][L * PER > 64 ? L * PER : 64];
+  double group[64 / L][64];
+  uint64_t kept[64 / L];
+  int id[64 / L][64];
+};
+
+template <int PER, int L> __device__ __forceinline__ double route_sum(const RouteRow<PER>& r) {
+  double sum = 0.0;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) sum += r.x[i] == -INFINITY ? 0.0 : exp((double)r.x[i] - r.mx);
+  return seg_sum<L>(sum);
+}
+template <int PER>
+__device__ __forceinline__ double route_score(const RouteArgs& a, const RouteRow<PER>& r, float v, double sum) {
+  if (a.score == GR_SCORE_SIGMOID) return 1.0 / (1.0 + exp(-(double)v));
+  if (r.nan) return NAN;
+  return v == -INFINITY ? 0.0 : exp((double)v - r.mx) / sum;
+}
+
+// The k choices of each of the wave's rows, into room.id.  T: the type in which c is
+// compared.  CHECK (float c of scores plus bias): two that had to be told apart are
+// unsure where they are not further from each other than their error may be; float32
+// scores are within 2^-22 (__expf's relative error grows with its argument, its share
+// of a score shrinks faster), the sum with the bias adds a rounding.  `order`: choices
+// are unsure; then the list goes on (`listed` entries) until the next is surely worse.
+// `groups`: which groups are kept is.
+struct RouteDoubt { bool order, groups; int listed; };
+template <int PER, int L, bool CHECK, typename T>
+__device__ __forceinline__ RouteDoubt route_choose(const RouteArgs& a, const T (&c)[PER], RouteRoom<PER, L>& room) {
+  using U = decltype(rank_key(T()));
+  const int lane = threadIdx.x & 63, l = lane % L, tok = lane / L, e0 = l * PER;
+  auto apart = [](T p, T q, float times) { return fabs(p - q) > times * (0x1p-19f + (fabs(p) + fabs(q)) * 0x1p-22f); };
+  RouteDoubt doubt{false, false, a.k};
+  U key[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) key[i] = e0 + i < a.E ? rank_key(c[i]) : U(0);
+  if (a.groups > 1) {
+    T *mine = reinterpret_cast<T*>(room.c[tok]), *value = reinterpret_cast<T*>(room.group[tok]);
+    const int n = a.E / a.groups;
+    auto add = [](T d, T& b0, T& b1) __attribute__((always_inline)) {  // the two best
+      const bool first = better(d, b0);
+      const T rest = first ? b0 : d;
+      b0 = first ? d : b0;
+      b1 = better(rest, b1) ? rest : b1;
+    };
+    auto of = [&](T b0, T b1) { return a.bias && n > 1 ? b0 + b1 : b0; };
+    // how group g ranks: groups ahead of it, and (CHECK) whether that is sure
+    auto rank = [&](int g, T v) __attribute__((always_inline)) {
+      int before = 0;
+      T next = NAN;  // the next worse value, where this group is the last that is kept
+#pragma unroll 4
+      for (int h = 0; h < a.groups; ++h) {
+        const T w = value[h];
+        const bool ahead = h != g && (better(w, v) || (h < g && !better(v, w)));
+        before += ahead ? 1 : 0;
+        if (CHECK && h != g && !ahead) next = better(w, next) ? w : next;
+      }
+      if (CHECK && before == a.top_groups - 1 && a.top_groups < a.groups) doubt.groups = !apart(v, next, 2.f);
+      return before < a.top_groups;
+    };
+    wave_sync();
+    const int span = n / PER;
+    if (n % PER == 0 && span <= L && (span & (span - 1)) == 0) {
+      // a group is whole lanes, a power of two of them (and the groups fill the lanes from
+      // the first on): its two best from registers
+      T b0 = NAN, b1 = NAN;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) add(c[i], b0, b1);
+      for (int step = 1; step < span; step *= 2) {
+        const T o0 = __shfl_xor(b0, step, 64), o1 = __shfl_xor(b1, step, 64);
+        add(o0, b0, b1);
+        add(o1, b0, b1);
+      }
+      const int g = l / span;
+      const T v = of(b0, b1);
+      if (l % span == 0 && g < a.groups) value[g] = v;
+      wave_sync();
+      if (g < a.groups && !rank(g, v))
+#pragma unroll
+        for (int i = 0; i < PER; ++i) key[i] = 0;
+    } else {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) mine[e0 + i] = c[i];
+      if (l == 0) room.kept[tok] = 0;
+      wave_sync();
+      for (int g = l; g < a.groups; g += L) {  // a lane scans whole groups, from its own place in them: its own banks
+        T b0 = NAN, b1 = NAN;
+        int at = g % n;
+#pragma unroll 4
+        for (int i = 0; i < n; ++i) {
+          add(mine[g * n + at], b0, b1);
+          at = at + 1 == n ? 0 : at + 1;
+        }
+        value[g] = of(b0, b1);
+      }
+      wave_sync();
+      for (int g = l; g < a.groups; g += L)
+        if (rank(g, value[g])) atomicOr(reinterpret_cast<unsigned long long*>(&room.kept[tok]), 1ull << g);
+      wave_sync();
+      const uint64_t kept = room.kept[tok];
+      int ge = e0 / n, re = e0 - ge * n;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        if (e0 + i < a.E && !(kept >> ge & 1)) key[i] = 0;
+        if (++re == n) {
+          re = 0;
+          ++ge;
+        }
+      }
+    }
+  }
+  T prev = 0;
+  bool open = true;  // CHECK: the list goes on
+  for (int j = 0; CHECK ? __ballot(open) != 0 : j < a.k; ++j) {
+    U best = key[0];
+#pragma unroll
+    for (int i = 1; i < PER; ++i) best = max(best, key[i]);
+    const U top = seg_max<L>(best);
+    if constexpr (CHECK) {
+      const T now = rank_value(top);
+      const bool near = j > 0 && !apart(prev, now, 1.f);
+      open = open && j < 64 && top != 0 && (j < a.k || near);
+      doubt.order |= open && near;
+      doubt.listed = open ? j + 1 : doubt.listed;
+      prev = now;
+    }
+    // the first lane that has it, and its first slot: the lowest index
+    const uint64_t mates = __ballot(best == top) >> (tok * L);
+    const bool win = l == __builtin_ctzll(mates) && open;
+    int at = 0;
+    bool found = false;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const bool hit = key[i] == top && !found;
+      found |= hit;
+      at = hit ? i : at;
+      key[i] = hit && win ? U(0) : key[i];
+    }
+    if (win) room.id[tok][j] = e0 + at;
+  }
+  if (CHECK && doubt.listed == 64 && a.k < 64) doubt.groups = true;  // (a list that did not end)
+  return doubt;
+}
+
+// L lanes a token, PER neighbouring experts a lane: a choice is one maximum over the L
+// lanes, and among equal keys the first lane's first slot is the lowest index.  Without
+// a bias the logits themselves rank.  With one, float32 sums of nearly equal ones could
+// come out in the wrong order: they are tried first, and where two of them are too close
+// to tell, the listed ones (groups: all) are ranked again in float64.
+// Bound by instructions where there are many tokens: a choice costs its reduction and a
+// few for each slot, so tokens share a wave (8 slots a lane: 8192 tokens of 256 experts
+// in 8 groups, k = 8, with a bias 18.9 us; 16 slots 24.7, as a row that is done again is
+// its wave's whole time; a wave a token, 4 slots a lane, all in float64 20.7; 8192 of 64
+// without a bias 5.7).  Few tokens take the shorter chain of 4 slots (8 of 64: 3.8).
+template <int DT, int PER, int L>
 __global__ __launch_bounds__(64 * RT_WAVES) void route_experts_k(RouteArgs a) {
   using E = Elem<DT>;
   using S = typename E::storage;
-  __shared__ double ch[RT_WAVES][64 * PER];
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int64_t t = (int64_t)blockIdx.x * RT_WAVES + wave;
-  if (t >= a.T) return;  // no barrier below: a wave works on its own
+  __shared__ RouteRoom<PER, L> rooms[RT_WAVES];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, l = lane % L, e0 = l * PER;
+  const int64_t t0 = ((int64_t)blockIdx.x * RT_WAVES + wave) * (64 / L);
+  if (t0 >= a.T) return;  // no barrier below: a wave works on its own
+  const int64_t t = min(t0 + lane / L, (int64_t)a.T - 1);  // (past the last token: it again, not stored)
+  const bool real = t0 + lane / L < a.T;
+  RouteRoom<PER, L>& room = rooms[wave];
   const S* row = static_cast<const S*>(a.logits) + t * a.stride;
-  double s[PER], c[PER];
-  double mx = -INFINITY;
+  const bool softmax = a.score == GR_SCORE_SOFTMAX;
+  RouteRow<PER> r;
+  r.mx = -INFINITY;
+  bool odd = false;
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
-    const int e = i * 64 + lane;
-    s[i] = e < a.E ? (double)E::to_float(row[e]) : -INFINITY;
-    c[i] = s[i];
-    mx = fmax(mx, s[i]);
+    r.x[i] = e0 + i < a.E ? E::to_float(row[e0 + i]) : -INFINITY;
+    r.mx = fmaxf(r.mx, r.x[i]);
+    odd |= r.x[i] != r.x[i];
   }
-  if (a.score == GR_SCORE_SOFTMAX) {
-    mx = wave_max_f64(mx);
-    double sum = 0.0;
+  r.nan = false;
+  if (softmax) {
+    r.mx = rank_value(seg_max<L>(rank_key(r.mx)));
+    r.nan = seg_max<L>(odd ? 1u : 0u) != 0 || r.mx == INFINITY;
+  }
+  if (!a.bias) {
+    route_choose<PER, L, false>(a, r.x, room);
+  } else {
+    float bias[PER], c[PER], sum = 0.f;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      s[i] = mx == -INFINITY && s[i] == -INFINITY ? 0.0 : exp(s[i] - mx);
-      sum += i * 64 + lane < a.E ? s[i] : 0.0;
+      bias[i] = e0 + i < a.E ? a.bias[e0 + i] : 0.f;
+      c[i] = softmax ? __expf(r.x[i] - r.mx) : __builtin_amdgcn_rcpf(1.0f + __expf(-r.x[i]));
+      sum += c[i];
     }
-    sum = wave_sum_f64(sum);
+    const float inv = softmax ? 1.0f / seg_sum<L>(sum) : 1.0f;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) s[i] = sum == 0.0 ? 0.0 : s[i] / sum;
-  } else {
+    for (int i = 0; i < PER; ++i) c[i] = fmaf(c[i], inv, bias[i]);
+    const RouteDoubt doubt = route_choose<PER, L, true>(a, c, room);
+    if (__ballot(doubt.groups || (softmax && (doubt.order || r.nan || r.mx == -INFINITY)))) {
+      const double all = softmax ? route_sum<PER, L>(r) : 1.0;
+      double d[PER];
 #pragma unroll
-    for (int i = 0; i < PER; ++i) s[i] = 1.0 / (1.0 + exp(-s[i]));
-  }
-  if (a.bias)
+      for (int i = 0; i < PER; ++i) d[i] = route_score(a, r, r.x[i], all) + (double)bias[i];
+      route_choose<PER, L, false>(a, d, room);
+    } else if (__ballot(doubt.order)) {
+      const int tok = lane / L, m = doubt.listed;
+      double* v = room.c[tok];
+      int* id = room.id[tok];
+      wave_sync();
+      for (int j = l; j < m; j += L) v[j] = route_score(a, r, E::to_float(row[id[j]]), 1.0) + (double)a.bias[id[j]];
+      wave_sync();
+      int to[64 / L], was[64 / L];
 #pragma unroll
-    for (int i = 0; i < PER; ++i)
-      if (i * 64 + lane < a.E) c[i] = s[i] + (double)a.bias[i * 64 + lane];
-  uint32_t open = 0;  // experts of this lane that may still be chosen
-#pragma unroll
-  for (int i = 0; i < PER; ++i)
-    if (i * 64 + lane < a.E) open |= 1u << i;
-  if (a.groups > 1) {
-    double* mine = ch[wave];
-#pragma unroll
-    for (int i = 0; i < PER; ++i) mine[i * 64 + lane] = c[i];
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    const int n = a.E / a.groups;
-    double v = NAN;
-    if (lane < a.groups) {
-      double b0 = NAN, b1 = NAN;
-      for (int i = 0; i < n; ++i) {
-        const double d = mine[lane * n + i];
-        if (i == 0 || ranks_before(d, 0, b0, 1)) { b1 = b0; b0 = d; }
-        else if (i == 1 || ranks_before(d, 0, b1, 1)) b1 = d;
+      for (int q = 0; q < 64 / L; ++q) {
+        const int j = l + q * L;
+        to[q] = 64;
+        if (j >= m) continue;
+        to[q] = 0;
+        was[q] = id[j];
+        for (int h = 0; h < m; ++h)
+          to[q] += better(v[h], v[j]) || (!better(v[j], v[h]) && id[h] < was[q]) ? 1 : 0;
       }
-      v = a.bias && n > 1 ? b0 + b1 : b0;
-    }
-    int before = 0;
-    for (int g = 0; g < a.groups; ++g) {
-      const double w = __shfl(v, g, 64);
-      before += ranks_before(w, g, v, lane) ? 1 : 0;
-    }
-    const uint64_t kept = __ballot(lane < a.groups && before < a.top_groups);
+      wave_sync();
 #pragma unroll
-    for (int i = 0; i < PER; ++i)
-      if ((open >> i & 1) && !(kept >> ((i * 64 + lane) / n) & 1)) open &= ~(1u << i);
+      for (int q = 0; q < 64 / L; ++q)
+        if (to[q] < a.k) id[to[q]] = was[q];
+    }
   }
-  double total = 0.0, mine_s = 0.0;
-  int mine_e = 0;
-  for (int j = 0; j < a.k; ++j) {
-    // this lane's best, then the wave's
-    double bv = NAN, bs = 0.0;
-    int be = 1 << 30;
-#pragma unroll
-    for (int i = 0; i < PER; ++i)
-      if ((open >> i & 1) && (be == 1 << 30 || ranks_before(c[i], i * 64 + lane, bv, be))) {
-        bv = c[i];
-        bs = s[i];
-        be = i * 64 + lane;
-      }
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) {
-      const double ov = __shfl_xor(bv, off, 64), os = __shfl_xor(bs, off, 64);
-      const int oe = __shfl_xor(be, off, 64);
-      if (oe != 1 << 30 && (be == 1 << 30 || ranks_before(ov, oe, bv, be))) { bv = ov; bs = os; be = oe; }
-    }
-    if ((be & 63) == lane) open &= ~(1u << (be >> 6));
-    if (lane == j) { mine_s = bs; mine_e = be; }
-    total += bs;
+  wave_sync();
+  // the chosen ones' scores, in float64 (a renormalised weight needs no sum of all)
+  const double all = softmax && !a.renorm ? route_sum<PER, L>(r) : 1.0;
+  const int* id = room.id[lane / L];
+  double total = 0.0;
+  for (int j = l; j < a.k; j += L) {
+    const double s = route_score(a, r, E::to_float(row[id[j]]), all);
+    room.c[lane / L][j] = s;  // (read by this lane alone)
+    total += s;
   }
-  if (lane < a.k) {
-    const double w = a.renorm ? (total == 0.0 ? 0.0 : mine_s / total) : mine_s;
-    a.weights[t * a.k + lane] = (float)(w * (double)a.scale);
-    a.ids[t * a.k + lane] = mine_e;
+  total = a.renorm ? seg_sum<L>(total) : 1.0;
+  if (!real) return;
+  for (int j = l; j < a.k; j += L) {
+    const double s = room.c[lane / L][j];
+    a.weights[t * a.k + j] = (float)((total == 0.0 ? 0.0 : s / total) * (double)a.scale);
+    a.ids[t * a.k + j] = id[j];
   }
 }
 
@@ -337,12 +529,28 @@ void launch_experts(const MmArgs& up, const MmArgs& down, int tiles, int bm, hip
   }
 }
 
-template <int DT>
-void launch_route(const RouteArgs& a, hipStream_t stream) {
-  const dim3 grid((unsigned)((a.T + RT_WAVES - 1) / RT_WAVES)), block(64 * RT_WAVES);
-  if (a.E <= 64) hipLaunchKernelGGL((route_experts_k<DT, 1>), grid, block, 0, stream, a);
-  else if (a.E <= 256) hipLaunchKernelGGL((route_experts_k<DT, 4>), grid, block, 0, stream, a);
-  else hipLaunchKernelGGL((route_experts_k<DT, 16>), grid, block, 0, stream, a);
+template <int DT, int PER, int L> void launch_route_k(const RouteArgs& a, hipStream_t stream) {
+  constexpr int PER_WG = RT_WAVES * (64 / L);
+  hipLaunchKernelGGL((route_experts_k<DT, PER, L>), dim3((unsigned)(((int64_t)a.T + PER_WG - 1) / PER_WG)),
+                     dim3(64 * RT_WAVES), 0, stream, a);
+}
+template <int DT> void launch_route(const RouteArgs& a, hipStream_t stream) {
+  const int64_t lanes4 = (int64_t)a.T * a.E / 4;  // with 4 slots a lane
+  if (a.E <= 256 && lanes4 <= 64 * 1024) {        // at most a wave for each of the 1024 SIMDs
+    if (a.E <= 64) launch_route_k<DT, 4, 16>(a, stream);
+    else if (a.E <= 128) launch_route_k<DT, 4, 32>(a, stream);
+    else launch_route_k<DT, 4, 64>(a, stream);
+  } else if (a.E <= 64) {
+    launch_route_k<DT, 8, 8>(a, stream);
+  } else if (a.E <= 128) {
+    launch_route_k<DT, 8, 16>(a, stream);
+  } else if (a.E <= 256) {
+    launch_route_k<DT, 8, 32>(a, stream);
+  } else if (a.E <= 512) {
+    launch_route_k<DT, 8, 64>(a, stream);
+  } else {
+    launch_route_k<DT, 16, 64>(a, stream);
+  }
 }
 
 bool aligned(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }

@@ -43,7 +43,8 @@ def _ptr(t: torch.Tensor | None) -> int | None:
 
 
 def _stream(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    # the handle alone: a torch.cuda.Stream object around it costs 2 us a call
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 def _dtype_code(t: torch.Tensor) -> int:
@@ -758,7 +759,7 @@ def _row_scales(name: str, t: torch.Tensor, rows: int, features: int) -> None:
 def _new_row_scales(rows: int, features: int, dev) -> torch.Tensor:
     """Scales of quantised rows, a group's scales of all rows side by side (the
     order in which the product reads them)."""
-    return torch.empty((_blocks(features), rows), dtype=torch.float32, device=dev).t()
+    return torch.empty_strided((rows, _blocks(features)), (1, max(rows, 1)), dtype=torch.float32, device=dev)
 
 
 def quant_fp8(x: torch.Tensor, *, out: torch.Tensor | None = None, scale: torch.Tensor | None = None):
@@ -771,12 +772,14 @@ def quant_fp8(x: torch.Tensor, *, out: torch.Tensor | None = None, scale: torch.
     T, K = x.shape
     if out is None:
         out = torch.empty((T, K), dtype=torch.float8_e4m3fn, device=dev)
-    _rows("out", out)
-    if out.shape != x.shape or out.dtype != torch.float8_e4m3fn:
-        raise ValueError("out must be a float8_e4m3fn tensor of x's shape")
+    else:
+        _rows("out", out)
+        if out.shape != x.shape or out.dtype != torch.float8_e4m3fn:
+            raise ValueError("out must be a float8_e4m3fn tensor of x's shape")
     if scale is None:
         scale = _new_row_scales(T, K, dev)
-    _row_scales("scale", scale, T, K)
+    else:
+        _row_scales("scale", scale, T, K)
     with _on(dev):
         code = _C.lib().gr_quant_fp8(out.data_ptr(), _row_stride(out), scale.data_ptr(), scale.stride(0), scale.stride(1),
                                      x.data_ptr(), _row_stride(x), T, K, _dtype_code(x), _stream(dev))
@@ -811,15 +814,16 @@ def linear_fp8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale:
     odt = torch.float8_e4m3fn if quantized else out_dtype
     if out is None:
         out = torch.empty((T, N), dtype=odt, device=dev)
-    _rows("out", out)
-    if out.shape != (T, N) or out.dtype != odt:
-        raise ValueError("out must be [tokens, out_features] of the result's type")
-    if quantized and out_scale is None:
-        out_scale = _new_row_scales(T, N, dev)
+    else:
+        _rows("out", out)
+        if out.shape != (T, N) or out.dtype != odt:
+            raise ValueError("out must be [tokens, out_features] of the result's type")
     if out_scale is not None:
         if not quantized:
             raise ValueError("out_scale goes with quantized=True")
         _row_scales("out_scale", out_scale, T, N)
+    elif quantized:
+        out_scale = _new_row_scales(T, N, dev)
     with _on(dev):
         code = _C.lib().gr_linear_fp8(
             out.data_ptr(), _row_stride(out), _ptr(out_scale), *(out_scale.stride() if quantized else (0, 0)),
@@ -900,9 +904,10 @@ def expert_mlp(x: torch.Tensor, gate_up: torch.Tensor, down: torch.Tensor, weigh
         raise ValueError("ids must name at least one expert a token")
     if out is None:
         out = torch.empty((T, H), dtype=x.dtype, device=dev)
-    _rows("out", out)
-    if out.shape != x.shape or out.dtype != x.dtype:
-        raise ValueError("out must match x")
+    else:
+        _rows("out", out)
+        if out.shape != x.shape or out.dtype != x.dtype:
+            raise ValueError("out must match x")
     need = expert_mlp_workspace_bytes(T, k, E, H, F, fp8)
     if workspace is None:
         workspace = torch.empty(need, dtype=torch.uint8, device=dev)

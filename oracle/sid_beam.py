@@ -59,9 +59,13 @@ def _rope(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> torch.Tensor
     return torch.cat((x1 * c - x2 * s, x2 * c + x1 * s), dim=-1)
 
 
-def decoder_logits(w: dict, cfg, tokens) -> torch.Tensor:
+def decoder_logits(w: dict, cfg, tokens, linear=None, mlp=None) -> torch.Tensor:
     """``w``: float64 weights (``weights_f64``); returns float64 ``[n, V]``
-    (the arithmetic follows the weights' dtype)."""
+    (the arithmetic follows the weights' dtype).  ``linear(h, name)`` stands for a
+    layer's product with ``w[name]``, ``mlp(h, prefix)`` for its whole MLP, where a
+    model has others than the plain ones."""
+    if linear is None:
+        linear = lambda h, name: h @ w[name].T
     n, D = len(tokens), cfg.head_dim
     Hq, Hkv = cfg.num_heads, cfg.num_kv_heads
     G = Hq // Hkv
@@ -75,7 +79,7 @@ def decoder_logits(w: dict, cfg, tokens) -> torch.Tensor:
     for i in range(cfg.num_layers):
         p = f"layers.{i}."
         h = _rms(x, w[p + "input_norm"], cfg.rms_eps)
-        qkv = h @ w[p + "qkv"].T
+        qkv = linear(h, p + "qkv")
         q = qkv[:, :Hq * D].reshape(n, Hq, D)
         k = qkv[:, Hq * D:(Hq + Hkv) * D].reshape(n, Hkv, D)
         v = qkv[:, (Hq + Hkv) * D:].reshape(n, Hkv, D)
@@ -87,11 +91,14 @@ def decoder_logits(w: dict, cfg, tokens) -> torch.Tensor:
         s = s.masked_fill(mask[None], float("-inf"))
         a = torch.softmax(s, dim=-1)
         o = torch.einsum("hts,shd->thd", a, v).reshape(n, Hq * D)
-        x = x + o @ w[p + "o"].T
+        x = x + linear(o, p + "o")
         h = _rms(x, w[p + "post_norm"], cfg.rms_eps)
-        gu = h @ w[p + "gate_up"].T
+        if mlp is not None:
+            x = x + mlp(h, p)
+            continue
+        gu = linear(h, p + "gate_up")
         g, u = gu[:, :cfg.ffn], gu[:, cfg.ffn:]
-        x = x + (torch.nn.functional.silu(g) * u) @ w[p + "down"].T
+        x = x + linear(torch.nn.functional.silu(g) * u, p + "down")
     x = _rms(x, w["final_norm"], cfg.rms_eps)
     return x @ w["lm_head"].T
 
@@ -196,10 +203,10 @@ def decoder_suffix_logits(w: dict, cfg, cache: PromptCache, suffixes) -> torch.T
     return _rms(x, w["final_norm"], cfg.rms_eps) @ w["lm_head"].T
 
 
-def decoder_next_logprobs(w: dict, cfg):
+def decoder_next_logprobs(w: dict, cfg, linear=None, mlp=None):
     """``tokens -> log_softmax(last-position logits)`` (float64 numpy)."""
     def f(tokens):
-        lg = decoder_logits(w, cfg, tokens)[-1]
+        lg = decoder_logits(w, cfg, tokens, linear, mlp)[-1]
         return torch.log_softmax(lg, dim=-1).numpy()
     return f
 

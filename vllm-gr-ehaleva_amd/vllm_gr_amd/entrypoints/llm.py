@@ -33,7 +33,7 @@ from .. import logprobs as lpm
 from .. import ops
 from ..tracing import roctx_range
 from ..v1.beam_kv import BeamKVTable
-from ..v1.sid_decoder import SID_DECODER_1P7B, DecoderConfig, SidDecoder, init_weights
+from ..v1.sid_decoder import SID_DECODER_1P7B, DecoderConfig, SidDecoder, init_weights, quantize_weights
 from ..v1.sid_runner import SidModelRunner
 from . import beam_search as bsm
 from .beam_search import BeamSearchParams
@@ -91,17 +91,24 @@ class LLM:
     generated tokens; a candidate the catalog rules out never becomes a beam
     (the reference keeps it as a -inf-score beam, serving_engine.py:504-506,
     which only reaches the output when fewer than beam_width valid sequences
-    exist)."""
+    exist).  ``quantization="fp8"`` serves the layers' projections and experts in
+    e4m3 (``quantize_weights``); weights that come with their scales are served so
+    in any case."""
 
     def __init__(self, cfg: DecoderConfig = SID_DECODER_1P7B, *, seed: int = 0, device="cuda",
                  num_blocks: int = 4096, block_size: int = 16, eos_token_id: int | None = None,
                  special_tokens: dict[str, int] | None = None, weights: dict | None = None,
-                 max_position: int = 32768, use_graphs: bool = True, catalog=None, logprobs: bool = True):
+                 max_position: int = 32768, use_graphs: bool = True, catalog=None, logprobs: bool = True,
+                 quantization: str | None = None):
         dev = torch.device(device)
         if dev.type != "cuda":
             raise ValueError("the beam path runs on a HIP device (torch 'cuda')")
+        if quantization not in (None, "fp8"):
+            raise ValueError("quantization must be None or 'fp8'")
         if weights is None:
             weights = init_weights(cfg, seed, dev)
+        if quantization:
+            weights = quantize_weights(weights)
         self.cfg = cfg
         self.model = SidDecoder(cfg, weights, max_position=max_position)
         self.runner = SidModelRunner(self.model, num_blocks, block_size, use_graphs=use_graphs)

@@ -10,8 +10,9 @@ from N(0, std) -- there are no checkpoints here:
 * per layer: RMSNorm, q/k/v projections (no bias), per-head RMSNorm of q and
   k, rotary embedding with rotate-half pairing (theta 1e6) at the positions
   the caller gives, attention through the BeamAttention backend, o
-  projection, residual add; RMSNorm, SwiGLU MLP (silu(gate) * up, down),
-  residual add;
+  projection, residual add; RMSNorm, SwiGLU MLP (silu(gate) * up, down) or,
+  with ``num_experts``, a router and the SwiGLU layers of the experts it
+  chooses for each token, residual add;
 * final RMSNorm; logits = lm_head products in ``cfg.dtype``, widened to float32.
 
 The projections of a decode step's qkv, o, gate_up (with its SiLU gate) and
@@ -19,7 +20,9 @@ lm_head are gr_linear where that is the faster (up to 512 rows, from at most 204
 features: ``_own_sizes``); the others are ``torch.nn.functional.linear`` (hipBLASLt on ROCm).  The
 elementwise stages are fused HIP kernels (include/gr_decoder.h): residual add
 + RMSNorm, per-head q/k RMSNorm + rotary + K/V cache write through the slot
-mapping, and the SiLU-gated product.  Attention is
+mapping, and the SiLU-gated product.  With weights from
+``quantize_weights`` a layer's projections and experts are e4m3 in blocks of 128 x 128
+(include/gr_experts.h), their inputs quantised token by token.  Attention is
 :class:`BeamAttentionImpl.forward`, the call vLLM's Attention layer makes
 (beam_attn.py:703-755), with the K/V already written (key/value None).
 Positions follow the reference's rule (a beam's j-th suffix token sits at prefix_len + j,
@@ -53,6 +56,17 @@ class DecoderConfig:
     tie_embeddings: bool = True
     init_std: float = 0.02
     dtype: torch.dtype = torch.bfloat16
+    # experts in place of the MLP (0: none; 16-bit dtypes): each token's
+    # experts_per_token of them, chosen by route_experts with these options
+    num_experts: int = 0
+    experts_per_token: int = 8
+    expert_ffn: int = 768
+    router_score: str = "softmax"
+    router_bias: bool = False
+    router_groups: int = 1
+    router_top_groups: int = 1
+    router_renormalize: bool = True
+    router_scale: float = 1.0
 
     @property
     def q_size(self) -> int:
@@ -64,8 +78,10 @@ class DecoderConfig:
 
     def num_params(self) -> int:
         H, L = self.hidden, self.num_layers
-        per_layer = (H * (self.q_size + 2 * self.kv_size) + self.q_size * H + 3 * H * self.ffn
-                     + 2 * H + 2 * self.head_dim)
+        mlp = 3 * H * self.ffn
+        if self.num_experts:
+            mlp = self.num_experts * (3 * H * self.expert_ffn + H + (1 if self.router_bias else 0))
+        per_layer = H * (self.q_size + 2 * self.kv_size) + self.q_size * H + mlp + 2 * H + 2 * self.head_dim
         emb = self.vocab * H * (1 if self.tie_embeddings else 2)
         return L * per_layer + emb + H
 
@@ -77,8 +93,10 @@ SID_DECODER_1P7B = DecoderConfig()
 def init_weights(cfg: DecoderConfig, seed: int, device="cpu") -> dict[str, torch.Tensor]:
     """Weights in nn.Linear layout ``[out, in]``, drawn from one generator on
     ``device`` in a fixed order (embedding, then per layer qkv, o, gate_up,
-    down), N(0, init_std) in float32 rounded to ``cfg.dtype``; norm weights
-    are ones.  The same seed and device give the same weights."""
+    down; with experts router, expert_gate_up ``[E, 2 F, H]``, expert_down ``[E, H,
+    F]``), N(0, init_std) in float32 rounded to ``cfg.dtype``; norm weights
+    are ones, a router's bias zeros (float32).  The same seed and device give the
+    same weights."""
     dev = torch.device(device)
     g = torch.Generator(device=dev)
     g.manual_seed(seed)
@@ -94,8 +112,16 @@ def init_weights(cfg: DecoderConfig, seed: int, device="cpu") -> dict[str, torch
         p = f"layers.{i}."
         w[p + "qkv"] = normal(cfg.q_size + 2 * cfg.kv_size, H)
         w[p + "o"] = normal(H, cfg.q_size)
-        w[p + "gate_up"] = normal(2 * cfg.ffn, H)
-        w[p + "down"] = normal(H, cfg.ffn)
+        if cfg.num_experts:
+            E, F_ = cfg.num_experts, cfg.expert_ffn
+            w[p + "router"] = normal(E, H)
+            if cfg.router_bias:
+                w[p + "router_bias"] = torch.zeros(E, device=dev)
+            w[p + "expert_gate_up"] = normal(E, 2 * F_, H)
+            w[p + "expert_down"] = normal(E, H, F_)
+        else:
+            w[p + "gate_up"] = normal(2 * cfg.ffn, H)
+            w[p + "down"] = normal(H, cfg.ffn)
         w[p + "input_norm"] = ones(H)
         w[p + "post_norm"] = ones(H)
         w[p + "q_norm"] = ones(cfg.head_dim)
@@ -103,6 +129,40 @@ def init_weights(cfg: DecoderConfig, seed: int, device="cpu") -> dict[str, torch
     w["final_norm"] = ones(H)
     w["lm_head"] = w["embed"] if cfg.tie_embeddings else normal(cfg.vocab, H)
     return w
+
+
+def quantize_blocks(w: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """``w [..., N, K]`` as e4m3 with a float32 scale for each block of 128 x 128
+    (``[..., ceil(N / 128), ceil(K / 128)]``): the block's largest magnitude over
+    448, at least 2^-80, as gr_quant_fp8 scales a row's groups."""
+    N, K = w.shape[-2:]
+    nb, kb = -(-N // ops.FP8_BLOCK), -(-K // ops.FP8_BLOCK)
+    x = F.pad(w.float(), (0, kb * ops.FP8_BLOCK - K, 0, nb * ops.FP8_BLOCK - N))
+    x = x.unflatten(-1, (kb, ops.FP8_BLOCK)).unflatten(-3, (nb, ops.FP8_BLOCK))
+    scale = (x.abs().amax((-3, -1)) / 448.0).clamp_min(2.0 ** -80)
+    x = (x / scale[..., :, None, :, None]).flatten(-2).flatten(-3, -2)[..., :N, :K]
+    return x.to(torch.float8_e4m3fn).contiguous(), scale.contiguous()
+
+
+_QUANTIZED = ("qkv", "o", "gate_up", "down", "expert_gate_up", "expert_down")
+
+
+def quantize_weights(weights: dict[str, torch.Tensor]) -> dict[str, torch.Tensor]:
+    """A decoder's weights with every layer's projections and experts in e4m3 and
+    their scales beside them (``<name>_scale``); gate and up are scaled apart.
+    Embedding, lm_head, norms and router stay as they are, and so does what has its
+    scales already."""
+    out = {}
+    for name, w in weights.items():
+        kind = name.rsplit(".", 1)[-1]
+        if not name.startswith("layers.") or kind not in _QUANTIZED or name + "_scale" in weights:
+            out[name] = w
+        elif kind.endswith("gate_up"):
+            w8, scale = quantize_blocks(w.unflatten(-2, (2, w.shape[-2] // 2)))
+            out[name], out[name + "_scale"] = w8.flatten(-3, -2), scale.flatten(-3, -2).contiguous()
+        else:
+            out[name], out[name + "_scale"] = quantize_blocks(w)
+    return out
 
 
 class RotaryEmbedding:
@@ -196,6 +256,8 @@ class SidDecoder:
     logits."""
 
     def __init__(self, cfg: DecoderConfig, weights: dict[str, torch.Tensor], *, max_position: int = 32768):
+        if cfg.num_experts and cfg.dtype not in (torch.bfloat16, torch.float16):
+            raise ValueError("experts need a 16-bit dtype")
         self.cfg = cfg
         self.w = weights
         dev = weights["embed"].device
@@ -208,6 +270,32 @@ class SidDecoder:
     @property
     def device(self) -> torch.device:
         return self.w["embed"].device
+
+    def _project(self, x: torch.Tensor, name: str) -> torch.Tensor:
+        w, scale = self.w[name], self.w.get(name + "_scale")
+        if scale is None:
+            return _linear(x, w)
+        return ops.linear_fp8(*ops.quant_fp8(x), w, scale, out_dtype=x.dtype)
+
+    def _mlp(self, x: torch.Tensor, p: str) -> torch.Tensor:
+        w, cfg = self.w, self.cfg
+        if cfg.num_experts:
+            router = w[p + "router"]
+            # the scores' order decides: float32 logits
+            logits = (ops.linear(x, router, out_f32=True) if _own_linear(x, router)
+                      else F.linear(x.float(), router.float()))
+            weights, ids = ops.route_experts(
+                logits, cfg.experts_per_token, score=cfg.router_score, bias=w.get(p + "router_bias"),
+                num_groups=cfg.router_groups, top_groups=cfg.router_top_groups,
+                renormalize=cfg.router_renormalize, scale=cfg.router_scale)
+            return ops.expert_mlp(x, w[p + "expert_gate_up"], w[p + "expert_down"], weights, ids,
+                                  gate_up_scale=w.get(p + "expert_gate_up_scale"),
+                                  down_scale=w.get(p + "expert_down_scale"))
+        scale = w.get(p + "gate_up_scale")
+        if scale is None:
+            return _linear(_swiglu(x, w[p + "gate_up"]), w[p + "down"])
+        act = ops.linear_fp8(*ops.quant_fp8(x), w[p + "gate_up"], scale, swiglu=True, quantized=True)
+        return ops.linear_fp8(*act, w[p + "down"], w[p + "down_scale"], out_dtype=x.dtype)
 
     def forward(self, input_ids: torch.Tensor, positions: torch.Tensor, attn_metadata,
                 kv_caches) -> torch.Tensor:
@@ -222,7 +310,7 @@ class SidDecoder:
             p = f"layers.{i}."
             if i:
                 x = ops.rms_norm(mlp, w[p + "input_norm"], eps, residual=h, out=x)
-            qkv = _linear(x, w[p + "qkv"])
+            qkv = self._project(x, p + "qkv")
             k_cache, v_cache = ops.split_kv_cache(kv_caches[i])
             q = ops.qk_norm_rope_cache(qkv, positions, self.rope.cos, self.rope.sin, w[p + "q_norm"],
                                        w[p + "k_norm"], k_cache, v_cache, slots, num_q_heads=cfg.num_heads,
@@ -230,9 +318,9 @@ class SidDecoder:
                                        status=status)
             attn = torch.empty_like(q)
             self.attn[i].forward(None, q, None, None, kv_caches[i], attn_metadata, output=attn)
-            x = ops.rms_norm(_linear(attn.view(T, cfg.q_size), w[p + "o"]), w[p + "post_norm"], eps,
+            x = ops.rms_norm(self._project(attn.view(T, cfg.q_size), p + "o"), w[p + "post_norm"], eps,
                              residual=h, out=x)
-            mlp = _linear(_swiglu(x, w[p + "gate_up"]), w[p + "down"])
+            mlp = self._mlp(x, p)
         return ops.rms_norm(mlp, w["final_norm"], eps, residual=h)
 
     def compute_logits(self, hidden: torch.Tensor) -> torch.Tensor:

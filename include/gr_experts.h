@@ -24,7 +24,7 @@ extern "C" {
  * (of the exact quotient: it is not rounded to float32 in between).  A group with
  * an infinity or a NaN gets that as its scale, so it reads back as NaN where the
  * scale is, or the product of 0 and infinity.  x [num_tokens, features] float32,
- * fp16 or bf16; features % 16 == 0, rows 16-byte aligned; out rows 8-byte aligned.
+ * fp16 or bf16; features % 16 == 0, rows of x and out 16-byte aligned.
  * scale [num_tokens, ceil(features / 128)] at the element strides scale_row /
  * scale_group.
  */

@@ -22,7 +22,7 @@ def test_quant_refusals(built_lib):
     for o in (dict(T=-1), dict(K=0), dict(dtype=3), dict(out=None), dict(scale=None), dict(x=None), dict(ostr=255),
               dict(xstr=255), dict(srow=-1), dict(sgrp=-1)):
         assert f(**o) == BAD, o
-    for o in (dict(K=248), dict(x=A + 2), dict(xstr=257), dict(out=A + 4), dict(ostr=260), dict(T=2 ** 31 - 1)):
+    for o in (dict(K=248), dict(x=A + 2), dict(xstr=257), dict(out=A + 8), dict(ostr=264), dict(T=2 ** 31 - 1)):
         assert f(**o) == UNSUPPORTED, o
 
 

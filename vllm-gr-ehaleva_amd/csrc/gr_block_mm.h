@@ -76,16 +76,42 @@ __device__ inline float quant_div(float x, float s, float r) {
   }
   return q;
 }
+// N values over their scale.  x r is within two ulps of x / s, so the side of a border
+// is known unless x r lies within four of one: the borders of normal e4m3 numbers are
+// where the 20 bits below their mantissa are one half.  Such values, and (low) any below
+// the normal numbers but 0, are divided as above, which is rarely any wave's business.
+template <int N> __device__ inline void quant_values(const float (&v)[N], float s, float r, bool low, float (&q)[N]) {
+  uint32_t near = ~0u;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    q[i] = v[i] * r;
+    near = min(near, (__builtin_bit_cast(uint32_t, q[i]) << 12) + 0x80004000u);
+  }
+  if (low || near < 0x8000u)
+#pragma unroll
+    for (int i = 0; i < N; ++i) q[i] = quant_div(v[i], s, r);
+}
+constexpr float QUANT_LOW = 0x1.0001p-6f;  // (a little over 2^-6, for the roundings)
+// whether any value but 0 is below the normal e4m3 numbers (2^-6) of its scale
+template <int N> __device__ inline bool quant_low(const float (&v)[N], float s) {
+  uint32_t low = ~0u;
+#pragma unroll
+  for (int i = 0; i < N; ++i) low = min(low, (__builtin_bit_cast(uint32_t, v[i]) & 0x7FFFFFFFu) - 1u);
+  return low != ~0u && __builtin_bit_cast(float, low + 1u) < s * QUANT_LOW;
+}
 // scale of a group from the bits of its largest |x| (a NaN's are the largest)
 __device__ inline float quant_scale(uint32_t amax_bits) {
   const float t = __builtin_bit_cast(float, amax_bits) / 448.0f;
   return t < 0x1p-80f ? 0x1p-80f : t;
 }
+__device__ inline uint32_t fp8_pack4(const float* q) {
+  const int p = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], p, true);
+}
 __device__ inline uint32_t quant_pack4(const float (&v)[4], float s, float r) {
-  int p = 0;
-  p = __builtin_amdgcn_cvt_pk_fp8_f32(quant_div(v[0], s, r), quant_div(v[1], s, r), p, false);
-  p = __builtin_amdgcn_cvt_pk_fp8_f32(quant_div(v[2], s, r), quant_div(v[3], s, r), p, true);
-  return (uint32_t)p;
+  float q[4];
+  quant_values(v, s, r, quant_low(v, s), q);
+  return fp8_pack4(q);
 }
 
 template <int DT> __device__ inline mm4_t mm_mma(u32x4_t a, u32x4_t b, mm4_t c) {

@@ -766,7 +766,7 @@ def quant_fp8(x: torch.Tensor, *, out: torch.Tensor | None = None, scale: torch.
     """Rows ``x [T, K]`` (float32, fp16 or bf16) as e4m3 with one float32 scale
     for each 128 features: ``(out [T, K] float8_e4m3fn, scale [T, ceil(K / 128)])``,
     the value being ``out * scale``; see ``gr_quant_fp8`` in gr_experts.h.  ``K`` is
-    a multiple of 16 and rows are 16-byte aligned; ``scale`` may have any strides."""
+    a multiple of 16 and rows of ``x`` and ``out`` are 16-byte aligned; ``scale`` may have any strides."""
     dev = _need_cuda(x, out, scale)
     _rows("x", x)
     T, K = x.shape

@@ -431,33 +431,57 @@ __global__ __launch_bounds__(PLAN_THREADS) void expert_plan_k(PlanArgs a) {
 struct CombineArgs {
   void* out;
   int64_t out_stride;
-  const float* y;
+  const void* y;         // float32, or MM_OUT_SCALED with the units' exponents
+  const int8_t* y_exp;
+  int exp_cols;          // columns of one exponent
   const float* weights;
   const int32_t* ids;
   int T, k, E, H;
 };
 
-template <int DT>
+// Bound by memory; a thread sums 8 columns over the token's choices, in order.
+template <int DT, bool SCALED>
 __global__ __launch_bounds__(256) void expert_combine_k(CombineArgs a) {
   const int64_t t = blockIdx.x;
-  const int h = (blockIdx.y * 256 + threadIdx.x) * 4;
+  const int h = (blockIdx.y * 256 + threadIdx.x) * 8;
   if (h >= a.H) return;
-  mm4_t acc = {0.f, 0.f, 0.f, 0.f};
+  const int groups = SCALED ? (a.H + a.exp_cols - 1) / a.exp_cols : 0;
+  float acc[8] = {};
+#pragma unroll 8
   for (int j = 0; j < a.k; ++j) {
-    const int e = a.ids[t * a.k + j];
-    if (e < 0 || e >= a.E) continue;
-    const float w = a.weights[t * a.k + j];
-    const mm4_t v = *reinterpret_cast<const mm4_t*>(a.y + (t * a.k + j) * a.H + h);
+    const int64_t row = t * a.k + j;
+    const int e = a.ids[row];
+    const bool here = e >= 0 && e < a.E;  // (another's row holds anything: loaded all the same, so that nothing waits
+    const float w = a.weights[row];       // for the id, and left out)
+    float v[8];
+    if constexpr (SCALED) {
+      const u32x4_t d = *reinterpret_cast<const u32x4_t*>(static_cast<const uint16_t*>(a.y) + row * a.H + h);
+      const float unit = __builtin_amdgcn_ldexpf(1.0f, a.y_exp[row * groups + h / a.exp_cols]);
 #pragma unroll
-    for (int u = 0; u < 4; ++u) acc[u] = fmaf(w, v[u], acc[u]);
+      for (int u = 0; u < 4; ++u) {
+        v[2 * u] = Mma<GR_DTYPE_F16>::lo(d[u]) * unit;
+        v[2 * u + 1] = Mma<GR_DTYPE_F16>::hi(d[u]) * unit;
+      }
+    } else {
+      const mm4_t* p = reinterpret_cast<const mm4_t*>(static_cast<const float*>(a.y) + row * a.H + h);
+      const mm4_t lo = p[0], hi = p[1];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        v[u] = lo[u];
+        v[u + 4] = hi[u];
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u) acc[u] = here ? fmaf(w, v[u], acc[u]) : acc[u];
   }
-  const float v[4] = {acc[0], acc[1], acc[2], acc[3]};
-  mm_store<DT>(a.out, t * a.out_stride + h, v);
+  const float lo[4] = {acc[0], acc[1], acc[2], acc[3]}, hi[4] = {acc[4], acc[5], acc[6], acc[7]};
+  mm_store<DT>(a.out, t * a.out_stride + h, lo);
+  mm_store<DT>(a.out, t * a.out_stride + h + 4, hi);
 }
 
 // ---- workspace -----------------------------------------------------------------
 struct Workspace {
-  int64_t hist, slot, tiles, num_tiles, x8, xs, act, act_scale, y, bytes;
+  int64_t hist, slot, tiles, num_tiles, x8, xs, act, act_scale, y, y_exp, bytes;
   int64_t max_tiles;
   int blocks;
 };
@@ -497,9 +521,14 @@ Workspace plan_workspace(int T, int k, int E, int H, int F, bool fp8, int bm) {
   } else {
     w.act = take(2 * rows * F);
   }
+  // (room for float32, whatever the results' type turns out to be)
   w.y = take(4 * rows * H);
+  w.y_exp = take(rows * ((H + 15) / 16));
   return w;
 }
+
+// columns of a wave of the down product with tiles of bm rows (launch_experts)
+int expert_wave_cols(int bm) { return bm == 16 ? 16 : bm <= 64 ? 32 : 64; }
 
 template <int XT>
 void launch_experts(const MmArgs& up, const MmArgs& down, int tiles, int bm, hipStream_t stream) {
@@ -662,7 +691,11 @@ extern "C" gr_status_t gr_expert_mlp(void* out, int64_t out_stride, const void* 
   dn.M = rows;
   dn.N = H;
   dn.kbytes = F * esize;
-  dn.out_type = GR_DTYPE_F32;
+  // Rounding the experts' results to fp16 multiples costs 2^-12 of each: an eighth of what bf16's own roundings do, and
+  // nothing beside e4m3 inputs; fp16 results of 16-bit weights are as exact as that themselves, and keep float32.
+  const bool scaled = fp8 || dtype == GR_DTYPE_BF16;
+  dn.out_type = scaled ? MM_OUT_SCALED : GR_DTYPE_F32;
+  dn.out_exp = reinterpret_cast<int8_t*>(ws + l.y_exp);
   dn.tiles = p.tiles;
   dn.num_tiles = p.num_tiles;
   dn.slot = p.slot;
@@ -679,10 +712,12 @@ extern "C" gr_status_t gr_expert_mlp(void* out, int64_t out_stride, const void* 
   else if (dtype == GR_DTYPE_BF16) launch_experts<GR_DTYPE_BF16>(up, dn, tiles, bm, stream);
   else launch_experts<GR_DTYPE_F16>(up, dn, tiles, bm, stream);
 
-  const CombineArgs c{out, out_stride, reinterpret_cast<const float*>(ws + l.y), weights, ids, T, top_k,
+  const CombineArgs c{out, out_stride, ws + l.y, dn.out_exp, expert_wave_cols(bm), weights, ids, T, top_k,
                       num_experts, H};
-  const dim3 grid((unsigned)T, (unsigned)((H + 1023) / 1024));
-  if (dtype == GR_DTYPE_BF16) hipLaunchKernelGGL(expert_combine_k<GR_DTYPE_BF16>, grid, dim3(256), 0, stream, c);
-  else hipLaunchKernelGGL(expert_combine_k<GR_DTYPE_F16>, grid, dim3(256), 0, stream, c);
+  const dim3 grid((unsigned)T, (unsigned)((H + 2047) / 2048));
+  auto go = [&](auto k) { hipLaunchKernelGGL(k, grid, dim3(256), 0, stream, c); };
+  if (dtype == GR_DTYPE_BF16) go(expert_combine_k<GR_DTYPE_BF16, true>);
+  else if (scaled) go(expert_combine_k<GR_DTYPE_F16, true>);
+  else go(expert_combine_k<GR_DTYPE_F16, false>);
   return launch_status();
 }

@@ -207,7 +207,8 @@ extern "C" gr_status_t gr_linear_fp8(void* out, int64_t out_stride, float* out_s
       (quant && (!out_scale || out_scale_row < 0 || out_scale_group < 0)))
     return GR_ERR_INVALID_ARG;
   if (in_features % 16 != 0 || ((swiglu || quant) && out_features % 16 != 0) || out_features > (1 << 28) ||
-      num_tokens > (1 << 28) || x_stride > (1 << 22) || w_stride > (1 << 22) || !aligned(x, 16) || x_stride % 16 != 0 || !aligned(w, 16) || w_stride % 16 != 0 ||
+      num_tokens > (1 << 28) || x_stride > (1 << 22) || w_stride > (1 << 22) || !aligned(x, 16) || x_stride % 16 != 0 ||
+      !aligned(w, 16) || w_stride % 16 != 0 ||
       !aligned(out, out_dtype == GR_DTYPE_F32 ? 16 : quant ? 4 : 8) || (quant && out_stride % 4 != 0) ||
       !aligned(x_scale, 4) || !aligned(w_scale, 4) || (quant && !aligned(out_scale, 4)) ||
       ((int64_t)num_tokens + 15) / 16 * ((out_features + 15) / 16) > INT32_MAX - 8)

@@ -38,7 +38,7 @@ typedef int mm8i_t __attribute__((__vector_size__(32)));
 // experts: fp16 multiples of a power of two for each row's columns of one wave, so
 // that the largest (of the finite ones) is within [2^14, 2^15): 2^-12 of a value that is
 // not 2^28 times smaller than its neighbours.  Half the bytes of float32, which are most
-// of what many tokens move (8192 tokens, 8 of 64 experts of 768: MEASURED us against 867).
+// of what many tokens move (8192 tokens, 8 of 64 experts of 768: 770 us against 860).
 constexpr int MM_OUT_SCALED = 16;
 
 enum { MM_PLAIN = 0, MM_SWIGLU = 1, MM_SWIGLU_Q = 2, MM_PLAIN_Q = 3 };
@@ -332,7 +332,8 @@ struct Mm {
     }
   }
   __device__ static __forceinline__ u32x4_t half(mm8i_t v, int h) {
-    return __builtin_bit_cast(u32x4_t, h ? __builtin_shufflevector(v, v, 4, 5, 6, 7) : __builtin_shufflevector(v, v, 0, 1, 2, 3));
+    return __builtin_bit_cast(u32x4_t, h ? __builtin_shufflevector(v, v, 4, 5, 6, 7)
+                                         : __builtin_shufflevector(v, v, 0, 1, 2, 3));
   }
   // fragment bytes 8 z .. + 7 as fp16
   __device__ static __forceinline__ u32x4_t fp16(mm8i_t v, int z) {
@@ -345,12 +346,14 @@ struct Mm {
       for (int z = 0; z < 4; ++z) wh[z][i] = fp16(w[i], z);
   }
   // products of fragment row j; xs, ws0, ws1: the row's scale and the weight blocks'
-  __device__ static __forceinline__ void mul(const mm8i_t (&w)[FN], mm8i_t x, int j, float xs, float ws0, float ws1, Acc& acc) {
+  __device__ static __forceinline__ void mul(const mm8i_t (&w)[FN], mm8i_t x, int j, float xs, float ws0, float ws1,
+                                             Acc& acc) {
     if constexpr (F8 && !EXACT) {
       const float c0 = xs * ws0, c1 = GATED ? xs * ws1 : c0;
 #pragma unroll
       for (int i = 0; i < FN; ++i) {
-        const mm4_t t = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w[i], x, mm4_t{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
+        const mm4_t z = {0.f, 0.f, 0.f, 0.f};
+        const mm4_t t = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w[i], x, z, 0, 0, 0, 0, 0, 0);
         const float c = GATED && (i & 1) ? c1 : c0;
 #pragma unroll
         for (int u = 0; u < 4; ++u) acc[i][j][u] = fmaf(t[u], c, acc[i][j][u]);

@@ -208,7 +208,11 @@ __device__ __forceinline__ RouteDoubt route_choose(const RouteArgs& a, const T (
     if constexpr (CHECK) {
       const T now = rank_value(top);
       const bool near = j > 0 && !apart(prev, now, 1.f);
-      open = open && j < 64 && top != 0 && (j < a.k || near);
+      open = open && top != 0 && (j < a.k || near);
+      if (open && j == 64) {  // (a list that does not end)
+        doubt.groups = true;
+        open = false;
+      }
       doubt.order |= open && near;
       doubt.listed = open ? j + 1 : doubt.listed;
       prev = now;
@@ -227,7 +231,6 @@ __device__ __forceinline__ RouteDoubt route_choose(const RouteArgs& a, const T (
     }
     if (win) room.id[tok][j] = e0 + at;
   }
-  if (CHECK && doubt.listed == 64 && a.k < 64) doubt.groups = true;  // (a list that did not end)
   return doubt;
 }
 

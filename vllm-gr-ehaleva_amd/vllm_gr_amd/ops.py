@@ -9,7 +9,6 @@ the HIP library every call raises.
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import weakref
 
@@ -746,9 +745,17 @@ def _row_stride(t: torch.Tensor) -> int:
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
-def _on(dev: torch.device):
-    """Launches go to ``dev``, also while another device is the current one."""
-    return contextlib.nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+def _launch(dev: torch.device, name: str, *args) -> None:
+    """Calls the library's ``name`` for tensors on ``dev``, also while another device
+    is the current one."""
+    fn = getattr(_C.lib(), name)
+    if dev.index == torch._C._cuda_getDevice():
+        code = fn(*args)
+    else:
+        with torch.cuda.device(dev):
+            code = fn(*args)
+    if code != _C.GR_OK:
+        _C.check(name, code)
 
 
 def _row_scales(name: str, t: torch.Tensor, rows: int, features: int) -> None:
@@ -780,10 +787,8 @@ def quant_fp8(x: torch.Tensor, *, out: torch.Tensor | None = None, scale: torch.
         scale = _new_row_scales(T, K, dev)
     else:
         _row_scales("scale", scale, T, K)
-    with _on(dev):
-        code = _C.lib().gr_quant_fp8(out.data_ptr(), _row_stride(out), scale.data_ptr(), scale.stride(0), scale.stride(1),
-                                     x.data_ptr(), _row_stride(x), T, K, _dtype_code(x), _stream(dev))
-    _C.check("gr_quant_fp8", code)
+    _launch(dev, "gr_quant_fp8", out.data_ptr(), _row_stride(out), scale.data_ptr(), scale.stride(0), scale.stride(1),
+            x.data_ptr(), _row_stride(x), T, K, _dtype_code(x), _stream(dev))
     return out, scale
 
 
@@ -829,13 +834,10 @@ def linear_fp8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale:
         _row_scales("out_scale", out_scale, T, N)
     elif quantized:
         out_scale = _new_row_scales(T, N, dev)
-    with _on(dev):
-        code = _C.lib().gr_linear_fp8(
-            out.data_ptr(), _row_stride(out), _ptr(out_scale), *(out_scale.stride() if quantized else (0, 0)),
-            x.data_ptr(), _row_stride(x), x_scale.data_ptr(), x_scale.stride(0), x_scale.stride(1), w.data_ptr(),
-            _row_stride(w), w_scale.data_ptr(), T, N, K, int(swiglu),
-            _C.GR_DTYPE_FP8_E4M3 if quantized else _dtype_code(out), _stream(dev))
-    _C.check("gr_linear_fp8", code)
+    _launch(dev, "gr_linear_fp8", out.data_ptr(), _row_stride(out), _ptr(out_scale),
+            *(out_scale.stride() if quantized else (0, 0)), x.data_ptr(), _row_stride(x), x_scale.data_ptr(),
+            x_scale.stride(0), x_scale.stride(1), w.data_ptr(), _row_stride(w), w_scale.data_ptr(), T, N, K,
+            int(swiglu), _C.GR_DTYPE_FP8_E4M3 if quantized else _dtype_code(out), _stream(dev))
     return (out, out_scale) if quantized else out
 
 
@@ -861,12 +863,9 @@ def route_experts(logits: torch.Tensor, top_k: int, *, score: str = "softmax", b
         raise ValueError("top_k must be at least 1")
     weights = torch.empty((T, top_k), dtype=torch.float32, device=dev)
     ids = torch.empty((T, top_k), dtype=torch.int32, device=dev)
-    with _on(dev):
-        code = _C.lib().gr_route_experts(
-            weights.data_ptr(), ids.data_ptr(), logits.data_ptr(), _row_stride(logits), _ptr(bias), T, E, top_k,
-            _SCORES[score], int(num_groups), int(top_groups), int(bool(renormalize)), float(scale), _dtype_code(logits),
-            _stream(dev))
-    _C.check("gr_route_experts", code)
+    _launch(dev, "gr_route_experts", weights.data_ptr(), ids.data_ptr(), logits.data_ptr(), _row_stride(logits),
+            _ptr(bias), T, E, top_k, _SCORES[score], int(num_groups), int(top_groups), int(bool(renormalize)),
+            float(scale), _dtype_code(logits), _stream(dev))
     return weights, ids
 
 
@@ -916,12 +915,9 @@ def expert_mlp(x: torch.Tensor, gate_up: torch.Tensor, down: torch.Tensor, weigh
     need = expert_mlp_workspace_bytes(T, k, E, H, F, fp8)
     if workspace is None:
         workspace = torch.empty(need, dtype=torch.uint8, device=dev)
-    with _on(dev):
-        code = _C.lib().gr_expert_mlp(
-            out.data_ptr(), _row_stride(out), x.data_ptr(), _row_stride(x), gate_up.data_ptr(), _ptr(gate_up_scale),
-            down.data_ptr(), _ptr(down_scale), weights.data_ptr(), ids.data_ptr(), T, k, E, H, F, _dtype_code(x),
-            workspace.data_ptr(), workspace.numel() * workspace.element_size(), _ptr(status), _stream(dev))
-    _C.check("gr_expert_mlp", code)
+    _launch(dev, "gr_expert_mlp", out.data_ptr(), _row_stride(out), x.data_ptr(), _row_stride(x), gate_up.data_ptr(),
+            _ptr(gate_up_scale), down.data_ptr(), _ptr(down_scale), weights.data_ptr(), ids.data_ptr(), T, k, E, H, F,
+            _dtype_code(x), workspace.data_ptr(), workspace.numel() * workspace.element_size(), _ptr(status), _stream(dev))
     return out
 
 

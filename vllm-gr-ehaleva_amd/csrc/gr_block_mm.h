@@ -675,12 +675,12 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void block_mm(MmArgs a) {
 template <int XT, int FM, int WK, int MODE, bool EXPERTS>
 __global__ __launch_bounds__(512) void few_mm(MmArgs a) {
   constexpr bool F8 = XT == GR_DTYPE_FP8_E4M3;
-  constexpr bool GATED = MODE == MM_SWIGLU || MODE == MM_SWIGLU_Q, QUANT = MODE == MM_SWIGLU_Q || MODE == MM_PLAIN_Q;
+  constexpr bool GATED = MODE == MM_SWIGLU;
   constexpr int WN = 8 / WK, FN = GATED ? 2 : 1, U = FM == 1 ? 4 : 2;
   using M = Mm<XT, 16 * FM, 16 * FN * WN, 1, WN, MODE, EXPERTS, F8>;
   using M1 = Mm<XT, 16, 16 * FN * WN, 1, WN, MODE, EXPERTS, F8>;  // one fragment row
-  static_assert(!QUANT || WK == 1, "a tile's columns are one group of the result");
-  constexpr int LDS = QUANT ? WN * 16 * FM * 4 + 16 * FM * 144 : WK * WN * FM * FN * 1024 + 8 * 16 * 80;
+  static_assert(MODE == MM_PLAIN || MODE == MM_SWIGLU, "results that are not quantised");
+  constexpr int LDS = WK * WN * FM * FN * 1024 + 8 * 16 * 80;
   __shared__ __attribute__((aligned(16))) uint8_t lds[LDS];
   MmTile t;
   if (!M::tile(a, t)) return;
@@ -738,32 +738,28 @@ __global__ __launch_bounds__(512) void few_mm(MmArgs a) {
         else M::mul(w[u], x[u][j], j, 0.f, 0.f, 0.f, acc);
     }
   }
-  if constexpr (QUANT) {
-    M::finish(a, t, acc, wave, 0, wn, lane, lds);
-  } else {
-    mm4_t* part = reinterpret_cast<mm4_t*>(lds);  // [wave][FM][FN][64]
+  mm4_t* part = reinterpret_cast<mm4_t*>(lds);  // [wave][FM][FN][64]
 #pragma unroll
-    for (int j = 0; j < FM; ++j)
+  for (int j = 0; j < FM; ++j)
 #pragma unroll
-      for (int i = 0; i < FN; ++i) part[((wave * FM + j) * FN + i) * 64 + lane] = acc[i][j];
-    __syncthreads();
-    // wave (k, n) finishes fragment rows k, k + WK, ... of column fragment n
-    for (int j = wk; j < FM; j += WK) {
-      typename M1::Acc sum;
+    for (int i = 0; i < FN; ++i) part[((wave * FM + j) * FN + i) * 64 + lane] = acc[i][j];
+  __syncthreads();
+  // wave (k, n) finishes fragment rows k, k + WK, ... of column fragment n
+  for (int j = wk; j < FM; j += WK) {
+    typename M1::Acc sum;
 #pragma unroll
-      for (int i = 0; i < FN; ++i) {
-        sum[i][0] = part[((wn * FM + j) * FN + i) * 64 + lane];
+    for (int i = 0; i < FN; ++i) {
+      sum[i][0] = part[((wn * FM + j) * FN + i) * 64 + lane];
 #pragma unroll
-        for (int k = 1; k < WK; ++k) {
-          const mm4_t v = part[(((k * WN + wn) * FM + j) * FN + i) * 64 + lane];
+      for (int k = 1; k < WK; ++k) {
+        const mm4_t v = part[(((k * WN + wn) * FM + j) * FN + i) * 64 + lane];
 #pragma unroll
-          for (int u = 0; u < 4; ++u) sum[i][0][u] += v[u];
-        }
+        for (int u = 0; u < 4; ++u) sum[i][0][u] += v[u];
       }
-      MmTile tj = t;
-      tj.m0 += 16 * j;
-      if (tj.m0 < tj.m_end) M1::store_any(a, tj, sum, wave, 0, wn, lane, lds + WK * WN * FM * FN * 1024);
     }
+    MmTile tj = t;
+    tj.m0 += 16 * j;
+    if (tj.m0 < tj.m_end) M1::store_any(a, tj, sum, wave, 0, wn, lane, lds + WK * WN * FM * FN * 1024);
   }
 }
 

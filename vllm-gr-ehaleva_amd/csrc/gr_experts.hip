@@ -531,15 +531,16 @@ Workspace plan_workspace(int T, int k, int E, int H, int F, bool fp8, int bm) {
 }
 
 // columns of a wave of the down product with tiles of bm rows (launch_experts)
-int expert_wave_cols(int bm) { return bm == 16 ? 16 : bm <= 64 ? 32 : 64; }
+int expert_wave_cols(int bm) { return bm == 16 ? 16 : bm == 64 ? 32 : 64; }
 
 template <int XT>
 void launch_experts(const MmArgs& up, const MmArgs& down, int tiles, int bm, hipStream_t stream) {
   if constexpr (XT == GR_DTYPE_FP8_E4M3) {
-    // (down's float32 results are summed into 16 bits: the 8-bit instruction will do)
+    // (down's float32 results are summed into 16 bits: the 8-bit instruction will do.  512 tokens, 64 rows an expert:
+    // 256 columns of it 38.3 us, 128 columns 39.9)
     if (bm == 32) {
       launch_mm<XT, 32, 256, 1, 4, 2, MM_SWIGLU_Q, true, true>(up, tiles, stream);
-      launch_mm<XT, 32, 128, 1, 4, 3, MM_PLAIN, true, false>(down, tiles, stream);
+      launch_mm<XT, 32, 256, 1, 4, 2, MM_PLAIN, true, false>(down, tiles, stream);
     } else {
       launch_mm<XT, 128, 256, 2, 4, 3, MM_SWIGLU_Q, true, true>(up, tiles, stream);
       launch_mm<XT, 128, 128, 2, 2, 2, MM_PLAIN, true, false>(down, tiles, stream);

@@ -24,7 +24,8 @@ extern "C" {
  * (of the exact quotient: it is not rounded to float32 in between).  A group with
  * an infinity or a NaN gets that as its scale, so it reads back as NaN where the
  * scale is, or the product of 0 and infinity.  x [num_tokens, features] float32,
- * fp16 or bf16; features % 16 == 0, rows of x and out 16-byte aligned.
+ * fp16 or bf16; features % 16 == 0, rows of x and out 16-byte aligned, at most 2^28
+ * groups.
  * scale [num_tokens, ceil(features / 128)] at the element strides scale_row /
  * scale_group.
  */
@@ -48,7 +49,8 @@ gr_status_t gr_quant_fp8(void* out, int64_t out_stride, float* scale, int64_t sc
  * matrix core adds the e4m3 products, in groups of 8 whose members are cut off
  * below 2^-13 of the largest (about 1.5e-5 of an ordinary result); the groups'
  * sums are float32.
- * in_features % 16 == 0; x and w rows 16-byte aligned, at most 4 MB apart.
+ * in_features % 16 == 0; x and w rows 16-byte aligned, at most 4 MB apart; no more
+ * than 2^35 results, less for sizes that leave 64 x 64 tiles part empty.
  */
 gr_status_t gr_linear_fp8(void* out, int64_t out_stride, float* out_scale, int64_t out_scale_row,
                           int64_t out_scale_group, const void* x, int64_t x_stride, const float* x_scale,
@@ -70,7 +72,7 @@ enum { GR_SCORE_SOFTMAX = 0, GR_SCORE_SIGMOID = 1 };
  * as computed in float64.  A row of -inf alone has s = 0; a NaN ranks last.
  * logits float32, fp16 or bf16 at logits_stride, bias float32 [num_experts] or
  * NULL; weights float32, ids int32 [num_tokens, top_k] contiguous.
- * num_experts <= 1024, num_groups <= 64, top_k <= 64.
+ * num_experts <= 1024, num_groups <= 64, top_k <= 64, at most 2^34 logits.
  */
 gr_status_t gr_route_experts(float* weights, int32_t* ids, const void* logits, int64_t logits_stride,
                              const float* bias, int num_tokens, int num_experts, int top_k, int score,
@@ -89,10 +91,15 @@ gr_status_t gr_route_experts(float* weights, int32_t* ids, const void* logits, i
  * expert is rounded to it.  With gate_up_scale [num_experts, 2 * ceil(ffn / 128),
  * ceil(hidden / 128)] and down_scale [num_experts, ceil(hidden / 128),
  * ceil(ffn / 128)] they are e4m3, and x and the gated products are quantised as
- * gr_quant_fp8 does.  Everything else is float32, out is rounded once.
+ * gr_quant_fp8 does.  Sums are float32 (of e4m3 weights in the down product as for
+ * gr_linear_fp8's 16-bit results), and with e4m3 weights or a bf16 out each expert's
+ * result is rounded to fp16 times a power of two (2^-12 of a value, 2^-39 of the
+ * largest of its 16 to 64 neighbouring columns) before the sum over j, which is
+ * float32 and in the order of j.
  * hidden % 16 == 0, ffn % 16 == 0; rows of x, and weights, 16-byte aligned; out
- * rows 8-byte aligned.  num_experts <= 1024, x spans less than 2 GB.  workspace: gr_expert_mlp_workspace_size
- * bytes, 256-byte aligned, no initial contents; calls that may overlap need one each.
+ * rows 8-byte aligned.  num_experts <= 1024, num_tokens < 2^23, x spans less than
+ * 2 GB.  workspace: gr_expert_mlp_workspace_size bytes, 256-byte aligned, no initial
+ * contents; calls that may overlap need one each.
  */
 size_t gr_expert_mlp_workspace_size(int num_tokens, int top_k, int num_experts, int hidden, int ffn, int fp8);
 gr_status_t gr_expert_mlp(void* out, int64_t out_stride, const void* x, int64_t x_stride, const void* gate_up,

@@ -186,7 +186,7 @@ extern "C" gr_status_t gr_quant_fp8(void* out, int64_t out_stride, float* scale,
   if (!out || !scale || !x || out_stride < features || x_stride < features || scale_row < 0 || scale_group < 0)
     return GR_ERR_INVALID_ARG;
   if (features % 16 != 0 || !aligned(x, 16) || x_stride * dtype_size(dtype) % 16 != 0 || !aligned(out, 16) ||
-      out_stride % 16 != 0 || !aligned(scale, 4) || (int64_t)num_tokens * ((features + 127) / 128) > INT32_MAX)
+      out_stride % 16 != 0 || !aligned(scale, 4) || (int64_t)num_tokens * ((features + 127) / 128) > (1 << 28))
     return GR_ERR_UNSUPPORTED;
   return launch_quant_fp8(out, out_stride, scale, scale_row, scale_group, x, x_stride, num_tokens, features, dtype,
                           stream);
@@ -211,7 +211,7 @@ extern "C" gr_status_t gr_linear_fp8(void* out, int64_t out_stride, float* out_s
       !aligned(w, 16) || w_stride % 16 != 0 ||
       !aligned(out, out_dtype == GR_DTYPE_F32 ? 16 : quant ? 4 : 8) || (quant && out_stride % 4 != 0) ||
       !aligned(x_scale, 4) || !aligned(w_scale, 4) || (quant && !aligned(out_scale, 4)) ||
-      ((int64_t)num_tokens + 15) / 16 * ((out_features + 15) / 16) > INT32_MAX - 8)
+      x_scale_group > INT32_MAX || ((int64_t)num_tokens + 63) / 64 * ((out_features + 63) / 64) > (1 << 23) - 8)
     return GR_ERR_UNSUPPORTED;
   MmArgs a{};
   a.x = static_cast<const uint8_t*>(x);

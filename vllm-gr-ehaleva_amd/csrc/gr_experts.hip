@@ -1,4 +1,6 @@
 // Routing of tokens to experts, and the chosen experts' SwiGLU layers.
+#include <algorithm>
+
 #include "gr_block_mm.h"
 
 namespace gr {
@@ -530,6 +532,9 @@ Workspace plan_workspace(int T, int k, int E, int H, int F, bool fp8, int bm) {
   return w;
 }
 
+// Workgroups of a launch, of up to 512 threads: their threads are counted in 32 bits.
+constexpr int GRID_MAX = (1 << 23) - 1;
+
 // columns of a wave of the down product with tiles of bm rows (launch_experts)
 int expert_wave_cols(int bm) { return bm == 16 ? 16 : bm == 64 ? 32 : 64; }
 
@@ -603,7 +608,10 @@ extern "C" gr_status_t gr_route_experts(float* weights, int32_t* ids, const void
     return GR_ERR_INVALID_ARG;
   if (num_tokens == 0) return GR_OK;
   if (!weights || !ids || !logits || logits_stride < num_experts) return GR_ERR_INVALID_ARG;
-  if (num_experts > MAX_EXPERTS || num_groups > 64 || top_k > 64 || num_tokens > (1 << 28)) return GR_ERR_UNSUPPORTED;
+  // (16 logits a thread at most, 8 up to 512 experts: their threads are counted in 32 bits)
+  if (num_experts > MAX_EXPERTS || num_groups > 64 || top_k > 64 || num_tokens > (1 << 28) ||
+      (int64_t)num_tokens * num_experts > (1ll << 34))
+    return GR_ERR_UNSUPPORTED;
   const RouteArgs a{weights, ids, logits, logits_stride, bias, num_tokens, num_experts, top_k, score,
                     num_groups, num_groups > 1 ? top_groups : 1, renormalize, scale};
   if (dtype == GR_DTYPE_F32) launch_route<GR_DTYPE_F32>(a, stream);
@@ -641,8 +649,8 @@ extern "C" gr_status_t gr_expert_mlp(void* out, int64_t out_stride, const void* 
     return GR_ERR_UNSUPPORTED;
   const int bm = expert_tile_rows((int64_t)T * top_k, num_experts, fp8);
   const Workspace l = plan_workspace(T, top_k, num_experts, H, F, fp8, bm);
-  if (l.max_tiles * ((2ll * F + 15) / 16) > INT32_MAX - 8 || l.max_tiles * ((H + 15) / 16) > INT32_MAX - 8)
-    return GR_ERR_UNSUPPORTED;
+  const int cols = bm == 16 ? 16 : bm == 64 ? 32 : 128;  // results of a workgroup, in the narrower product
+  if (l.max_tiles * ((std::max(F, H) + cols - 1) / cols) > GRID_MAX - 8 || T > GRID_MAX) return GR_ERR_UNSUPPORTED;
   if (!workspace || !aligned(workspace, 256) || workspace_bytes < (size_t)l.bytes) return GR_ERR_WORKSPACE;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   const int rows = T * top_k, hb = (H + 127) / 128, fb = (F + 127) / 128;

@@ -7,85 +7,9 @@ namespace {
 
 constexpr int QT_THREADS = 256, QT_GROUPS = QT_THREADS / 8;
 
-struct QuantArgs {
-  uint8_t* out;
-  int64_t out_stride;
-  float* scale;
-  int64_t scale_row, scale_grp;
-  const void* x;
-  int64_t x_stride;
-  int T, K, groups;
-};
-
-// One group of 128 features per 8 lanes, 16 features a lane (wide loads and stores);
-// a workgroup's 32 groups are neighbours in their row.  Bound by memory: ROWS rows below
-// each other keep that many pairs of loads on their way, and their scales, which lie side
-// by side, reach one line together.
-template <int DT, int ROWS>
-__global__ __launch_bounds__(QT_THREADS) void quant_fp8_k(QuantArgs a) {
-  using E = Elem<DT>;
-  using S = typename E::storage;
-  constexpr bool HALF = sizeof(S) == 2;
-  constexpr int WORDS = HALF ? 8 : 16;
-  struct alignas(16) Vec { uint32_t w[WORDS]; };
-  typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
-  const uint32_t item = blockIdx.x * QT_GROUPS + (threadIdx.x >> 3);  // (below 2^31 by the entry's check)
-  const int l = threadIdx.x & 7;
-  const uint32_t block = item / (uint32_t)a.groups;
-  const int g = (int)(item - block * (uint32_t)a.groups);
-  const int64_t t0 = (int64_t)block * ROWS;
-  if (t0 >= a.T) return;  // whole 8-lane groups leave together
-  const int k = g * 128 + l * 16;
-  // (unconditional, past the end the last again: a load in a branch of its own would be waited for there)
-  const S* x = static_cast<const S*>(a.x) + (k < a.K ? k : 0);
-  Vec in[ROWS];
-#pragma unroll
-  for (int j = 0; j < ROWS; ++j) in[j] = *reinterpret_cast<const Vec*>(x + min(t0 + j, (int64_t)a.T - 1) * a.x_stride);
-#pragma unroll
-  for (int j = 0; j < ROWS; ++j) {
-    if (j > 0 && t0 + j >= a.T) break;
-    float v[16];
-    uint32_t m = 0;
-    float v_least;  // the smallest magnitude but 0
-    if (k >= a.K) in[j] = Vec{};
-    if constexpr (HALF) {  // magnitudes of 16-bit values order as their bits do, two at a time
-      u16x2 most = {0, 0}, least = {0xFFFF, 0xFFFF};
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const uint32_t w = in[j].w[i];
-        const u16x2 mag = __builtin_bit_cast(u16x2, w & 0x7FFF7FFFu);
-        most = __builtin_elementwise_max(most, mag);
-        least = __builtin_elementwise_min(least, (u16x2)(mag - (u16x2){1, 1}));
-        v[2 * i] = E::to_float((uint16_t)w);
-        v[2 * i + 1] = E::to_float((uint16_t)(w >> 16));
-      }
-      m = __builtin_bit_cast(uint32_t, E::to_float(max(most[0], most[1])));
-      const uint16_t one = min(least[0], least[1]);  // the smallest but 0, less one; 0xFFFF: none
-      v_least = one == 0xFFFF ? INFINITY : E::to_float((uint16_t)(one + 1));
-    } else {
-      uint32_t least = ~0u;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        v[i] = __builtin_bit_cast(float, in[j].w[i]);
-        m = max(m, in[j].w[i] & 0x7FFFFFFFu);
-        least = min(least, (in[j].w[i] & 0x7FFFFFFFu) - 1u);
-      }
-      v_least = least == ~0u ? INFINITY : __builtin_bit_cast(float, least + 1u);
-    }
-    // over the 8 lanes, by DPP moves: the xor of 1 and 2, a mirror of 8
-    m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0xB1, 0xf, 0xf, true));
-    m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x4E, 0xf, 0xf, true));
-    m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x141, 0xf, 0xf, true));
-    const float s = quant_scale(m), r = 1.0f / s;
-    const int64_t t = t0 + j;
-    if (k < a.K) {
-      float q[16];
-      quant_values(v, s, r, v_least < s * QUANT_LOW, q);
-      *reinterpret_cast<u32x4_t*>(a.out + t * a.out_stride + k) =
-          u32x4_t{fp8_pack4(q), fp8_pack4(q + 4), fp8_pack4(q + 8), fp8_pack4(q + 12)};
-    }
-    if (l == 0) a.scale[t * a.scale_row + g * a.scale_grp] = s;
-  }
+template <int DT, int ROWS> __global__ __launch_bounds__(QT_THREADS) void quant_fp8_k(QuantArgs a) {
+  // (items: below 2^31 by the entry's check)
+  quant_group<DT, ROWS>(a, blockIdx.x * QT_GROUPS + (threadIdx.x >> 3), threadIdx.x & 7);
 }
 
 // The tile with the least estimated time, over the workgroups of the XCD that gets
@@ -154,22 +78,6 @@ void launch_linear_fp8(const MmArgs& a, hipStream_t stream) {
 
 }  // namespace
 
-gr_status_t launch_quant_fp8(void* out, int64_t out_stride, float* scale, int64_t scale_row, int64_t scale_group,
-                             const void* x, int64_t x_stride, int num_tokens, int features, int dtype,
-                             hipStream_t stream) {
-  QuantArgs a{static_cast<uint8_t*>(out), out_stride, scale, scale_row, scale_group, x, x_stride,
-              num_tokens, features, (features + 127) / 128};
-  // rows below each other once that still leaves eight workgroups to a CU
-  const int rows = (int64_t)num_tokens * a.groups >= 2ll * QT_GROUPS * 8 * 256 ? 2 : 1;
-  const int64_t items = ((int64_t)num_tokens + rows - 1) / rows * a.groups, per = QT_GROUPS;
-  const dim3 grid((unsigned)((items + per - 1) / per)), block(QT_THREADS);
-  auto go = [&](auto one, auto two) { hipLaunchKernelGGL(rows == 2 ? two : one, grid, block, 0, stream, a); };
-  if (dtype == GR_DTYPE_F32) go(quant_fp8_k<GR_DTYPE_F32, 1>, quant_fp8_k<GR_DTYPE_F32, 2>);
-  else if (dtype == GR_DTYPE_F16) go(quant_fp8_k<GR_DTYPE_F16, 1>, quant_fp8_k<GR_DTYPE_F16, 2>);
-  else go(quant_fp8_k<GR_DTYPE_BF16, 1>, quant_fp8_k<GR_DTYPE_BF16, 2>);
-  return launch_status();
-}
-
 }  // namespace gr
 
 using namespace gr;
@@ -188,8 +96,16 @@ extern "C" gr_status_t gr_quant_fp8(void* out, int64_t out_stride, float* scale,
   if (features % 16 != 0 || !aligned(x, 16) || x_stride * dtype_size(dtype) % 16 != 0 || !aligned(out, 16) ||
       out_stride % 16 != 0 || !aligned(scale, 4) || (int64_t)num_tokens * ((features + 127) / 128) > (1 << 28))
     return GR_ERR_UNSUPPORTED;
-  return launch_quant_fp8(out, out_stride, scale, scale_row, scale_group, x, x_stride, num_tokens, features, dtype,
-                          stream);
+  const QuantArgs a{static_cast<uint8_t*>(out), out_stride, scale, scale_row, scale_group, x, x_stride,
+                    num_tokens, features, (features + 127) / 128};
+  const int rows = quant_rows(num_tokens, a.groups);
+  const int64_t items = ((int64_t)num_tokens + rows - 1) / rows * a.groups;
+  const dim3 grid((unsigned)((items + QT_GROUPS - 1) / QT_GROUPS)), block(QT_THREADS);
+  auto go = [&](auto one, auto two) { hipLaunchKernelGGL(rows == 2 ? two : one, grid, block, 0, stream, a); };
+  if (dtype == GR_DTYPE_F32) go(quant_fp8_k<GR_DTYPE_F32, 1>, quant_fp8_k<GR_DTYPE_F32, 2>);
+  else if (dtype == GR_DTYPE_F16) go(quant_fp8_k<GR_DTYPE_F16, 1>, quant_fp8_k<GR_DTYPE_F16, 2>);
+  else go(quant_fp8_k<GR_DTYPE_BF16, 1>, quant_fp8_k<GR_DTYPE_BF16, 2>);
+  return launch_status();
 }
 
 extern "C" gr_status_t gr_linear_fp8(void* out, int64_t out_stride, float* out_scale, int64_t out_scale_row,

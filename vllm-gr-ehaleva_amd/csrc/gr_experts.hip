@@ -5,10 +5,6 @@
 
 namespace gr {
 
-gr_status_t launch_quant_fp8(void* out, int64_t out_stride, float* scale, int64_t scale_row, int64_t scale_group,
-                             const void* x, int64_t x_stride, int num_tokens, int features, int dtype,
-                             hipStream_t stream);
-
 namespace {
 
 // ---- routing -----------------------------------------------------------------
@@ -388,8 +384,7 @@ __device__ inline void plan_count(const PlanArgs& a, const int (&e)[PLAN_PER], i
 }
 
 // more choices than one workgroup sorts: how many of each expert every one of them has
-__global__ __launch_bounds__(PLAN_THREADS) void expert_count_k(PlanArgs a) {
-  __shared__ int n[MAX_EXPERTS];
+__device__ __forceinline__ void expert_count(const PlanArgs& a, int* n) {
   int e[PLAN_PER];
   plan_load(a, e, true);
   plan_count(a, e, n);
@@ -399,9 +394,7 @@ __global__ __launch_bounds__(PLAN_THREADS) void expert_count_k(PlanArgs a) {
 // Sorts this workgroup's choices by expert into the rows of the experts' tiles.
 // Where a row lands within its expert differs from run to run (an atomic in LDS
 // hands out the places); its result does not.
-__global__ __launch_bounds__(PLAN_THREADS) void expert_plan_k(PlanArgs a) {
-  __shared__ int next[MAX_EXPERTS];
-  __shared__ int part[PLAN_THREADS / 64];
+__device__ __forceinline__ void expert_plan(const PlanArgs& a, int* next, int* part) {
   const int tid = threadIdx.x;
   int e[PLAN_PER];
   plan_load(a, e, a.blocks == 1);
@@ -430,6 +423,27 @@ __global__ __launch_bounds__(PLAN_THREADS) void expert_plan_k(PlanArgs a) {
 #pragma unroll
   for (int i = 0; i < PLAN_PER; ++i)
     if (e[i] >= 0) a.slot[atomicAdd(&next[e[i]], 1)] = blockIdx.x * PLAN_ROWS + i * PLAN_THREADS + tid;
+}
+
+__global__ __launch_bounds__(PLAN_THREADS) void expert_count_k(PlanArgs a) {
+  __shared__ int n[MAX_EXPERTS];
+  expert_count(a, n);
+}
+__global__ __launch_bounds__(PLAN_THREADS) void expert_plan_k(PlanArgs a) {
+  __shared__ int next[MAX_EXPERTS], part[PLAN_THREADS / 64];
+  expert_plan(a, next, part);
+}
+// With e4m3 weights the tokens are quantised by the workgroups behind those that sort
+// (or count, where several do): a launch less, and the sort's waits are theirs alone
+// (512 tokens 6.1 us against 4.8 + 5.8 one after the other).
+template <int DT, int ROWS> __global__ __launch_bounds__(PLAN_THREADS) void expert_start_k(PlanArgs a, QuantArgs q) {
+  __shared__ int next[MAX_EXPERTS], part[PLAN_THREADS / 64];
+  if ((int)blockIdx.x >= a.blocks)
+    quant_group<DT, ROWS>(q, (blockIdx.x - a.blocks) * (PLAN_THREADS / 8) + (threadIdx.x >> 3), threadIdx.x & 7);
+  else if (a.blocks > 1)
+    expert_count(a, next);
+  else
+    expert_plan(a, next, part);
 }
 
 // ---- out[t] = sum_j weights[t, j] * y[t, j] ---------------------------------------
@@ -658,8 +672,21 @@ extern "C" gr_status_t gr_expert_mlp(void* out, int64_t out_stride, const void* 
   PlanArgs p{ids, rows, num_experts, bm, l.blocks, reinterpret_cast<int32_t*>(ws + l.hist),
              reinterpret_cast<int32_t*>(ws + l.slot), reinterpret_cast<int4*>(ws + l.tiles),
              reinterpret_cast<int32_t*>(ws + l.num_tiles), dev_status};
-  if (l.blocks > 1) hipLaunchKernelGGL(expert_count_k, dim3(l.blocks), dim3(PLAN_THREADS), 0, stream, p);
-  hipLaunchKernelGGL(expert_plan_k, dim3(l.blocks), dim3(PLAN_THREADS), 0, stream, p);
+  float* xs = reinterpret_cast<float*>(ws + l.xs);
+  if (fp8) {
+    const QuantArgs q{ws + l.x8, H, xs, 1, T, x, x_stride, T, H, hb};
+    const int quant = quant_rows(T, hb);
+    const int64_t items = ((int64_t)T + quant - 1) / quant * hb, per = PLAN_THREADS / 8;
+    const dim3 grid((unsigned)(l.blocks + (items + per - 1) / per));
+    auto go = [&](auto one, auto two) {
+      hipLaunchKernelGGL(quant == 2 ? two : one, grid, dim3(PLAN_THREADS), 0, stream, p, q);
+    };
+    if (dtype == GR_DTYPE_F16) go(expert_start_k<GR_DTYPE_F16, 1>, expert_start_k<GR_DTYPE_F16, 2>);
+    else go(expert_start_k<GR_DTYPE_BF16, 1>, expert_start_k<GR_DTYPE_BF16, 2>);
+  } else if (l.blocks > 1) {
+    hipLaunchKernelGGL(expert_count_k, dim3(l.blocks), dim3(PLAN_THREADS), 0, stream, p);
+  }
+  if (!fp8 || l.blocks > 1) hipLaunchKernelGGL(expert_plan_k, dim3(l.blocks), dim3(PLAN_THREADS), 0, stream, p);
 
   const int esize = fp8 ? 1 : 2;
   MmArgs up{};
@@ -679,8 +706,6 @@ extern "C" gr_status_t gr_expert_mlp(void* out, int64_t out_stride, const void* 
   up.slot = p.slot;
   up.gather = top_k;
   if (fp8) {
-    float* xs = reinterpret_cast<float*>(ws + l.xs);
-    launch_quant_fp8(ws + l.x8, H, xs, 1, T, x, x_stride, T, H, dtype, stream);
     up.x = ws + l.x8;
     up.x_stride = H;
     up.xs = xs;

@@ -740,9 +740,9 @@ def _blocks(n: int) -> int:
     return -(-n // FP8_BLOCK)
 
 
-def _row_stride(t: torch.Tensor) -> int:
+def _row_stride(t: torch.Tensor, rows: int, features: int) -> int:
     """Elements from row to row; of a single row, whose stride means nothing, its length."""
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    return t.stride(0) if rows > 1 else features
 
 
 def _launch(dev: torch.device, name: str, *args) -> None:
@@ -787,8 +787,8 @@ def quant_fp8(x: torch.Tensor, *, out: torch.Tensor | None = None, scale: torch.
         scale = _new_row_scales(T, K, dev)
     else:
         _row_scales("scale", scale, T, K)
-    _launch(dev, "gr_quant_fp8", out.data_ptr(), _row_stride(out), scale.data_ptr(), scale.stride(0), scale.stride(1),
-            x.data_ptr(), _row_stride(x), T, K, _dtype_code(x), _stream(dev))
+    _launch(dev, "gr_quant_fp8", out.data_ptr(), _row_stride(out, T, K), scale.data_ptr(), *scale.stride(),
+            x.data_ptr(), _row_stride(x, T, K), T, K, _dtype_code(x), _stream(dev))
     return out, scale
 
 
@@ -808,8 +808,8 @@ def linear_fp8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale:
     if x.dtype != torch.float8_e4m3fn or w.dtype != torch.float8_e4m3fn:
         raise ValueError("x and w must be float8_e4m3fn")
     T, K = x.shape
-    rows = w.shape[0]
-    if w.shape[1] != K or (swiglu and rows % 2):
+    rows, in_features = w.shape
+    if in_features != K or (swiglu and rows % 2):
         raise ValueError("w must be [out_features, in_features] (twice the rows with swiglu)")
     N = rows // 2 if swiglu else rows
     _row_scales("x_scale", x_scale, T, K)
@@ -834,9 +834,9 @@ def linear_fp8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale:
         _row_scales("out_scale", out_scale, T, N)
     elif quantized:
         out_scale = _new_row_scales(T, N, dev)
-    _launch(dev, "gr_linear_fp8", out.data_ptr(), _row_stride(out), _ptr(out_scale),
-            *(out_scale.stride() if quantized else (0, 0)), x.data_ptr(), _row_stride(x), x_scale.data_ptr(),
-            x_scale.stride(0), x_scale.stride(1), w.data_ptr(), _row_stride(w), w_scale.data_ptr(), T, N, K,
+    _launch(dev, "gr_linear_fp8", out.data_ptr(), _row_stride(out, T, N), _ptr(out_scale),
+            *(out_scale.stride() if quantized else (0, 0)), x.data_ptr(), _row_stride(x, T, K), x_scale.data_ptr(),
+            *x_scale.stride(), w.data_ptr(), _row_stride(w, rows, K), w_scale.data_ptr(), T, N, K,
             int(swiglu), _C.GR_DTYPE_FP8_E4M3 if quantized else _dtype_code(out), _stream(dev))
     return (out, out_scale) if quantized else out
 
@@ -863,7 +863,7 @@ def route_experts(logits: torch.Tensor, top_k: int, *, score: str = "softmax", b
         raise ValueError("top_k must be at least 1")
     weights = torch.empty((T, top_k), dtype=torch.float32, device=dev)
     ids = torch.empty((T, top_k), dtype=torch.int32, device=dev)
-    _launch(dev, "gr_route_experts", weights.data_ptr(), ids.data_ptr(), logits.data_ptr(), _row_stride(logits),
+    _launch(dev, "gr_route_experts", weights.data_ptr(), ids.data_ptr(), logits.data_ptr(), _row_stride(logits, T, E),
             _ptr(bias), T, E, top_k, _SCORES[score], int(num_groups), int(top_groups), int(bool(renormalize)),
             float(scale), _dtype_code(logits), _stream(dev))
     return weights, ids
@@ -915,9 +915,10 @@ def expert_mlp(x: torch.Tensor, gate_up: torch.Tensor, down: torch.Tensor, weigh
     need = expert_mlp_workspace_bytes(T, k, E, H, F, fp8)
     if workspace is None:
         workspace = torch.empty(need, dtype=torch.uint8, device=dev)
-    _launch(dev, "gr_expert_mlp", out.data_ptr(), _row_stride(out), x.data_ptr(), _row_stride(x), gate_up.data_ptr(),
-            _ptr(gate_up_scale), down.data_ptr(), _ptr(down_scale), weights.data_ptr(), ids.data_ptr(), T, k, E, H, F,
-            _dtype_code(x), workspace.data_ptr(), workspace.numel() * workspace.element_size(), _ptr(status), _stream(dev))
+    _launch(dev, "gr_expert_mlp", out.data_ptr(), _row_stride(out, T, H), x.data_ptr(), _row_stride(x, T, H),
+            gate_up.data_ptr(), _ptr(gate_up_scale), down.data_ptr(), _ptr(down_scale), weights.data_ptr(),
+            ids.data_ptr(), T, k, E, H, F, _dtype_code(x), workspace.data_ptr(),
+            workspace.numel() * workspace.element_size(), _ptr(status), _stream(dev))
     return out
 
 

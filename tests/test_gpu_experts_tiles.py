@@ -38,7 +38,7 @@ def test_linear_quantised_tiles(device, M, N, K, swiglu):
     check_quantised(*ops.linear_fp8(x8, xs, w8, ws, swiglu=swiglu, quantized=True), y, err)
 
 
-# rows per expert of 4 and fewer, to 80, 512 and beyond (16-bit weights: tiles of 16 to 256 rows; 8-bit: 32 and 128)
+# rows per expert of 8 and fewer, some dozens, hundreds and more (16-bit weights: tiles of 16 to 256 rows; 8-bit: 32 and 128)
 @pytest.mark.parametrize("fp8", [False, True])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("T,E,k,H,F", [(8, 16, 4, 144, 272), (200, 3, 1, 400, 80), (601, 3, 2, 272, 208),

@@ -404,7 +404,8 @@ __device__ __forceinline__ void expert_plan(const PlanArgs& a, int* next, int* p
     total = next[tid];
     __syncthreads();
   } else if (tid < a.E) {
-    for (int b = 0; b < a.blocks; ++b) {
+#pragma unroll 8
+    for (int b = 0; b < a.blocks; ++b) {  // (eight loads on their way)
       const int n = a.hist[(int64_t)b * a.E + tid];
       if (b < (int)blockIdx.x) before += n;
       total += n;
@@ -509,13 +510,13 @@ struct Workspace {
 // weights' way from memory: then more workgroups on a CU count, later the rows a
 // weight is read for.  Measured (64 experts of 768 features, hidden 2048, 8 of them a
 // token; us, by tile rows; 16-bit weights, then e4m3):
-//   rows an expert   1             8              32              64              256             1024
-//   16 / 64        86 / 96      145 / 143      285 / 159        - / 190         - / 432         -
-//   128 / 256     105 / 120     162 / 186      172 / 190       197 / 213       300 / 322     934 / 867
-//   32 / 128       61 / 78       82 / 124      104 / 132       126 / 147      (280 at 128)    - / 920
+//   rows an expert    1            8            32           64           96          256          512         1024
+//   16 / 64       95 / 107    139 / 139    296 / 146    511 / 182    724 / 206     - / 407     - / 696    - / 1216
+//   128 / 256    140 / 165    156 / 181    164 / 187    175 / 197    183 / 208   280 / 310   448 / 435   808 / 744
+//   32 / 128      58 / 75      77 / 119     97 / 123    113 / 127    151 / 132   294 / 255   495 / 415   923 / 763
 int expert_tile_rows(int64_t rows, int E, bool fp8) {
-  if (fp8) return rows <= 112ll * E ? 32 : 128;
-  return rows <= 4ll * E ? 16 : rows <= 80ll * E ? 64 : rows <= 512ll * E ? 128 : 256;
+  if (fp8) return rows <= 80ll * E ? 32 : 128;
+  return rows <= 8ll * E ? 16 : rows <= 56ll * E ? 64 : rows <= 448ll * E ? 128 : 256;
 }
 
 Workspace plan_workspace(int T, int k, int E, int H, int F, bool fp8, int bm) {

@@ -6,7 +6,8 @@ import pytest
 
 from tests.test_device_code import VMEM, _disassembly, _kernels, _scratch_sizes
 
-NAMES = ("block_mm", "few_mm", "quant_fp8_k", "route_experts_k", "expert_count_k", "expert_plan_k", "expert_combine_k")
+NAMES = ("block_mm", "few_mm", "quant_fp8_k", "route_experts_k", "expert_count_k", "expert_plan_k", "expert_start_k",
+         "expert_combine_k")
 
 
 def test_kernels_keep_no_stack():

@@ -38,7 +38,7 @@ def test_linear_quantised_tiles(device, M, N, K, swiglu):
     check_quantised(*ops.linear_fp8(x8, xs, w8, ws, swiglu=swiglu, quantized=True), y, err)
 
 
-# rows per expert of 8 and fewer, some dozens, hundreds and more (16-bit weights: tiles of 16 to 256 rows; 8-bit: 32 and 128)
+# rows per expert of 8 and fewer, some dozens, hundreds and more (16-bit weights: tiles of 16 to 256 rows; 8-bit: 32, 128)
 @pytest.mark.parametrize("fp8", [False, True])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("T,E,k,H,F", [(8, 16, 4, 144, 272), (200, 3, 1, 400, 80), (601, 3, 2, 272, 208),
@@ -120,3 +120,26 @@ def test_two_graphs_of_one_layer(device):
         torch.cuda.synchronize()
         for _, out, want, _ in runs:
             assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("M", [1, 300, 2000])
+def test_gate_far_below_zero(device, M):
+    """A gate whose sigmoid is below the normal float32 numbers still counts beside a huge
+    factor: the exponential of g is off by |g| log2(e) 2^-24 and half a unit of the
+    product g log2(e), 2^-18 of a value near 128."""
+    N, K = 256, 128
+    gates = [-88.0, -80.0, -72.0, -1.0, 0.0, 80.0]
+    x = torch.zeros(M, K)
+    x[:, 0] = 1
+    w = torch.zeros(2 * N, K)
+    w[:N, 0] = torch.tensor(gates).repeat(N // len(gates) + 1)[:N]
+    w[N:, 0] = 448
+    ws = torch.ones(4, 1)
+    ws[2:] = 2.0 ** 90
+    to8 = lambda t: t.to(torch.float8_e4m3fn).to(device)
+    got = ops.linear_fp8(to8(x), torch.ones(M, 1, device=device), to8(w), ws.to(device), swiglu=True,
+                         out_dtype=torch.float32).cpu().double()
+    g = w[:N, 0].double()
+    want = g * torch.sigmoid(g) * 448 * 2.0 ** 90
+    assert (want[g == -88].abs() > 1e-8).all()
+    assert ((got - want).abs() <= want.abs() * 2.0 ** -16).all()

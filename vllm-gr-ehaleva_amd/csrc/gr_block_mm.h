@@ -487,7 +487,8 @@ struct Mm {
     for (int u = 0; u < 4; ++u) {
       if constexpr (GATED) {
         const float g = acc[2 * i][j][u];
-        v[u] = g * __builtin_amdgcn_rcpf(1.0f + __expf(-g)) * acc[2 * i + 1][j][u];
+        // (2^-8: the reciprocal instruction loses what is below the normal numbers, from a gate of -87 on)
+        v[u] = g * 0x1p-8f * __builtin_amdgcn_rcpf(fmaf(__expf(-g), 0x1p-8f, 0x1p-8f)) * acc[2 * i + 1][j][u];
       } else {
         v[u] = acc[i][j][u];
       }

@@ -44,7 +44,9 @@ gr_status_t gr_quant_fp8(void* out, int64_t out_stride, float* scale, int64_t sc
  * out = silu(gate) * up, out_features % 16 == 0.
  * out: out_dtype float32, fp16 or bf16, rounded once; or GR_DTYPE_FP8_E4M3: the
  * float32 results quantised as gr_quant_fp8 does, with out_scale at strides
- * out_scale_row / out_scale_group (needs out_features % 16 == 0).
+ * out_scale_row / out_scale_group (needs out_features % 16 == 0).  out is 16-byte
+ * aligned for float32 and 8-byte for 16 bits, at any row stride; e4m3 rows are each
+ * 4-byte aligned.
  * Sums are float32 throughout for a float32 or e4m3 result.  For a 16-bit one the
  * matrix core adds the e4m3 products, in groups of 8 whose members are cut off
  * below 2^-13 of the largest (about 1.5e-5 of an ordinary result); the groups'

@@ -801,7 +801,8 @@ def linear_fp8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale:
     gr_experts.h.  ``swiglu``: ``silu(gate) * up`` of the two halves of ``w``'s
     rows, whose block scales stand one half's after the other's.  Returns ``[T, N]``
     of ``out_dtype`` (float32, fp16, bf16), or with ``quantized`` the pair
-    ``quant_fp8`` would give of the float32 results."""
+    ``quant_fp8`` would give of the float32 results.  ``out`` is aligned to 16 bytes
+    (float32), 8 (16 bits) or, each of its rows, 4 (e4m3); ``out_scale`` may have any strides."""
     dev = _need_cuda(x, x_scale, w, w_scale, out, out_scale)
     _rows("x", x)
     _rows("w", w)
@@ -816,15 +817,8 @@ def linear_fp8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale:
     if (w_scale.dtype != torch.float32 or w_scale.shape != (_blocks(N) * (2 if swiglu else 1), _blocks(K))
             or not w_scale.is_contiguous()):
         raise ValueError("w_scale must be a contiguous float32 [blocks of rows, blocks of features] tensor")
-    if quantized and T <= 64 and N % 16 == 0:
-        # a group of 128 results is one workgroup's, too few of them for few rows: 8 x 6144 SwiGLU columns of 2048
-        # features 24.6 us in one launch, 14 in two; 128 rows 25 either way
-        y = linear_fp8(x, x_scale, w, w_scale, swiglu=swiglu, out_dtype=torch.float32)
-        return quant_fp8(y, out=out, scale=out_scale)
     odt = torch.float8_e4m3fn if quantized else out_dtype
-    if out is None:
-        out = torch.empty((T, N), dtype=odt, device=dev)
-    else:
+    if out is not None:
         _rows("out", out)
         if out.shape != (T, N) or out.dtype != odt:
             raise ValueError("out must be [tokens, out_features] of the result's type")
@@ -832,7 +826,16 @@ def linear_fp8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale:
         if not quantized:
             raise ValueError("out_scale goes with quantized=True")
         _row_scales("out_scale", out_scale, T, N)
-    elif quantized:
+    if (quantized and T <= 64 and N % 16 == 0
+            and (out is None or (out.data_ptr() % 16 == 0 and _row_stride(out, T, N) % 16 == 0))):
+        # a group of 128 results is one workgroup's, too few of them for few rows: 8 x 6144 SwiGLU columns of 2048
+        # features 24.6 us in one launch, 14 in two; 128 rows 25 either way.  (quant_fp8 stores 16 bytes at a time;
+        # rows that are not aligned so take the one launch.)
+        y = linear_fp8(x, x_scale, w, w_scale, swiglu=swiglu, out_dtype=torch.float32)
+        return quant_fp8(y, out=out, scale=out_scale)
+    if out is None:
+        out = torch.empty((T, N), dtype=odt, device=dev)
+    if quantized and out_scale is None:
         out_scale = _new_row_scales(T, N, dev)
     _launch(dev, "gr_linear_fp8", out.data_ptr(), _row_stride(out, T, N), _ptr(out_scale),
             *(out_scale.stride() if quantized else (0, 0)), x.data_ptr(), _row_stride(x, T, K), x_scale.data_ptr(),

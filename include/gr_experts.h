@@ -41,7 +41,9 @@ gr_status_t gr_quant_fp8(void* out, int64_t out_stride, float* scale, int64_t sc
  * [ceil(out_features / 128), ceil(in_features / 128)] contiguous.
  * swiglu: w is [2 * out_features, in_features] (gate | up), w_scale
  * [2 * ceil(out_features / 128), ...] (gate's blocks, then up's) and
- * out = silu(gate) * up, out_features % 16 == 0.
+ * out = silu(gate) * up, out_features % 16 == 0.  silu is within
+ * 2^-20 + |gate| 2^-23 of itself; a gate below -91.8, where it is no normal float32
+ * number, may count as 0.
  * out: out_dtype float32, fp16 or bf16, rounded once; or GR_DTYPE_FP8_E4M3: the
  * float32 results quantised as gr_quant_fp8 does, with out_scale at strides
  * out_scale_row / out_scale_group (needs out_features % 16 == 0).  out is 16-byte

@@ -487,8 +487,10 @@ struct Mm {
     for (int u = 0; u < 4; ++u) {
       if constexpr (GATED) {
         const float g = acc[2 * i][j][u];
-        // (2^-8: the reciprocal instruction loses what is below the normal numbers, from a gate of -87 on)
-        v[u] = g * 0x1p-8f * __builtin_amdgcn_rcpf(fmaf(__expf(-g), 0x1p-8f, 0x1p-8f)) * acc[2 * i + 1][j][u];
+        // (g sigmoid(g) = 2^-7 g / (2^-7 + 2^(-g log2(e) - 7)): neither the power nor its reciprocal leaves the normal
+        // numbers before the product does, at a gate of -91.8)
+        const float e = __builtin_amdgcn_exp2f(fmaf(g, -LOG2E, -7.0f));
+        v[u] = g * 0x1p-7f * __builtin_amdgcn_rcpf(e + 0x1p-7f) * acc[2 * i + 1][j][u];
       } else {
         v[u] = acc[i][j][u];
       }

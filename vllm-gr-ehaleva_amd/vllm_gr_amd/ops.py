@@ -67,6 +67,14 @@ def _need_cuda(*ts: torch.Tensor | None) -> torch.device:
     return dev
 
 
+def _workspace_bytes(t: torch.Tensor) -> int:
+    """Bytes that a caller's workspace holds: of an expanded or strided tensor its
+    elements would not say."""
+    if not t.is_contiguous():
+        raise ValueError("workspace must be contiguous")
+    return t.numel() * t.element_size()
+
+
 def _need_i32(name: str, t: torch.Tensor) -> None:
     if t.dtype != torch.int32 or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous int32 tensor")
@@ -528,7 +536,7 @@ def beam_prune_topk(logits: torch.Tensor, cum: torch.Tensor, k: int, eos_token_i
         parent, token, score, eos_score = out
         if score.dtype != sdt or eos_score.dtype != sdt:
             raise ValueError("score / eos_score must have cum's dtype")
-    ws_bytes = workspace.numel() * workspace.element_size()
+    ws_bytes = _workspace_bytes(workspace)
     if catalog is not None:
         _need_cuda(catalog.node_start, catalog.child_token, catalog.child_node)
         for name, t in (("node_start", catalog.node_start), ("child_token", catalog.child_token),
@@ -883,7 +891,7 @@ def expert_mlp(x: torch.Tensor, gate_up: torch.Tensor, down: torch.Tensor, weigh
     float8_e4m3fn with ``gate_up_scale [E, 2 ceil(F / 128), ceil(H / 128)]`` and
     ``down_scale [E, ceil(H / 128), ceil(F / 128)]``.  An id below 0 adds nothing;
     one of E or more adds nothing and is flagged in ``status``.  ``workspace``: uint8,
-    ``expert_mlp_workspace_bytes`` of it (allocated when None)."""
+    contiguous, ``expert_mlp_workspace_bytes`` of it (allocated when None)."""
     dev = _need_cuda(x, gate_up, down, weights, ids, gate_up_scale, down_scale, out, workspace, status)
     _rows("x", x)
     T, H = x.shape
@@ -921,7 +929,7 @@ def expert_mlp(x: torch.Tensor, gate_up: torch.Tensor, down: torch.Tensor, weigh
     _launch(dev, "gr_expert_mlp", out.data_ptr(), _row_stride(out, T, H), x.data_ptr(), _row_stride(x, T, H),
             gate_up.data_ptr(), _ptr(gate_up_scale), down.data_ptr(), _ptr(down_scale), weights.data_ptr(),
             ids.data_ptr(), T, k, E, H, F, _dtype_code(x), workspace.data_ptr(),
-            workspace.numel() * workspace.element_size(), _ptr(status), _stream(dev))
+            _workspace_bytes(workspace), _ptr(status), _stream(dev))
     return out
 
 

@@ -613,9 +613,14 @@ def beam_prune_topk_noalloc(logits: torch.Tensor, cum: torch.Tensor, k: int, eos
 # ---- fused decoder stages (include/gr_decoder.h) ---------------------------
 
 
+_INT_MAX = 2 ** 31 - 1  # sizes are C ints, to which ctypes cuts a larger number off without a word
+
+
 def _rows(name: str, t: torch.Tensor) -> None:
     if t.dim() != 2 or t.stride(1) != 1:
         raise ValueError(f"{name} must be a [tokens, features] tensor with contiguous features")
+    if max(t.shape) > _INT_MAX:
+        raise ValueError(f"{name} has more than 2^31 - 1 rows or features")
 
 
 def linear_supported(x: torch.Tensor, w: torch.Tensor, swiglu: bool = False) -> bool:
@@ -869,13 +874,15 @@ def route_experts(logits: torch.Tensor, top_k: int, *, score: str = "softmax", b
         raise ValueError("score must be 'softmax' or 'sigmoid'")
     if bias is not None and (bias.shape != (E,) or bias.dtype != torch.float32 or not bias.is_contiguous()):
         raise ValueError("bias must be a contiguous float32 [experts] tensor")
-    top_k = int(top_k)
+    top_k, num_groups, top_groups = int(top_k), int(num_groups), int(top_groups)
     if top_k < 1:
         raise ValueError("top_k must be at least 1")
+    if top_k > E or not 1 <= top_groups <= num_groups <= E:
+        raise ValueError("top_k and num_groups are at most the number of experts, top_groups at most num_groups")
     weights = torch.empty((T, top_k), dtype=torch.float32, device=dev)
     ids = torch.empty((T, top_k), dtype=torch.int32, device=dev)
     _launch(dev, "gr_route_experts", weights.data_ptr(), ids.data_ptr(), logits.data_ptr(), _row_stride(logits, T, E),
-            _ptr(bias), T, E, top_k, _SCORES[score], int(num_groups), int(top_groups), int(bool(renormalize)),
+            _ptr(bias), T, E, top_k, _SCORES[score], num_groups, top_groups, int(bool(renormalize)),
             float(scale), _dtype_code(logits), _stream(dev))
     return weights, ids
 
@@ -917,6 +924,8 @@ def expert_mlp(x: torch.Tensor, gate_up: torch.Tensor, down: torch.Tensor, weigh
     k = ids.shape[1]
     if k < 1:
         raise ValueError("ids must name at least one expert a token")
+    if max(k, E, F) > _INT_MAX:
+        raise ValueError("ids, gate_up or down has a size above 2^31 - 1")
     if out is None:
         out = torch.empty((T, H), dtype=x.dtype, device=dev)
     else:

@@ -243,6 +243,42 @@ def _swiglu(x: torch.Tensor, w: torch.Tensor) -> torch.Tensor:
     return ops.linear(x, w, swiglu=True) if _own_linear(x, w, True) else ops.silu_mul(F.linear(x, w))
 
 
+def _check_experts(cfg: DecoderConfig) -> None:
+    """Refuses what route_experts and expert_mlp would refuse in the first forward."""
+    E, k, groups, top = cfg.num_experts, cfg.experts_per_token, cfg.router_groups, cfg.router_top_groups
+    if cfg.dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError("experts need a 16-bit dtype")
+    if cfg.hidden % 16 or cfg.expert_ffn % 16 or cfg.expert_ffn < 1 or E > 1024:
+        raise ValueError("experts need hidden and expert_ffn in multiples of 16, and are at most 1024")
+    if cfg.router_score not in ("softmax", "sigmoid"):
+        raise ValueError("router_score must be 'softmax' or 'sigmoid'")
+    if not 1 <= top <= groups <= 64 or E % groups or not 1 <= k <= min(64, E // groups * top):
+        raise ValueError("experts_per_token (64 at most) are chosen from router_top_groups of router_groups equal groups")
+
+
+def _check_quantized(cfg: DecoderConfig, weights: dict[str, torch.Tensor]) -> None:
+    """Refuses 8-bit weights that the products would refuse in the first forward."""
+    names = ("expert_gate_up", "expert_down") if cfg.num_experts else ("gate_up", "down")
+    for i in range(cfg.num_layers):
+        p = f"layers.{i}."
+        for name in (p + "qkv", p + "o", p + names[0], p + names[1]):
+            w, scale = weights.get(name), weights.get(name + "_scale")
+            if w is None or (scale is None and w.dtype != torch.float8_e4m3fn):
+                continue
+            if scale is None or w.dtype != torch.float8_e4m3fn:
+                raise ValueError(f"{name}: float8_e4m3fn weights and {name}_scale go together")
+            parts = 2 if name.endswith("gate_up") else 1  # gate's rows, then up's
+            N, K = w.shape[-2] // parts, w.shape[-1]
+            if K % 16 or w.shape[-2] % parts or (parts == 2 and N % 16):
+                raise ValueError(f"{name}: 8-bit weights need sizes in multiples of 16, not {list(w.shape)}")
+            blocks = [-(-n // ops.FP8_BLOCK) for n in (N, K)]
+            shape = (*w.shape[:-2], parts * blocks[0], blocks[1])
+            if scale.shape != shape or scale.dtype != torch.float32 or not scale.is_contiguous():
+                raise ValueError(f"{name}_scale must be a contiguous float32 {list(shape)} tensor")
+        if (p + names[0] + "_scale" in weights) != (p + names[1] + "_scale" in weights):
+            raise ValueError(f"{p}{names[0]} and {p}{names[1]} are 8-bit together or not at all")
+
+
 class SidDecoder:
     """The decoder's forward over a flat batch of tokens.
 
@@ -256,8 +292,9 @@ class SidDecoder:
     logits."""
 
     def __init__(self, cfg: DecoderConfig, weights: dict[str, torch.Tensor], *, max_position: int = 32768):
-        if cfg.num_experts and cfg.dtype not in (torch.bfloat16, torch.float16):
-            raise ValueError("experts need a 16-bit dtype")
+        if cfg.num_experts:
+            _check_experts(cfg)
+        _check_quantized(cfg, weights)
         self.cfg = cfg
         self.w = weights
         dev = weights["embed"].device

@@ -97,7 +97,7 @@ gr_status_t gr_route_experts(float* weights, int32_t* ids, const void* logits, i
  * ceil(ffn / 128)] they are e4m3, and x and the gated products are quantised as
  * gr_quant_fp8 does.  Sums are float32 (of e4m3 weights in the down product as for
  * gr_linear_fp8's 16-bit results), and with e4m3 weights or a bf16 out each expert's
- * result is rounded to fp16 times a power of two (2^-12 of a value, 2^-39 of the
+ * result is rounded to fp16 times a power of two (2^-11 of a value, 2^-39 of the
  * largest of its 16 to 64 neighbouring columns) before the sum over j, which is
  * float32 and in the order of j.
  * hidden % 16 == 0, ffn % 16 == 0; rows of x, and weights, 16-byte aligned; out

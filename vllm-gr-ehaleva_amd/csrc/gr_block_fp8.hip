@@ -63,8 +63,8 @@ void launch_linear_fp8(const MmArgs& a, hipStream_t stream) {
     // as long as two workgroups a CU hold them all (8 rows x 4096 columns 4.8 us, by 64 x 64 tiles 8.7; 64 x 4096
     // 8.5; 64 x 8192, twice that many, 14.5 against 9.5)
     const int64_t cols = (a.N + 15) / 16, few = (M + 15) / 16 * cols, few2 = (M + 31) / 32 * cols;
-    if (few <= 256 || (M <= 16 && few <= 512)) return launch_few<T, 1, 8, MODE, false>(a, (M + 15) / 16, stream);
-    if (few2 <= 512) return launch_few<T, 2, 8, MODE, false>(a, (M + 31) / 32, stream);
+    if (few <= 256 || (M <= 16 && few <= 512)) return launch_few<T, 1, MODE, false>(a, (M + 15) / 16, stream);
+    if (few2 <= 512) return launch_few<T, 2, MODE, false>(a, (M + 31) / 32, stream);
     switch (EXACT ? pick_tile(kExact, M, rows_w, stages) : pick_tile(kFast, M, rows_w, stages)) {
       case 0: launch_mm<T, 64, 64, 2, 2, 4, MODE, false, EXACT>(a, (M + 63) / 64, stream); break;
       case 1: launch_mm<T, 64, 128, 2, 2, 3, MODE, false, EXACT>(a, (M + 63) / 64, stream); break;

@@ -752,28 +752,28 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void block_mm(MmArgs a) {
 // Few rows: BM = 16 FM.  What bounds this is the weights' way from memory (or, for a
 // single projection, one round trip), so nothing is shared through LDS: every weight
 // is loaded once, by the one wave that multiplies it, straight into the registers of
-// the operand, U stages at a time, and the eight waves split the depth WK ways (wave
-// k takes stages k, k + WK, ...) and the columns 8 / WK ways, 16 columns a wave.  The
-// partial sums of the depth meet in LDS.  The rows are read by every workgroup, from L2.
-template <int XT, int FM, int WK, int MODE, bool EXPERTS>
+// the operand, U stages at a time, and the eight waves of 16 columns split the depth
+// (wave k takes stages k, k + 8, ...).  Their partial sums meet in LDS.  The rows are
+// read by every workgroup, from L2.
+template <int XT, int FM, int MODE, bool EXPERTS>
 __global__ __launch_bounds__(512) void few_mm(MmArgs a) {
   constexpr bool F8 = XT == GR_DTYPE_FP8_E4M3;
   constexpr bool GATED = MODE == MM_SWIGLU;
-  constexpr int WN = 8 / WK, FN = GATED ? 2 : 1, U = FM == 1 ? 4 : 2;
-  using M = Mm<XT, 16 * FM, 16 * FN * WN, 1, WN, MODE, EXPERTS, F8>;
-  using M1 = Mm<XT, 16, 16 * FN * WN, 1, WN, MODE, EXPERTS, F8>;  // one fragment row
+  constexpr int WK = 8, FN = GATED ? 2 : 1, U = FM == 1 ? 4 : 2;
+  using M = Mm<XT, 16 * FM, 16 * FN, 1, 1, MODE, EXPERTS, F8>;
+  using M1 = Mm<XT, 16, 16 * FN, 1, 1, MODE, EXPERTS, F8>;  // one fragment row
   static_assert(MODE == MM_PLAIN || MODE == MM_SWIGLU, "results that are not quantised");
-  constexpr int LDS = WK * WN * FM * FN * 1024 + 8 * 16 * 80;
+  constexpr int LDS = WK * FM * FN * 1024 + 8 * 16 * 80;
   __shared__ __attribute__((aligned(16))) uint8_t lds[LDS];
   MmTile t;
   if (!M::tile(a, t)) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int wk = wave / WN, wn = wave % WN, r16 = lane & 15, q = lane >> 4;
+  const int r16 = lane & 15, q = lane >> 4;
   const int n = (a.kbytes + 127) >> 7, nb = (a.N + 127) >> 7;
-  const int col = min(t.n0 + wn * 16 + r16, a.N - 1);
+  const int col = min(t.n0 + r16, a.N - 1);
   const uint8_t* w0 = t.w + (int64_t)col * a.w_stride + q * 16;
   const int64_t up = (int64_t)a.N * a.w_stride;
-  const float* ws = F8 ? t.ws + (int64_t)min((t.n0 + wn * 16) >> 7, nb - 1) * n : nullptr;
+  const float* ws = F8 ? t.ws + (int64_t)min(t.n0 >> 7, nb - 1) * n : nullptr;
   const uint8_t* x0[FM];
   const float* xs[FM];
 #pragma unroll
@@ -793,7 +793,7 @@ __global__ __launch_bounds__(512) void few_mm(MmArgs a) {
   for (int i = 0; i < FN; ++i)
 #pragma unroll
     for (int j = 0; j < FM; ++j) acc[i][j] = mm4_t{0.f, 0.f, 0.f, 0.f};
-  for (int s0 = wk; s0 < n; s0 += WK * U) {
+  for (int s0 = wave; s0 < n; s0 += WK * U) {
     mm8i_t w[U][FN], x[U][FM];
     float sx[U][FM], sw[U][FN];
 #pragma unroll
@@ -827,22 +827,22 @@ __global__ __launch_bounds__(512) void few_mm(MmArgs a) {
 #pragma unroll
     for (int i = 0; i < FN; ++i) part[((wave * FM + j) * FN + i) * 64 + lane] = acc[i][j];
   __syncthreads();
-  // wave (k, n) finishes fragment rows k, k + WK, ... of column fragment n
-  for (int j = wk; j < FM; j += WK) {
+  // wave j finishes fragment row j
+  if (const int j = wave; j < FM) {
     typename M1::Acc sum;
 #pragma unroll
     for (int i = 0; i < FN; ++i) {
-      sum[i][0] = part[((wn * FM + j) * FN + i) * 64 + lane];
+      sum[i][0] = part[(j * FN + i) * 64 + lane];
 #pragma unroll
       for (int k = 1; k < WK; ++k) {
-        const mm4_t v = part[(((k * WN + wn) * FM + j) * FN + i) * 64 + lane];
+        const mm4_t v = part[((k * FM + j) * FN + i) * 64 + lane];
 #pragma unroll
         for (int u = 0; u < 4; ++u) sum[i][0][u] += v[u];
       }
     }
     MmTile tj = t;
     tj.m0 += 16 * j;
-    if (tj.m0 < tj.m_end) M1::store_any(a, tj, sum, wave, 0, wn, lane, lds + WK * WN * FM * FN * 1024);
+    if (tj.m0 < tj.m_end) M1::store_any(a, tj, sum, wave, 0, 0, lane, lds + WK * FM * FN * 1024);
   }
 }
 
@@ -857,13 +857,12 @@ void launch_mm(MmArgs a, int tiles_m, hipStream_t stream) {
                      dim3(64 * WM * WN), 0, stream, a);
 }
 
-template <int XT, int FM, int WK, int MODE, bool EXPERTS>
+template <int XT, int FM, int MODE, bool EXPERTS>
 void launch_few(MmArgs a, int tiles_m, hipStream_t stream) {
-  constexpr int OC = 16 * (8 / WK);
   a.tiles_m = tiles_m;
-  a.tiles_n = (a.N + OC - 1) / OC;
+  a.tiles_n = (a.N + 15) / 16;
   const int64_t total = (int64_t)tiles_m * a.tiles_n;
-  hipLaunchKernelGGL((few_mm<XT, FM, WK, MODE, EXPERTS>), dim3((unsigned)((total + 7) / 8 * 8)), dim3(512), 0, stream, a);
+  hipLaunchKernelGGL((few_mm<XT, FM, MODE, EXPERTS>), dim3((unsigned)((total + 7) / 8 * 8)), dim3(512), 0, stream, a);
 }
 
 }  // namespace

@@ -8,7 +8,7 @@ namespace gr {
 namespace {
 
 // ---- routing -----------------------------------------------------------------
-constexpr int RT_WAVES = 4;  // one token each
+constexpr int RT_WAVES = 4;
 constexpr int MAX_EXPERTS = 1024;
 
 struct RouteArgs {
@@ -567,8 +567,8 @@ void launch_experts(const MmArgs& up, const MmArgs& down, int tiles, int bm, hip
     }
   } else {
     if (bm == 16) {
-      launch_few<XT, 1, 8, MM_SWIGLU, true>(up, tiles, stream);
-      launch_few<XT, 1, 8, MM_PLAIN, true>(down, tiles, stream);
+      launch_few<XT, 1, MM_SWIGLU, true>(up, tiles, stream);
+      launch_few<XT, 1, MM_PLAIN, true>(down, tiles, stream);
     } else if (bm == 64) {
       launch_mm<XT, 64, 64, 2, 2, 4, MM_SWIGLU, true, false>(up, tiles, stream);
       launch_mm<XT, 64, 64, 2, 2, 4, MM_PLAIN, true, false>(down, tiles, stream);

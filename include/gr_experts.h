@@ -52,7 +52,11 @@ gr_status_t gr_quant_fp8(void* out, int64_t out_stride, float* scale, int64_t sc
  * Sums are float32 throughout for a float32 or e4m3 result.  For a 16-bit one the
  * matrix core adds the e4m3 products, in groups of 8 whose members are cut off
  * below 2^-13 of the largest (about 1.5e-5 of an ordinary result); the groups'
- * sums are float32.
+ * sums are float32.  The sizes of a call choose its kernel, and with it the order
+ * of the sums and, for small results, float32 sums of 16-bit ones too: a row's last
+ * bits may differ between calls of other sizes (not between calls of the same).
+ * x_scale * w_scale is formed first, in float32: a block where that overflows is
+ * infinite or NaN, one where it is below 2^-126 keeps as many bits as that has.
  * in_features % 16 == 0; x and w rows 16-byte aligned, at most 4 MB apart; no more
  * than 2^35 results, less for sizes that leave 64 x 64 tiles part empty.
  */
@@ -99,7 +103,8 @@ gr_status_t gr_route_experts(float* weights, int32_t* ids, const void* logits, i
  * gr_linear_fp8's 16-bit results), and with e4m3 weights or a bf16 out each expert's
  * result is rounded to fp16 times a power of two (2^-11 of a value, 2^-39 of the
  * largest of its 16 to 64 neighbouring columns) before the sum over j, which is
- * float32 and in the order of j.
+ * float32 and in the order of j.  As for gr_linear_fp8, a token's last bits may
+ * differ between calls of other sizes.
  * hidden % 16 == 0, ffn % 16 == 0; rows of x, and weights, 16-byte aligned; out
  * rows 8-byte aligned.  num_experts <= 1024, num_tokens < 2^23, x spans less than
  * 2 GB.  workspace: gr_expert_mlp_workspace_size bytes, 256-byte aligned, no initial

@@ -1,0 +1,183 @@
+// The chosen experts' SwiGLU layers with 4-bit microscaled weights (gr_mx_mm.h): the
+// tokens are quantised once, each expert's gated product is written in 4 bits, and its
+// result waits for the sum over a token's experts as scaled fp16.
+#include <algorithm>
+
+#include "gr_expert_rows.h"
+#include "gr_mx_mm.h"
+
+#include "gr_mxfp4.h"
+
+namespace gr {
+namespace {
+
+// The tokens are quantised by the workgroups behind those that sort (or count, where
+// several do).
+template <int DT, int ROWS> __global__ __launch_bounds__(PLAN_THREADS) void mx_expert_start_k(PlanArgs a, MxQuantArgs q) {
+  __shared__ int next[MAX_EXPERTS], part[PLAN_THREADS / 64];
+  if ((int)blockIdx.x >= a.blocks)
+    mx_quant_item<DT, ROWS>(q, (blockIdx.x - a.blocks) * PLAN_THREADS + threadIdx.x);
+  else if (a.blocks > 1)
+    expert_count(a, next);
+  else
+    expert_plan(a, next, part);
+}
+
+struct MxWorkspace {
+  int64_t hist, slot, tiles, num_tiles, x4, xs, act, act_scale, y, y_exp, bytes;
+  int64_t max_tiles;
+  int blocks;
+};
+
+// Rows of a tile, by the rows an expert gets on average.
+int mx_tile_rows(int64_t rows, int E) { return rows <= 8ll * E ? 16 : rows <= 80ll * E ? 32 : 128; }
+// columns of a wave of the down product with tiles of bm rows (launch_mx_experts)
+int mx_wave_cols(int bm) { return bm == 16 ? 16 : 64; }
+
+MxWorkspace plan_mx_workspace(int T, int k, int E, int H, int F, int bm) {
+  MxWorkspace w{};
+  const int64_t rows = (int64_t)T * k;
+  auto take = [&](int64_t bytes) {
+    const int64_t at = w.bytes;
+    w.bytes += (bytes + 255) / 256 * 256;
+    return at;
+  };
+  w.blocks = (int)((rows + PLAN_ROWS - 1) / PLAN_ROWS);
+  w.max_tiles = rows / bm + (rows < E ? rows : E);
+  w.num_tiles = take(4);
+  w.hist = take(4ll * w.blocks * E);
+  w.slot = take(4 * rows);
+  w.tiles = take(16 * w.max_tiles);
+  w.x4 = take((int64_t)T * ((H + 1) / 2));
+  w.xs = take((int64_t)T * ((H + 31) / 32));
+  w.act = take(rows * ((F + 1) / 2));
+  w.act_scale = take(rows * ((F + 31) / 32));
+  w.y = take(2 * rows * H);
+  w.y_exp = take(rows * ((H + 15) / 16));
+  return w;
+}
+
+void launch_mx_experts(const MxArgs& up, const MxArgs& down, int tiles, int bm, hipStream_t stream) {
+  if (bm == 16) {
+    launch_mx_few<1, 2, 4, MM_SWIGLU_Q, true>(up, tiles, stream);
+    launch_mx_few<1, 1, 4, MM_PLAIN, true>(down, tiles, stream);
+  } else if (bm == 32) {
+    launch_mx<32, 256, 1, 4, 2, MM_SWIGLU_Q, true>(up, tiles, stream);
+    launch_mx<32, 256, 1, 4, 2, MM_PLAIN, true>(down, tiles, stream);
+  } else {
+    launch_mx<128, 256, 2, 4, 3, MM_SWIGLU_Q, true>(up, tiles, stream);
+    launch_mx<128, 256, 2, 4, 3, MM_PLAIN, true>(down, tiles, stream);
+  }
+}
+
+bool aligned(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+
+}  // namespace
+}  // namespace gr
+
+using namespace gr;
+
+extern "C" size_t gr_expert_mlp_mxfp4_workspace_size(int num_tokens, int top_k, int num_experts, int hidden, int ffn) {
+  if (num_tokens < 1 || top_k < 1 || num_experts < 1 || hidden < 1 || ffn < 1) return 0;
+  const int bm = mx_tile_rows((int64_t)num_tokens * top_k, num_experts);
+  return (size_t)plan_mx_workspace(num_tokens, top_k, num_experts, hidden, ffn, bm).bytes;
+}
+
+extern "C" gr_status_t gr_expert_mlp_mxfp4(void* out, int64_t out_stride, const void* x, int64_t x_stride,
+                                           const void* gate_up, const uint8_t* gate_up_scale, const void* down,
+                                           const uint8_t* down_scale, const float* weights, const int32_t* ids,
+                                           int num_tokens, int top_k, int num_experts, int hidden, int ffn, int dtype,
+                                           void* workspace, size_t workspace_bytes, int32_t* dev_status,
+                                           hipStream_t stream) {
+  if (num_tokens < 0 || top_k < 1 || num_experts < 1 || hidden < 1 || ffn < 1 || !dtype_valid(dtype))
+    return GR_ERR_INVALID_ARG;
+  if (num_tokens == 0) return GR_OK;
+  if (!out || !x || !gate_up || !gate_up_scale || !down || !down_scale || !weights || !ids || out_stride < hidden ||
+      x_stride < hidden)
+    return GR_ERR_INVALID_ARG;
+  const int T = num_tokens, H = hidden, F = ffn;
+  if (dtype == GR_DTYPE_F32 || hidden % 32 != 0 || ffn % 32 != 0 || hidden > (1 << 21) || ffn > (1 << 21) ||
+      num_experts > MAX_EXPERTS || (int64_t)T * top_k > (1 << 26) || !aligned(x, 16) || x_stride % 8 != 0 ||
+      !aligned(gate_up, 16) || !aligned(down, 16) || !aligned(out, 8) || out_stride % 4 != 0 ||
+      (int64_t)T * H > (1ll << 32) - (1 << 24))
+    return GR_ERR_UNSUPPORTED;
+  const int bm = mx_tile_rows((int64_t)T * top_k, num_experts);
+  const MxWorkspace l = plan_mx_workspace(T, top_k, num_experts, H, F, bm);
+  const int cols = bm == 16 ? 16 : 128;  // results of a workgroup, in the narrower product
+  if (l.max_tiles * ((std::max(F, H) + cols - 1) / cols) > GRID_MAX - 8 || T > GRID_MAX) return GR_ERR_UNSUPPORTED;
+  if (!workspace || !aligned(workspace, 256) || workspace_bytes < (size_t)l.bytes) return GR_ERR_WORKSPACE;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  const int rows = T * top_k;
+
+  const PlanArgs p{ids, rows, num_experts, bm, l.blocks, reinterpret_cast<int32_t*>(ws + l.hist),
+                   reinterpret_cast<int32_t*>(ws + l.slot), reinterpret_cast<int4*>(ws + l.tiles),
+                   reinterpret_cast<int32_t*>(ws + l.num_tiles), dev_status};
+  const MxQuantArgs q{ws + l.x4, H / 2, ws + l.xs, H / 32, x, x_stride, T, H};
+  const int quant = mx_quant_rows(T, H, dtype);
+  const int64_t items = ((int64_t)T + quant - 1) / quant * (H / 16);
+  const dim3 start((unsigned)(l.blocks + (items + PLAN_THREADS - 1) / PLAN_THREADS));
+  auto first = [&](auto one, auto two) {
+    hipLaunchKernelGGL(quant == 2 ? two : one, start, dim3(PLAN_THREADS), 0, stream, p, q);
+  };
+  if (dtype == GR_DTYPE_F16) first(mx_expert_start_k<GR_DTYPE_F16, 1>, mx_expert_start_k<GR_DTYPE_F16, 2>);
+  else first(mx_expert_start_k<GR_DTYPE_BF16, 1>, mx_expert_start_k<GR_DTYPE_BF16, 2>);
+  if (l.blocks > 1) hipLaunchKernelGGL(expert_plan_k, dim3(l.blocks), dim3(PLAN_THREADS), 0, stream, p);
+
+  MxArgs up{};
+  up.x = q.out;
+  up.x_stride = H / 2;
+  up.xs4 = q.scale;
+  up.xs4_row = H / 32;
+  up.w = static_cast<const uint8_t*>(gate_up);
+  up.w_stride = H / 2;
+  up.w_expert = 2ll * F * (H / 2);
+  up.ws4 = gate_up_scale;
+  up.ws4_row = H / 32;
+  up.ws4_expert = 2ll * F * (H / 32);
+  up.out = ws + l.act;
+  up.out_stride = F / 2;
+  up.os4 = ws + l.act_scale;
+  up.os4_row = F / 32;
+  up.M = rows;
+  up.N = F;
+  up.kbytes = H / 2;
+  up.blocks = H / 32;
+  up.loose = up.blocks % 4 != 0 || !aligned(gate_up_scale, 4);
+  up.tiles = p.tiles;
+  up.num_tiles = p.num_tiles;
+  up.slot = p.slot;
+  up.gather = top_k;
+  MxArgs dn{};
+  dn.x = ws + l.act;
+  dn.x_stride = F / 2;
+  dn.xs4 = up.os4;
+  dn.xs4_row = F / 32;
+  dn.w = static_cast<const uint8_t*>(down);
+  dn.w_stride = F / 2;
+  dn.w_expert = (int64_t)H * (F / 2);
+  dn.ws4 = down_scale;
+  dn.ws4_row = F / 32;
+  dn.ws4_expert = (int64_t)H * (F / 32);
+  dn.out = ws + l.y;
+  dn.out_stride = H;
+  dn.M = rows;
+  dn.N = H;
+  dn.kbytes = F / 2;
+  dn.blocks = F / 32;
+  dn.loose = dn.blocks % 4 != 0 || !aligned(down_scale, 4);
+  // (up to 2^-11 of each expert's result: half a step of an fp16 output, little beside the 2^-2 of its 4-bit operands)
+  dn.out_type = MM_OUT_SCALED;
+  dn.out_exp = reinterpret_cast<int8_t*>(ws + l.y_exp);
+  dn.tiles = p.tiles;
+  dn.num_tiles = p.num_tiles;
+  dn.slot = p.slot;
+  dn.scatter = 1;
+  launch_mx_experts(up, dn, (int)l.max_tiles, bm, stream);
+
+  const CombineArgs c{out, out_stride, ws + l.y, dn.out_exp, mx_wave_cols(bm), weights, ids, T, top_k, num_experts, H};
+  const dim3 grid((unsigned)T, (unsigned)((H + 2047) / 2048));
+  auto go = [&](auto k) { hipLaunchKernelGGL(k, grid, dim3(256), 0, stream, c); };
+  if (dtype == GR_DTYPE_BF16) go(expert_combine_k<GR_DTYPE_BF16, true>);
+  else go(expert_combine_k<GR_DTYPE_F16, true>);
+  return launch_status();
+}

@@ -1,0 +1,481 @@
+// Products of 4-bit microscaled (MXFP4) rows, and the pieces that the quantiser,
+// the projections (gr_mxfp4.hip) and the experts' layers (gr_mx_experts.hip) share.
+//
+//   y[t, n] = sum_b 2^(xs[t, b] - 127) 2^(ws[n, b] - 127) sum_{k in block b of 32} x[t, k] w[n, k]
+//
+// The matrix core takes 32 numbers of e2m1 a lane and the block's two scale bytes
+// beside them, and sums 128 products a result: exactly, measured, as long as the four
+// blocks' scales are within 2^6 of each other, and to 2^-24 of the sum of magnitudes
+// beyond.  So float32 results and results that are rounded to 4 bits again need no
+// other path than 16-bit ones.
+//
+// A stage is 128 bytes of each row of both operands, 256 features or 8 blocks, moved
+// and laid out as gr_block_mm.h does (Mm below: tiles, transfers, results); lane
+// (r = l % 16, q = l / 16) of a fragment of 16 rows multiplies blocks 2 q and 2 q + 1
+// of row r, so that a stage's scales are two neighbouring bytes of that row.
+#pragma once
+
+#include "gr_block_mm.h"
+
+namespace gr {
+namespace {
+
+// A byte's scale, as a float: 2^(byte - 127) (the conversions read 0 as 2^-127 and 255 as NaN).
+__device__ inline float mx_unit(uint32_t byte) { return __builtin_bit_cast(float, byte << 23); }
+// The scale byte of a block from the bits of its largest magnitude (a NaN's are the
+// largest): the least 2^e with max < 7 * 2^e, that is, where the largest rounds to 6 at
+// most -- from 1.75 times a power of two on the next one.
+__device__ inline uint32_t mx_scale(uint32_t amax_bits) {
+  if (amax_bits >= 0x7F800000u) return 255u;
+  const uint32_t e = (amax_bits + 0x200000u) >> 23;
+  return e < 2 ? 0u : e - 2;
+}
+// 8 values in 4 bits
+__device__ inline uint32_t mx_codes(const float (&v)[8], float unit) {
+  uint32_t c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, v[0], v[1], unit, 0);
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[2], v[3], unit, 1);
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[4], v[5], unit, 2);
+  return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[6], v[7], unit, 3);
+}
+
+struct MxArgs : MmArgs {  // kbytes: in_features / 2; strides of x and w in bytes; out in 4 bits: out_stride in bytes
+  const uint8_t* xs4;     // scale bytes of a row side by side
+  int64_t xs4_row;
+  const uint8_t* ws4;
+  int64_t ws4_row, ws4_expert;
+  uint8_t* os4;  // *_Q
+  int64_t os4_row;
+  int blocks;  // of a row: in_features / 32
+  int loose;   // scales are not whole, aligned dwords: blocks or a row's stride % 4 != 0
+};
+
+// BM rows by BN weight rows, WM x WN waves (SwiGLU: 16 gate rows and their 16 up rows alternate)
+template <int BM, int BN, int WM, int WN, int MODE, bool EXPERTS>
+struct Mx {
+  static constexpr bool GATED = MODE == MM_SWIGLU || MODE == MM_SWIGLU_Q;
+  static constexpr bool QUANT = MODE == MM_SWIGLU_Q || MODE == MM_PLAIN_Q;
+  using M = Mm<GR_DTYPE_BF16, BM, BN, WM, WN, GATED ? MM_SWIGLU : MM_PLAIN, EXPERTS, false>;  // rows of bytes
+  static constexpr int NW = WM * WN, ROWS = BM + BN, TILE = M::TILE, LPS = M::LPS, FM = M::FM, FN = M::FN, OC = M::OC;
+  static constexpr int SPS = (2 * ROWS + 64 * NW - 1) / (64 * NW);  // transfers of scales a wave and stage, a dword a lane
+  static constexpr int OPS = LPS + SPS, SCALES = NW * SPS * 256;
+  static_assert(ROWS % (8 * NW) == 0 && NW % 2 == 0, "whole transfers; a wave's rows keep their parity of 8");
+  static_assert(!QUANT || OC / WN % 32 == 0, "a block of the result is one wave's");
+  using Acc = typename M::Acc;
+
+  // Chunks of 16 bytes in LDS are XORed with the row's bits 1 to 3: 16 rows of one
+  // logical chunk, which a fragment reads at once, lie on all 64 banks.
+  __device__ static __forceinline__ int swizzle(int row) { return row >> 1 & 7; }
+
+  struct Source {
+    typename M::Source rows;
+    const uint8_t* scale[SPS];
+  };
+  __device__ static __forceinline__ int w_row(const MmTile& t, int b, int N) {  // weight row of tile row BM + b
+    if constexpr (GATED) return min(t.n0 + (b >> 5) * 16 + (b & 15), N - 1) + (b >> 4 & 1) * N;
+    else return min(t.n0 + b, N - 1);
+  }
+  __device__ static __forceinline__ void source(const MxArgs& a, const MmTile& t, int wave, int lane, Source& s) {
+    s.rows.ch = ((lane & 7) ^ swizzle(wave * 8 + (lane >> 3))) * 16;
+    const int first = EXPERTS && a.gather ? 0 : t.m0;
+    const u32x4_t xb = mm_buffer(a.x + (int64_t)first * a.x_stride);
+    const u32x4_t wb = mm_buffer(t.w + (int64_t)t.n0 * a.w_stride);
+    const u32x4_t ub = GATED ? mm_buffer(t.w + (int64_t)(t.n0 + a.N) * a.w_stride) : wb;
+#pragma unroll
+    for (int i = 0; i < LPS; ++i) {
+      const int r8 = 8 * (wave + NW * i), row = r8 + (lane >> 3);
+      if (r8 < BM) {
+        s.rows.buf[i] = xb;
+        s.rows.off[i] = (uint32_t)((M::x_row(a, t, row) - first) * (uint32_t)a.x_stride) + s.rows.ch;
+      } else {
+        const int b = row - BM;
+        const bool up = GATED && ((r8 - BM) >> 4 & 1);
+        s.rows.buf[i] = up ? ub : wb;
+        s.rows.off[i] = (uint32_t)((w_row(t, b, a.N) - (up ? a.N : 0) - t.n0) * (uint32_t)a.w_stride) + s.rows.ch;
+      }
+    }
+    const uint8_t* ws = a.ws4;
+    if constexpr (EXPERTS) ws += __builtin_amdgcn_readfirstlane(a.tiles[t.mt].x) * a.ws4_expert;
+#pragma unroll
+    for (int i = 0; i < SPS; ++i) {  // entry: a row's first or second four blocks of the stage
+      const int r = min(((wave * SPS + i) * 64 + lane) >> 1, ROWS - 1);
+      s.scale[i] = r < BM ? a.xs4 + M::x_row(a, t, r) * a.xs4_row : ws + w_row(t, r - BM, a.N) * a.ws4_row;
+    }
+  }
+
+  // Stage k into the buffers at LDS bytes `rows` and `scales` of lds.  Past a row's
+  // last block its last four scales stand (a NaN there is the row's anyway); the
+  // numbers there are zeros.
+  __device__ static __forceinline__ void fetch(const MxArgs& a, const Source& s, int k, uint8_t* lds, int rows, int scales,
+                                               int wave, int lane) {
+    const uint32_t lds0 = (uint32_t)reinterpret_cast<uintptr_t>(lds);
+    if (a.loose) {  // (its loads are waited for before anything below is sent: the transfers' count stays an upper bound)
+#pragma unroll
+      for (int i = 0; i < SPS; ++i) {
+        uint32_t v = 0;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) v |= (uint32_t)s.scale[i][min(8 * k + 4 * (lane & 1) + b, a.blocks - 1)] << (8 * b);
+        *reinterpret_cast<uint32_t*>(lds + scales + ((wave * SPS + i) * 64 + lane) * 4) = v;
+      }
+    } else {
+      const int at = min(8 * k + 4 * (lane & 1), a.blocks - 4);
+#pragma unroll
+      for (int i = 0; i < SPS; ++i) dma_v1(lds0 + scales + (wave * SPS + i) * 256, s.scale[i] + at);
+    }
+    M::fetch(a, s.rows, k, lds0 + rows, 0, wave);
+  }
+
+  struct Lane {
+    int xo, wo, fch[2], xso, wso;
+  };
+  __device__ static __forceinline__ Lane lane_of(int wm, int wn, int lane) {
+    const int r16 = lane & 15, q = lane >> 4;
+    Lane l;
+    l.fch[0] = (2 * q ^ swizzle(r16)) * 16;
+    l.fch[1] = ((2 * q + 1) ^ swizzle(r16)) * 16;
+    const int xr = wm * (BM / WM) + r16, wr = BM + wn * (BN / WN) + r16;
+    l.xo = xr * 128;
+    l.wo = wr * 128;
+    l.xso = xr * 8 + 2 * q;
+    l.wso = wr * 8 + 2 * q;
+    return l;
+  }
+  struct Frag {  // a lane's two blocks of a fragment of 16 rows
+    mm4i_t v[2];
+    int s;
+  };
+  __device__ static __forceinline__ Frag read(const uint8_t* rows, const uint8_t* scale, const Lane& l) {
+    return {{*reinterpret_cast<const mm4i_t*>(rows + l.fch[0]), *reinterpret_cast<const mm4i_t*>(rows + l.fch[1])},
+            *reinterpret_cast<const uint16_t*>(scale)};
+  }
+};
+
+// 128 features deep; H: which of a fragment's blocks
+template <int H> __device__ __forceinline__ mm4_t mx_mma(mm4i_t w, int ws, mm4i_t x, int xs, mm4_t c) {
+  constexpr int E2M1 = 4;
+  const mm8i_t a = __builtin_shufflevector(w, w, 0, 1, 2, 3, -1, -1, -1, -1);
+  const mm8i_t b = __builtin_shufflevector(x, x, 0, 1, 2, 3, -1, -1, -1, -1);
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, E2M1, E2M1, H, ws, H, xs);
+}
+
+// A 4-bit block of 32 results of row r % 16 of a fragment row: scale byte, and this
+// lane's 4 + 4 codes of output fragments i and i + 1.
+template <typename M> __device__ __forceinline__ uint32_t mx_block(const typename M::Acc& acc, int i, int j, uint32_t& codes) {
+  float lo[4], hi[4];
+  M::value(acc, i, j, lo);
+  M::value(acc, i + 1, j, hi);
+  const float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+  uint32_t m = 0;
+#pragma unroll
+  for (int u = 0; u < 8; ++u) m = max(m, __builtin_bit_cast(uint32_t, v[u]) & 0x7FFFFFFFu);
+  m = max(m, (uint32_t)__shfl_xor((int)m, 16, 64));
+  m = max(m, (uint32_t)__shfl_xor((int)m, 32, 64));
+  const uint32_t s = mx_scale(m);
+  codes = s == 255u ? 0u : mx_codes(v, mx_unit(s));
+  return s;
+}
+
+// ST stages of LDS, one barrier a stage, as block_mm: stage s has landed when all but the
+// ST - 2 younger ones' transfers have; past its barrier nobody reads stage s - 1, whose
+// buffer takes stage s + ST - 1.
+template <int BM, int BN, int WM, int WN, int ST, int MODE, bool EXPERTS>
+__global__ __launch_bounds__(64 * WM * WN, 2) void mx_mm(MxArgs a) {
+  using X = Mx<BM, BN, WM, WN, MODE, EXPERTS>;
+  using M = typename X::M;
+  constexpr int BLOCKS = X::OC / 32, PITCH = X::OC / 2 + 16;  // of a row in 4 bits
+  static_assert(!X::QUANT || BM * (PITCH + BLOCKS) <= ST * X::TILE, "the results' rows fit");
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[ST * (X::TILE + X::SCALES)];
+  MmTile t;
+  if (!M::tile(a, t)) return;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave / WN, wn = wave % WN;
+  typename X::Source src;
+  X::source(a, t, wave, lane, src);
+  const typename X::Lane l = X::lane_of(wm, wn, lane);
+  const int n = __builtin_amdgcn_readfirstlane((a.kbytes + 127) >> 7);
+  auto fetch = [&](int s, int buf) __attribute__((always_inline)) {
+    X::fetch(a, src, s, lds, buf * X::TILE, ST * X::TILE + buf * X::SCALES, wave, lane);
+  };
+  typename X::Acc acc;
+#pragma unroll
+  for (int i = 0; i < X::FN; ++i)
+#pragma unroll
+    for (int j = 0; j < X::FM; ++j) acc[i][j] = mm4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int s = 0; s < ST - 1; ++s)
+    if (s < n) fetch(s, s);
+  int buf = 0;
+  for (int s = 0; s < n; ++s) {
+    if (s + ST - 1 <= n) mm_wait_barrier<(ST - 2) * X::OPS>();
+    else mm_wait_barrier<0>();
+    if (s + ST - 1 < n) fetch(s + ST - 1, buf == 0 ? ST - 1 : buf - 1);
+    const uint8_t *p = lds + buf * X::TILE, *sc = lds + ST * X::TILE + buf * X::SCALES;
+    typename X::Frag w[X::FN];
+#pragma unroll
+    for (int i = 0; i < X::FN; ++i) w[i] = X::read(p + l.wo + i * 2048, sc + l.wso + i * 128, l);
+#pragma unroll
+    for (int j = 0; j < X::FM; ++j) {
+      const typename X::Frag x = X::read(p + l.xo + j * 2048, sc + l.xso + j * 128, l);
+#pragma unroll
+      for (int i = 0; i < X::FN; ++i) acc[i][j] = mx_mma<0>(w[i].v[0], w[i].s, x.v[0], x.s, acc[i][j]);
+#pragma unroll
+      for (int i = 0; i < X::FN; ++i) acc[i][j] = mx_mma<1>(w[i].v[1], w[i].s, x.v[1], x.s, acc[i][j]);
+    }
+    buf = buf + 1 == ST ? 0 : buf + 1;
+  }
+  __syncthreads();
+  if constexpr (X::QUANT) {
+    // through LDS, so that a row's blocks of the tile are written side by side
+    const int r16 = lane & 15, q = lane >> 4, c0 = wn * (X::OC / WN);
+    uint8_t* scale = lds + BM * PITCH;
+#pragma unroll
+    for (int j = 0; j < X::FM; ++j) {
+      const int r = wm * (BM / WM) + j * 16 + r16;
+#pragma unroll
+      for (int g = 0; g < M::FO / 2; ++g) {
+        uint32_t codes;
+        const uint32_t s = mx_block<M>(acc, 2 * g, j, codes);
+        uint16_t* o = reinterpret_cast<uint16_t*>(lds + r * PITCH + (c0 + 32 * g) / 2) + q;
+        o[0] = (uint16_t)codes;
+        o[4] = (uint16_t)(codes >> 16);
+        if (q == 0) scale[r * BLOCKS + c0 / 32 + g] = (uint8_t)s;
+      }
+    }
+    __syncthreads();
+    for (int c = threadIdx.x; c < BM * BLOCKS; c += 64 * X::NW) {
+      const int r = c / BLOCKS, b = c % BLOCKS;
+      if (t.m0 + r >= t.m_end || t.n0 + 32 * b >= a.N) continue;
+      const int64_t row = M::out_row(a, t, r);
+      *reinterpret_cast<u32x4_t*>(static_cast<uint8_t*>(a.out) + row * a.out_stride + t.n0 / 2 + 16 * b) =
+          *reinterpret_cast<const u32x4_t*>(lds + r * PITCH + 16 * b);
+      a.os4[row * a.os4_row + t.n0 / 32 + b] = scale[c];
+    }
+  } else {
+    M::store_any(a, t, acc, wave, wm, wn, lane, lds);
+  }
+}
+
+// Few rows: BM = 16 FM, 16 NF columns.  Bound by the weights' way from memory, or by one
+// round trip: each weight is loaded once, by the wave that multiplies it, into the
+// registers of the operand, and the WK waves split the depth (wave k takes stages k,
+// k + WK, ...).  Their partial sums meet in LDS.  The rows are read by every workgroup,
+// from L2.
+template <int FM, int NF, int WK, int MODE, bool EXPERTS>
+__global__ __launch_bounds__(64 * WK) void mx_few(MxArgs a) {
+  constexpr bool GATED = MODE == MM_SWIGLU || MODE == MM_SWIGLU_Q, QUANT = MODE == MM_SWIGLU_Q || MODE == MM_PLAIN_Q;
+  constexpr int FN = NF * (GATED ? 2 : 1), U = FM * FN <= 2 ? 4 : 2;
+  using M = Mm<GR_DTYPE_BF16, 16 * FM, 16 * FN, 1, 1, GATED ? MM_SWIGLU : MM_PLAIN, EXPERTS, false>;
+  using M1 = Mm<GR_DTYPE_BF16, 16, 16 * FN, 1, 1, GATED ? MM_SWIGLU : MM_PLAIN, EXPERTS, false>;  // one fragment row
+  static_assert(FM <= WK && (!QUANT || NF == 2), "a wave finishes a fragment row; a block of the result is 32 columns");
+  constexpr int PART = WK * FM * FN * 1024, ROOM = 16 * (16 * NF * 4 + 16);
+  __shared__ __attribute__((aligned(16))) uint8_t lds[PART + (QUANT ? 0 : FM * ROOM)];
+  MmTile t;
+  if (!M::tile(a, t)) return;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r16 = lane & 15, q = lane >> 4;
+  const int n = (a.kbytes + 127) >> 7;
+  const uint8_t *w0[FN], *ws[FN], *x0[FM], *xs[FM];
+  const uint8_t* ws4 = a.ws4;
+  if constexpr (EXPERTS) ws4 += __builtin_amdgcn_readfirstlane(a.tiles[t.mt].x) * a.ws4_expert;
+#pragma unroll
+  for (int i = 0; i < FN; ++i) {
+    const int64_t r = min(t.n0 + 16 * (GATED ? i >> 1 : i) + r16, a.N - 1) + (GATED && (i & 1) ? a.N : 0);
+    w0[i] = t.w + r * a.w_stride + q * 32;
+    ws[i] = ws4 + r * a.ws4_row + q * 2;
+  }
+#pragma unroll
+  for (int j = 0; j < FM; ++j) {
+    const int64_t r = M::x_row(a, t, 16 * j + r16);
+    x0[j] = a.x + r * a.x_stride + q * 32;
+    xs[j] = a.xs4 + r * a.xs4_row + q * 2;
+  }
+  struct Piece {
+    mm4i_t v[2];
+    int s;
+  };
+  // (past the last block zeros, whose scale is 2^-127)
+  auto load = [&](const uint8_t* p, const uint8_t* sp, int s) __attribute__((always_inline)) {
+    Piece f{{{0, 0, 0, 0}, {0, 0, 0, 0}}, 0};
+    const int left = a.blocks - 8 * s - 2 * q;
+    if (left > 0) f.v[0] = *reinterpret_cast<const mm4i_t*>(p + (int64_t)s * 128);
+    if (left > 1) f.v[1] = *reinterpret_cast<const mm4i_t*>(p + (int64_t)s * 128 + 16);
+    if (left > 1) {
+      uint16_t two;
+      __builtin_memcpy(&two, sp + (int64_t)s * 8, 2);
+      f.s = two;
+    } else if (left == 1) {
+      f.s = sp[(int64_t)s * 8];
+    }
+    return f;
+  };
+  typename M::Acc acc;
+#pragma unroll
+  for (int i = 0; i < FN; ++i)
+#pragma unroll
+    for (int j = 0; j < FM; ++j) acc[i][j] = mm4_t{0.f, 0.f, 0.f, 0.f};
+  for (int s0 = wave; s0 < n; s0 += WK * U) {
+    Piece w[U][FN], x[U][FM];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+#pragma unroll
+      for (int i = 0; i < FN; ++i) w[u][i] = load(w0[i], ws[i], s0 + u * WK);
+#pragma unroll
+      for (int j = 0; j < FM; ++j) x[u][j] = load(x0[j], xs[j], s0 + u * WK);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (u && s0 + u * WK >= n) break;
+#pragma unroll
+      for (int j = 0; j < FM; ++j)
+#pragma unroll
+        for (int i = 0; i < FN; ++i) {
+          acc[i][j] = mx_mma<0>(w[u][i].v[0], w[u][i].s, x[u][j].v[0], x[u][j].s, acc[i][j]);
+          acc[i][j] = mx_mma<1>(w[u][i].v[1], w[u][i].s, x[u][j].v[1], x[u][j].s, acc[i][j]);
+        }
+    }
+  }
+  mm4_t* part = reinterpret_cast<mm4_t*>(lds);  // [wave][FM][FN][64]
+#pragma unroll
+  for (int j = 0; j < FM; ++j)
+#pragma unroll
+    for (int i = 0; i < FN; ++i) part[((wave * FM + j) * FN + i) * 64 + lane] = acc[i][j];
+  __syncthreads();
+  if (const int j = wave; j < FM) {
+    typename M1::Acc sum;
+#pragma unroll
+    for (int i = 0; i < FN; ++i) {
+      sum[i][0] = part[(j * FN + i) * 64 + lane];
+#pragma unroll
+      for (int k = 1; k < WK; ++k) {
+        const mm4_t v = part[((k * FM + j) * FN + i) * 64 + lane];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) sum[i][0][u] += v[u];
+      }
+    }
+    MmTile tj = t;
+    tj.m0 += 16 * j;
+    if (tj.m0 >= tj.m_end) return;
+    if constexpr (QUANT) {
+      uint32_t codes;
+      const uint32_t s = mx_block<M1>(sum, 0, 0, codes);
+      if (tj.m0 + r16 < tj.m_end) {
+        const int64_t row = M1::out_row(a, tj, r16);
+        uint16_t* o = reinterpret_cast<uint16_t*>(static_cast<uint8_t*>(a.out) + row * a.out_stride + t.n0 / 2) + q;
+        o[0] = (uint16_t)codes;
+        o[4] = (uint16_t)(codes >> 16);
+        if (q == 0) a.os4[row * a.os4_row + t.n0 / 32] = (uint8_t)s;
+      }
+    } else {
+      M1::store_any(a, tj, sum, wave, 0, 0, lane, lds + PART);
+    }
+  }
+}
+
+template <int BM, int BN, int WM, int WN, int ST, int MODE, bool EXPERTS>
+void launch_mx(MxArgs a, int tiles_m, hipStream_t stream) {
+  using X = Mx<BM, BN, WM, WN, MODE, EXPERTS>;
+  a.tiles_m = tiles_m;
+  a.tiles_n = (a.N + X::OC - 1) / X::OC;
+  const int64_t total = (int64_t)tiles_m * a.tiles_n;
+  hipLaunchKernelGGL((mx_mm<BM, BN, WM, WN, ST, MODE, EXPERTS>), dim3((unsigned)((total + 7) / 8 * 8)), dim3(64 * WM * WN),
+                     0, stream, a);
+}
+template <int FM, int NF, int WK, int MODE, bool EXPERTS>
+void launch_mx_few(MxArgs a, int tiles_m, hipStream_t stream) {
+  a.tiles_m = tiles_m;
+  a.tiles_n = (a.N + 16 * NF - 1) / (16 * NF);
+  const int64_t total = (int64_t)tiles_m * a.tiles_n;
+  hipLaunchKernelGGL((mx_few<FM, NF, WK, MODE, EXPERTS>), dim3((unsigned)((total + 7) / 8 * 8)), dim3(64 * WK), 0, stream, a);
+}
+
+// ---- rows to 4 bits ------------------------------------------------------------
+struct MxQuantArgs {
+  uint8_t* out;
+  int64_t out_stride;  // bytes
+  uint8_t* scale;
+  int64_t scale_row;
+  const void* x;
+  int64_t x_stride;  // elements
+  int T, K;
+};
+// N features a lane, 32 / N neighbouring lanes a block: 32 bytes of a row in one piece,
+// whatever their type.
+template <int DT> constexpr int mx_quant_features() { return DT == GR_DTYPE_F32 ? 8 : 16; }
+// Lane `item` of ROWS rows below each other: bound by memory, and each row's loads are on
+// their way together.
+template <int DT, int ROWS> __device__ __forceinline__ void mx_quant_item(const MxQuantArgs& a, uint32_t item) {
+  constexpr int N = mx_quant_features<DT>();
+  struct alignas(16) Vec { uint32_t w[8]; };
+  typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+  typedef __bf16 bf2_t __attribute__((ext_vector_type(2)));
+  typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
+  const uint32_t per = (uint32_t)a.K / N, band = item / per;
+  const int k = (int)(item - band * per) * N;
+  const int64_t t0 = (int64_t)band * ROWS;
+  if (t0 >= a.T) return;  // (a block's lanes leave together)
+  Vec in[ROWS];
+#pragma unroll
+  for (int j = 0; j < ROWS; ++j) {  // (past the last row: it again)
+    const int64_t at = min(t0 + j, (int64_t)a.T - 1) * a.x_stride + k;
+    in[j] = DT == GR_DTYPE_F32 ? *reinterpret_cast<const Vec*>(static_cast<const float*>(a.x) + at)
+                               : *reinterpret_cast<const Vec*>(static_cast<const uint16_t*>(a.x) + at);
+  }
+#pragma unroll
+  for (int j = 0; j < ROWS; ++j) {
+    uint32_t m = 0;
+    if constexpr (DT == GR_DTYPE_F32) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) m = max(m, in[j].w[i] & 0x7FFFFFFFu);
+    } else {  // magnitudes of 16-bit values order as their bits do, two at a time
+      u16x2 most = {0, 0};
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, in[j].w[i] & 0x7FFF7FFFu));
+      m = max(most[0], most[1]);
+    }
+    // over the block's lanes, by DPP moves: the xor of 1 (and 2)
+    m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0xB1, 0xf, 0xf, true));
+    if constexpr (N == 8) m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x4E, 0xf, 0xf, true));
+    if constexpr (DT != GR_DTYPE_F32) m = __builtin_bit_cast(uint32_t, Elem<DT>::to_float((uint16_t)m));
+    const uint32_t s = mx_scale(m);
+    const float unit = mx_unit(s);
+    uint32_t c[N / 8];
+    if constexpr (DT == GR_DTYPE_F32) {
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = __builtin_bit_cast(float, in[j].w[i]);
+      c[0] = mx_codes(v, unit);
+    } else {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t* w = in[j].w + 4 * h;
+        if constexpr (DT == GR_DTYPE_BF16) {
+          c[h] = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(0u, __builtin_bit_cast(bf2_t, w[0]), unit, 0);
+          c[h] = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c[h], __builtin_bit_cast(bf2_t, w[1]), unit, 1);
+          c[h] = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c[h], __builtin_bit_cast(bf2_t, w[2]), unit, 2);
+          c[h] = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c[h], __builtin_bit_cast(bf2_t, w[3]), unit, 3);
+        } else {
+          c[h] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(0u, __builtin_bit_cast(h2_t, w[0]), unit, 0);
+          c[h] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(c[h], __builtin_bit_cast(h2_t, w[1]), unit, 1);
+          c[h] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(c[h], __builtin_bit_cast(h2_t, w[2]), unit, 2);
+          c[h] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(c[h], __builtin_bit_cast(h2_t, w[3]), unit, 3);
+        }
+      }
+    }
+    if (s == 255u)
+#pragma unroll
+      for (int h = 0; h < N / 8; ++h) c[h] = 0;
+    const int64_t t = t0 + j;
+    if (j > 0 && t >= a.T) break;
+    uint8_t* o = a.out + t * a.out_stride + k / 2;
+    if constexpr (N == 16) *reinterpret_cast<u32x2_t*>(o) = u32x2_t{c[0], c[N / 8 - 1]};
+    else *reinterpret_cast<uint32_t*>(o) = c[0];
+    if (k % 32 == 0) a.scale[t * a.scale_row + k / 32] = (uint8_t)s;
+  }
+}
+// rows below each other once that still leaves eight waves to each of the 1024 SIMDs
+inline int mx_quant_rows(int64_t T, int K, int dtype) {
+  return T * (K / (dtype == GR_DTYPE_F32 ? 8 : 16)) >= 2ll * 64 * 8 * 1024 ? 2 : 1;
+}
+
+}  // namespace
+}  // namespace gr

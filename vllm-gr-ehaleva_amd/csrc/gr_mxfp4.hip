@@ -1,0 +1,181 @@
+// 4-bit microscaled (MXFP4) tensors: rows to 4 bits and back, and the product of such
+// rows with such weights (gr_mx_mm.h).
+#include "gr_mx_mm.h"
+
+#include "gr_mxfp4.h"
+
+namespace gr {
+namespace {
+
+constexpr int MXQ_THREADS = 256;
+
+template <int DT, int ROWS> __global__ __launch_bounds__(MXQ_THREADS) void mx_quant_k(MxQuantArgs a) {
+  // (items: below 2^31 by the entry's check)
+  mx_quant_item<DT, ROWS>(a, blockIdx.x * MXQ_THREADS + threadIdx.x);
+}
+
+// ---- 4 bits to values ------------------------------------------------------------
+struct MxDequantArgs {
+  void* out;
+  int64_t out_stride;  // elements
+  const uint8_t* x;
+  int64_t x_stride;  // bytes
+  const uint8_t* scale;
+  int64_t scale_row;
+  int T, K;
+};
+// 8 features a lane (16 or 32 bytes of results) of ROWS rows below each other.  Bound by
+// memory, by its stores above all.
+template <int DT, int ROWS> __global__ __launch_bounds__(MXQ_THREADS) void mx_dequant_k(MxDequantArgs a) {
+  const uint32_t item = blockIdx.x * MXQ_THREADS + threadIdx.x, per = (uint32_t)a.K / 8, band = item / per;
+  const int k = (int)(item - band * per) * 8;
+  const int64_t t0 = (int64_t)band * ROWS;
+  if (t0 >= a.T) return;
+  uint32_t c[ROWS], s[ROWS];
+#pragma unroll
+  for (int j = 0; j < ROWS; ++j) {  // (past the last row: it again)
+    const int64_t t = min(t0 + j, (int64_t)a.T - 1);
+    c[j] = *reinterpret_cast<const uint32_t*>(a.x + t * a.x_stride + k / 2);
+    s[j] = a.scale[t * a.scale_row + k / 32];
+  }
+#pragma unroll
+  for (int j = 0; j < ROWS; ++j) {
+    if (j > 0 && t0 + j >= a.T) break;
+    const float unit = mx_unit(s[j]);
+    const int64_t at = (t0 + j) * a.out_stride + k;
+    if constexpr (DT == GR_DTYPE_F32) {
+      typedef float f32x2 __attribute__((ext_vector_type(2)));
+      const f32x2 v0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c[j], unit, 0), v1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c[j], unit, 1),
+                  v2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c[j], unit, 2), v3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c[j], unit, 3);
+      mm4_t* o = reinterpret_cast<mm4_t*>(static_cast<float*>(a.out) + at);
+      o[0] = mm4_t{v0[0], v0[1], v1[0], v1[1]};
+      o[1] = mm4_t{v2[0], v2[1], v3[0], v3[1]};
+    } else {
+      u32x4_t v;
+      if constexpr (DT == GR_DTYPE_BF16)
+        v = u32x4_t{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c[j], unit, 0)),
+                    __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c[j], unit, 1)),
+                    __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c[j], unit, 2)),
+                    __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c[j], unit, 3))};
+      else
+        v = u32x4_t{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c[j], unit, 0)),
+                    __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c[j], unit, 1)),
+                    __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c[j], unit, 2)),
+                    __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c[j], unit, 3))};
+      *reinterpret_cast<u32x4_t*>(static_cast<uint16_t*>(a.out) + at) = v;
+    }
+  }
+}
+
+// ---- products ----------------------------------------------------------------------
+template <int MODE> void launch_linear_mx(const MxArgs& a, hipStream_t stream) {
+  constexpr bool GATED = MODE == MM_SWIGLU || MODE == MM_SWIGLU_Q, QUANT = MODE == MM_SWIGLU_Q || MODE == MM_PLAIN_Q;
+  constexpr int NF = QUANT ? 2 : 1;
+  const int M = a.M, rows_w = GATED ? 2 * a.N : a.N;
+  const int64_t cols = (a.N + 16 * NF - 1) / (16 * NF), few = (M + 15) / 16 * cols, few2 = (M + 31) / 32 * cols;
+  if (few <= 256 || (M <= 16 && few <= 512)) return launch_mx_few<1, NF, 8, MODE, false>(a, (M + 15) / 16, stream);
+  if (few2 <= 512) return launch_mx_few<2, NF, 8, MODE, false>(a, (M + 31) / 32, stream);
+  const auto tiles = [&](int bm, int bn) { return (int64_t)((M + bm - 1) / bm) * ((rows_w + bn - 1) / bn); };
+  if (tiles(256, 256) >= 256) return launch_mx<256, 256, 2, 4, 2, MODE, false>(a, (M + 255) / 256, stream);
+  if (tiles(128, 256) >= 192) return launch_mx<128, 256, 2, 4, 3, MODE, false>(a, (M + 127) / 128, stream);
+  if (tiles(128, 128) >= 192) return launch_mx<128, 128, 2, 2, 2, MODE, false>(a, (M + 127) / 128, stream);
+  launch_mx<64, 128, 2, 2, 3, MODE, false>(a, (M + 63) / 64, stream);
+}
+
+bool aligned(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+
+}  // namespace
+}  // namespace gr
+
+using namespace gr;
+
+extern "C" gr_status_t gr_quant_mxfp4(void* out, int64_t out_stride, uint8_t* scale, int64_t scale_stride, const void* x,
+                                      int64_t x_stride, int num_tokens, int features, int dtype, hipStream_t stream) {
+  if (num_tokens < 0 || features < 1 || !dtype_valid(dtype)) return GR_ERR_INVALID_ARG;
+  if (num_tokens == 0) return GR_OK;
+  if (!out || !scale || !x || out_stride < (features + 1) / 2 || x_stride < features || scale_stride < (features + 31) / 32)
+    return GR_ERR_INVALID_ARG;
+  if (features % 32 != 0 || !aligned(x, 16) || x_stride * dtype_size(dtype) % 16 != 0 || !aligned(out, 16) ||
+      out_stride % 16 != 0 || (int64_t)num_tokens * (features / 32) > (1 << 29) - (1 << 20))
+    return GR_ERR_UNSUPPORTED;
+  const MxQuantArgs a{static_cast<uint8_t*>(out), out_stride, scale, scale_stride, x, x_stride, num_tokens, features};
+  const int rows = mx_quant_rows(num_tokens, features, dtype);
+  const int64_t items = ((int64_t)num_tokens + rows - 1) / rows * (features / (dtype == GR_DTYPE_F32 ? 8 : 16));
+  const dim3 grid((unsigned)((items + MXQ_THREADS - 1) / MXQ_THREADS)), block(MXQ_THREADS);
+  auto go = [&](auto one, auto two) { hipLaunchKernelGGL(rows == 2 ? two : one, grid, block, 0, stream, a); };
+  if (dtype == GR_DTYPE_F32) go(mx_quant_k<GR_DTYPE_F32, 1>, mx_quant_k<GR_DTYPE_F32, 2>);
+  else if (dtype == GR_DTYPE_F16) go(mx_quant_k<GR_DTYPE_F16, 1>, mx_quant_k<GR_DTYPE_F16, 2>);
+  else go(mx_quant_k<GR_DTYPE_BF16, 1>, mx_quant_k<GR_DTYPE_BF16, 2>);
+  return launch_status();
+}
+
+extern "C" gr_status_t gr_dequant_mxfp4(void* out, int64_t out_stride, const void* x, int64_t x_stride,
+                                        const uint8_t* scale, int64_t scale_stride, int num_tokens, int features,
+                                        int dtype, hipStream_t stream) {
+  if (num_tokens < 0 || features < 1 || !dtype_valid(dtype)) return GR_ERR_INVALID_ARG;
+  if (num_tokens == 0) return GR_OK;
+  if (!out || !scale || !x || out_stride < features || x_stride < (features + 1) / 2 || scale_stride < (features + 31) / 32)
+    return GR_ERR_INVALID_ARG;
+  if (features % 32 != 0 || !aligned(x, 4) || x_stride % 4 != 0 || !aligned(out, 16) ||
+      out_stride * dtype_size(dtype) % 16 != 0 || (int64_t)num_tokens * (features / 32) > (1 << 29) - (1 << 20))
+    return GR_ERR_UNSUPPORTED;
+  const MxDequantArgs a{out, out_stride, static_cast<const uint8_t*>(x), x_stride, scale, scale_stride, num_tokens, features};
+  const int rows = (int64_t)num_tokens * (features / 8) >= 4ll * 64 * 8 * 1024 ? 4 : 1;
+  const int64_t items = ((int64_t)num_tokens + rows - 1) / rows * (features / 8);
+  const dim3 grid((unsigned)((items + MXQ_THREADS - 1) / MXQ_THREADS)), block(MXQ_THREADS);
+  auto go = [&](auto one, auto four) { hipLaunchKernelGGL(rows == 4 ? four : one, grid, block, 0, stream, a); };
+  if (dtype == GR_DTYPE_F32) go(mx_dequant_k<GR_DTYPE_F32, 1>, mx_dequant_k<GR_DTYPE_F32, 4>);
+  else if (dtype == GR_DTYPE_F16) go(mx_dequant_k<GR_DTYPE_F16, 1>, mx_dequant_k<GR_DTYPE_F16, 4>);
+  else go(mx_dequant_k<GR_DTYPE_BF16, 1>, mx_dequant_k<GR_DTYPE_BF16, 4>);
+  return launch_status();
+}
+
+extern "C" gr_status_t gr_linear_mxfp4(void* out, int64_t out_stride, uint8_t* out_scale, int64_t out_scale_stride,
+                                       const void* x, int64_t x_stride, const uint8_t* x_scale, int64_t x_scale_stride,
+                                       const void* w, int64_t w_stride, const uint8_t* w_scale, int64_t w_scale_stride,
+                                       int num_tokens, int out_features, int in_features, int swiglu, int out_dtype,
+                                       hipStream_t stream) {
+  const bool quant = out_dtype == GR_DTYPE_MXFP4;
+  if (num_tokens < 0 || out_features < 1 || in_features < 1 || (swiglu != 0 && swiglu != 1) ||
+      (!dtype_valid(out_dtype) && !quant))
+    return GR_ERR_INVALID_ARG;
+  if (num_tokens == 0) return GR_OK;
+  const int64_t row = ((int64_t)in_features + 1) / 2, row_scales = ((int64_t)in_features + 31) / 32;
+  if (!out || !x || !x_scale || !w || !w_scale || x_stride < row || w_stride < row || x_scale_stride < row_scales ||
+      w_scale_stride < row_scales || out_stride < (quant ? ((int64_t)out_features + 1) / 2 : out_features) ||
+      (quant && (!out_scale || out_scale_stride < ((int64_t)out_features + 31) / 32)))
+    return GR_ERR_INVALID_ARG;
+  if (in_features % 32 != 0 || (swiglu && out_features % 16 != 0) || (quant && out_features % 32 != 0) ||
+      out_features > (1 << 28) || num_tokens > (1 << 28) || x_stride > (1 << 22) || w_stride > (1 << 22) ||
+      !aligned(x, 16) || x_stride % 16 != 0 || !aligned(w, 16) || w_stride % 16 != 0 ||
+      !aligned(out, out_dtype == GR_DTYPE_F32 || quant ? 16 : 8) || (quant && out_stride % 16 != 0) ||
+      ((int64_t)num_tokens + 63) / 64 * ((out_features + 63) / 64) > (1 << 23) - 8)
+    return GR_ERR_UNSUPPORTED;
+  MxArgs a{};
+  a.x = static_cast<const uint8_t*>(x);
+  a.x_stride = x_stride;
+  a.xs4 = x_scale;
+  a.xs4_row = x_scale_stride;
+  a.w = static_cast<const uint8_t*>(w);
+  a.w_stride = w_stride;
+  a.ws4 = w_scale;
+  a.ws4_row = w_scale_stride;
+  a.out = out;
+  a.out_stride = out_stride;
+  a.os4 = out_scale;
+  a.os4_row = out_scale_stride;
+  a.M = num_tokens;
+  a.N = out_features;
+  a.kbytes = in_features / 2;
+  a.blocks = in_features / 32;
+  a.loose = a.blocks % 4 != 0 || !aligned(x_scale, 4) || x_scale_stride % 4 != 0 || !aligned(w_scale, 4) || w_scale_stride % 4 != 0;
+  a.out_type = out_dtype;
+  if (quant) {
+    if (swiglu) launch_linear_mx<MM_SWIGLU_Q>(a, stream);
+    else launch_linear_mx<MM_PLAIN_Q>(a, stream);
+  } else {
+    if (swiglu) launch_linear_mx<MM_SWIGLU>(a, stream);
+    else launch_linear_mx<MM_PLAIN>(a, stream);
+  }
+  return launch_status();
+}

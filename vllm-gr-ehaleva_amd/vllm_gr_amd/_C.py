@@ -1,5 +1,5 @@
 """ctypes binding of libgr_beam.so (declared in include/gr_beam.h,
-include/gr_decoder.h and include/gr_experts.h).
+include/gr_decoder.h, include/gr_experts.h and include/gr_mxfp4.h).
 
 The library is the product: there is no Python or CPU fallback.  Loading
 fails loudly with an ImportError-like RuntimeError when the shared object is
@@ -33,6 +33,7 @@ GR_DTYPE_F32 = 0
 GR_DTYPE_F16 = 1
 GR_DTYPE_BF16 = 2
 GR_DTYPE_FP8_E4M3 = 3  # KV caches and block-scaled operands
+GR_DTYPE_MXFP4 = 4  # results in 4 bits with a scale for each 32
 
 _P = ctypes.c_void_p
 _I = ctypes.c_int
@@ -117,6 +118,20 @@ SIGNATURES = {
     ]),
     "gr_expert_mlp_workspace_size": (_SZ, [_I, _I, _I, _I, _I, _I]),
     "gr_expert_mlp": (_I, [
+        _P, _L, _P, _L, _P, _P, _P, _P, # out, out_stride, x, x_stride, gate_up, its scale, down, its scale
+        _P, _P,                         # weights, ids
+        _I, _I, _I, _I, _I, _I,         # tokens, top_k, experts, hidden, ffn, dtype
+        _P, _SZ, _P, _P,                # workspace, bytes, dev_status, stream
+    ]),
+    "gr_quant_mxfp4": (_I, [_P, _L, _P, _L, _P, _L, _I, _I, _I, _P]),
+    "gr_dequant_mxfp4": (_I, [_P, _L, _P, _L, _P, _L, _I, _I, _I, _P]),
+    "gr_linear_mxfp4": (_I, [
+        _P, _L, _P, _L,                 # out, out_stride, out_scale, its stride
+        _P, _L, _P, _L, _P, _L, _P, _L, # x, x_scale, w, w_scale, each with its stride
+        _I, _I, _I, _I, _I, _P,         # tokens, out_features, in_features, swiglu, out_dtype, stream
+    ]),
+    "gr_expert_mlp_mxfp4_workspace_size": (_SZ, [_I, _I, _I, _I, _I]),
+    "gr_expert_mlp_mxfp4": (_I, [
         _P, _L, _P, _L, _P, _P, _P, _P, # out, out_stride, x, x_stride, gate_up, its scale, down, its scale
         _P, _P,                         # weights, ids
         _I, _I, _I, _I, _I, _I,         # tokens, top_k, experts, hidden, ffn, dtype

@@ -1,5 +1,5 @@
 """torch-tensor entry points over the C ABI (include/gr_beam.h,
-include/gr_decoder.h, include/gr_experts.h).
+include/gr_decoder.h, include/gr_experts.h, include/gr_mxfp4.h).
 
 Each function validates shapes/devices on the host, allocates outputs with
 the torch caching allocator when the caller passes none, and launches on
@@ -945,3 +945,163 @@ def expert_mlp(x: torch.Tensor, gate_up: torch.Tensor, down: torch.Tensor, weigh
 def expert_mlp_workspace_bytes(num_tokens: int, top_k: int, num_experts: int, hidden: int, ffn: int, fp8: bool) -> int:
     """Workspace of ``expert_mlp``."""
     return int(_C.lib().gr_expert_mlp_workspace_size(num_tokens, top_k, num_experts, hidden, ffn, int(fp8)))
+
+
+# ---- 4-bit microscaled tensors (include/gr_mxfp4.h) --------------------------
+
+#: features of a row that share a scale byte
+MXFP4_BLOCK = 32
+_MX_CODES = (torch.uint8, torch.float4_e2m1fn_x2)
+_MX_SCALES = (torch.uint8, torch.float8_e8m0fnu)
+
+
+def _mx_rows(name: str, t: torch.Tensor, scale: torch.Tensor) -> int:
+    """Features of the rows of a 4-bit matrix."""
+    _rows(name, t)
+    K = 2 * t.shape[1]
+    if t.dtype not in _MX_CODES or K % MXFP4_BLOCK or K > _INT_MAX:
+        raise ValueError(f"{name} must hold two codes a byte (uint8 or float4_e2m1fn_x2), 16 bytes a block of 32")
+    _mx_scales(f"{name}_scale" if name != "out" else "out_scale", scale, t.shape[0], K)
+    return K
+
+
+def _mx_scales(name: str, t: torch.Tensor, rows: int, features: int) -> None:
+    if (t.dtype not in _MX_SCALES or t.shape != (rows, features // MXFP4_BLOCK)
+            or (t.shape[1] > 1 and t.stride(1) != 1)):
+        raise ValueError(f"{name} must be a uint8 or float8_e8m0fnu [rows, features / 32] tensor, a row's bytes side by side")
+
+
+def _mx_new(rows: int, features: int, dev):
+    return (torch.empty((rows, features // 2), dtype=torch.uint8, device=dev),
+            torch.empty((rows, features // MXFP4_BLOCK), dtype=torch.uint8, device=dev))
+
+
+def quant_mxfp4(x: torch.Tensor, *, out: torch.Tensor | None = None, scale: torch.Tensor | None = None):
+    """Rows ``x [T, K]`` (float32, fp16 or bf16) in 4 bits: ``(out [T, K / 2] uint8,
+    scale [T, K / 32] uint8)``, two e2m1 codes a byte and a power of two for each 32
+    features; see ``gr_quant_mxfp4`` in gr_mxfp4.h.  ``K`` is a multiple of 32 and
+    rows of ``x`` and ``out`` are 16-byte aligned."""
+    dev = _need_cuda(x, out, scale)
+    _rows("x", x)
+    T, K = x.shape
+    if K % MXFP4_BLOCK:
+        raise ValueError("x must have a multiple of 32 features")
+    new = _mx_new(T, K, dev) if out is None or scale is None else (None, None)
+    out = new[0] if out is None else out
+    scale = new[1] if scale is None else scale
+    if _mx_rows("out", out, scale) != K or out.shape[0] != T:
+        raise ValueError("out must be a [tokens, features / 2] tensor")
+    _launch(dev, "gr_quant_mxfp4", out.data_ptr(), _row_stride(out, T, K // 2), scale.data_ptr(),
+            _row_stride(scale, T, K // MXFP4_BLOCK), x.data_ptr(), _row_stride(x, T, K), T, K, _dtype_code(x), _stream(dev))
+    return out, scale
+
+
+def dequant_mxfp4(x: torch.Tensor, scale: torch.Tensor, *, dtype: torch.dtype = torch.bfloat16,
+                  out: torch.Tensor | None = None) -> torch.Tensor:
+    """The values ``[T, K]`` of 4-bit rows ``x [T, K / 2]`` with ``scale [T, K / 32]``, in
+    ``dtype`` (float32, fp16, bf16); see ``gr_dequant_mxfp4`` in gr_mxfp4.h."""
+    dev = _need_cuda(x, scale, out)
+    K = _mx_rows("x", x, scale)
+    T = x.shape[0]
+    if out is None:
+        out = torch.empty((T, K), dtype=dtype, device=dev)
+    else:
+        _rows("out", out)
+        if out.shape != (T, K) or out.dtype != dtype:
+            raise ValueError("out must be a [tokens, features] tensor of dtype")
+    _launch(dev, "gr_dequant_mxfp4", out.data_ptr(), _row_stride(out, T, K), x.data_ptr(), _row_stride(x, T, K // 2),
+            scale.data_ptr(), _row_stride(scale, T, K // MXFP4_BLOCK), T, K, _dtype_code(out), _stream(dev))
+    return out
+
+
+def linear_mxfp4(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, *,
+                 swiglu: bool = False, quantized: bool = False, out_dtype: torch.dtype = torch.bfloat16,
+                 out: torch.Tensor | None = None, out_scale: torch.Tensor | None = None):
+    """``x [T, K] @ w[N, K].T`` of 4-bit operands with float32 sums: ``x [T, K / 2]``,
+    ``w [N, K / 2]`` and their scales ``[.., K / 32]`` as ``quant_mxfp4`` gives them; see
+    ``gr_linear_mxfp4`` in gr_mxfp4.h.  ``swiglu``: ``silu(gate) * up`` of the two
+    halves of ``w``'s rows.  Returns ``[T, N]`` of ``out_dtype`` (float32, fp16, bf16), or
+    with ``quantized`` the pair ``quant_mxfp4`` would give of the float32 results.
+    ``out`` is aligned to 16 bytes (float32), 8 (16 bits) or, each of its rows, 16 (4 bits)."""
+    dev = _need_cuda(x, x_scale, w, w_scale, out, out_scale)
+    K = _mx_rows("x", x, x_scale)
+    T, rows = x.shape[0], w.shape[0]
+    if _mx_rows("w", w, w_scale) != K or (swiglu and rows % 2):
+        raise ValueError("w must be [out_features, in_features / 2] (twice the rows with swiglu)")
+    N = rows // 2 if swiglu else rows
+    if quantized:
+        if N % MXFP4_BLOCK:
+            raise ValueError("a quantized result needs a multiple of 32 columns")
+        new = _mx_new(T, N, dev) if out is None or out_scale is None else (None, None)
+        out = new[0] if out is None else out
+        out_scale = new[1] if out_scale is None else out_scale
+        if _mx_rows("out", out, out_scale) != N or out.shape[0] != T:
+            raise ValueError("out must be a [tokens, out_features / 2] tensor")
+        pitch, odt = _row_stride(out, T, N // 2), _C.GR_DTYPE_MXFP4
+    else:
+        if out_scale is not None:
+            raise ValueError("out_scale goes with quantized=True")
+        if out is None:
+            out = torch.empty((T, N), dtype=out_dtype, device=dev)
+        else:
+            _rows("out", out)
+            if out.shape != (T, N) or out.dtype != out_dtype:
+                raise ValueError("out must be [tokens, out_features] of the result's type")
+        pitch, odt = _row_stride(out, T, N), _dtype_code(out)
+    _launch(dev, "gr_linear_mxfp4", out.data_ptr(), pitch, _ptr(out_scale),
+            _row_stride(out_scale, T, N // MXFP4_BLOCK) if quantized else 0, x.data_ptr(), _row_stride(x, T, K // 2),
+            x_scale.data_ptr(), _row_stride(x_scale, T, K // MXFP4_BLOCK), w.data_ptr(), _row_stride(w, rows, K // 2),
+            w_scale.data_ptr(), _row_stride(w_scale, rows, K // MXFP4_BLOCK), T, N, K, int(swiglu), odt, _stream(dev))
+    return (out, out_scale) if quantized else out
+
+
+def expert_mlp_mxfp4(x: torch.Tensor, gate_up: torch.Tensor, gate_up_scale: torch.Tensor, down: torch.Tensor,
+                     down_scale: torch.Tensor, weights: torch.Tensor, ids: torch.Tensor, *,
+                     out: torch.Tensor | None = None, workspace: torch.Tensor | None = None,
+                     status: torch.Tensor | None = None) -> torch.Tensor:
+    """``expert_mlp`` with 4-bit weights: ``gate_up [E, 2 F, H / 2]`` (gate | up) and ``down
+    [E, H, F / 2]`` with their scales ``[E, 2 F, H / 32]`` and ``[E, H, F / 32]``, all
+    contiguous; ``x [T, H]`` (fp16 or bf16) and the gated products are quantised as
+    ``quant_mxfp4`` does; see ``gr_expert_mlp_mxfp4`` in gr_mxfp4.h.  ``workspace``: uint8,
+    contiguous, ``expert_mlp_mxfp4_workspace_bytes`` of it (allocated when None)."""
+    dev = _need_cuda(x, gate_up, down, weights, ids, gate_up_scale, down_scale, out, workspace, status)
+    _rows("x", x)
+    T, H = x.shape
+    if gate_up.dim() != 3 or down.dim() != 3 or gate_up.shape[1] % 2:
+        raise ValueError("gate_up must be [E, 2 F, H / 2] and down [E, H, F / 2]")
+    E, F = gate_up.shape[0], gate_up.shape[1] // 2
+    if H % MXFP4_BLOCK or F % MXFP4_BLOCK:
+        raise ValueError("4-bit experts need multiples of 32 features")
+    for name, t, types, shape in (("gate_up", gate_up, _MX_CODES, (E, 2 * F, H // 2)),
+                                  ("down", down, _MX_CODES, (E, H, F // 2)),
+                                  ("gate_up_scale", gate_up_scale, _MX_SCALES, (E, 2 * F, H // MXFP4_BLOCK)),
+                                  ("down_scale", down_scale, _MX_SCALES, (E, H, F // MXFP4_BLOCK))):
+        if t.dtype not in types or t.shape != shape or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous {list(shape)} tensor of {' or '.join(map(str, types))}")
+    if ids.dim() != 2 or ids.shape[0] != T or ids.dtype != torch.int32 or not ids.is_contiguous():
+        raise ValueError("ids must be a contiguous int32 [tokens, top_k] tensor")
+    if weights.shape != ids.shape or weights.dtype != torch.float32 or not weights.is_contiguous():
+        raise ValueError("weights must be a contiguous float32 [tokens, top_k] tensor")
+    k = ids.shape[1]
+    if k < 1:
+        raise ValueError("ids must name at least one expert a token")
+    if max(k, E, F) > _INT_MAX:
+        raise ValueError("ids, gate_up or down has a size above 2^31 - 1")
+    if out is None:
+        out = torch.empty((T, H), dtype=x.dtype, device=dev)
+    else:
+        _rows("out", out)
+        if out.shape != x.shape or out.dtype != x.dtype:
+            raise ValueError("out must match x")
+    if workspace is None:
+        workspace = torch.empty(expert_mlp_mxfp4_workspace_bytes(T, k, E, H, F), dtype=torch.uint8, device=dev)
+    _launch(dev, "gr_expert_mlp_mxfp4", out.data_ptr(), _row_stride(out, T, H), x.data_ptr(), _row_stride(x, T, H),
+            gate_up.data_ptr(), gate_up_scale.data_ptr(), down.data_ptr(), down_scale.data_ptr(), weights.data_ptr(),
+            ids.data_ptr(), T, k, E, H, F, _dtype_code(x), workspace.data_ptr(), _workspace_bytes(workspace), _ptr(status),
+            _stream(dev))
+    return out
+
+
+def expert_mlp_mxfp4_workspace_bytes(num_tokens: int, top_k: int, num_experts: int, hidden: int, ffn: int) -> int:
+    """Workspace of ``expert_mlp_mxfp4``."""
+    return int(_C.lib().gr_expert_mlp_mxfp4_workspace_size(num_tokens, top_k, num_experts, hidden, ffn))

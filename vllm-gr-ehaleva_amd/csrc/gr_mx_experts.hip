@@ -29,10 +29,19 @@ struct MxWorkspace {
   int blocks;
 };
 
-// Rows of a tile, by the rows an expert gets on average.
-int mx_tile_rows(int64_t rows, int E) { return rows <= 8ll * E ? 16 : rows <= 80ll * E ? 32 : 128; }
-// columns of a wave of the down product with tiles of bm rows (launch_mx_experts)
-int mx_wave_cols(int bm) { return bm == 16 ? 16 : 64; }
+// Rows of a tile, by the rows an expert gets on average: few rows are bound by the weights'
+// way from memory, many by the products and the results.  Measured (64 experts of 768
+// features, hidden 2048, 8 of them a token; us of both products, by tile rows):
+//   rows an expert    1     2     8    16    32    64   128   256   375   625  1024
+//   16             25.4  31.4  40.3
+//   32                   29.9  35.8  42.5  50.6  59.2  97.5
+//   64                   33.8  41.0  42.3  45.6  53.0  77.5
+//   128                                    55.3  66.2  79.9   115   155   233   346
+//   256                                    70.5  75.8  90.3   119   135   205   303
+int mx_tile_rows(int64_t rows, int E) {
+  return 2 * rows <= 3ll * E ? 16 : rows <= 20ll * E ? 32 : rows <= 144ll * E ? 64 : rows <= 300ll * E ? 128 : 256;
+}
+constexpr int MX_WAVE_COLS = 64;  // columns of a wave of the down product, whatever its tiles
 
 MxWorkspace plan_mx_workspace(int T, int k, int E, int H, int F, int bm) {
   MxWorkspace w{};
@@ -60,13 +69,19 @@ MxWorkspace plan_mx_workspace(int T, int k, int E, int H, int F, int bm) {
 void launch_mx_experts(const MxArgs& up, const MxArgs& down, int tiles, int bm, hipStream_t stream) {
   if (bm == 16) {
     launch_mx_few<1, 2, 4, MM_SWIGLU_Q, true>(up, tiles, stream);
-    launch_mx_few<1, 1, 4, MM_PLAIN, true>(down, tiles, stream);
+    launch_mx_few<1, 4, 2, MM_PLAIN, true>(down, tiles, stream);
   } else if (bm == 32) {
-    launch_mx<32, 256, 1, 4, 2, MM_SWIGLU_Q, true>(up, tiles, stream);
-    launch_mx<32, 256, 1, 4, 2, MM_PLAIN, true>(down, tiles, stream);
+    launch_mx<32, 256, 1, 4, 2, 1, MM_SWIGLU_Q, true>(up, tiles, stream);
+    launch_mx<32, 256, 1, 4, 2, 1, MM_PLAIN, true>(down, tiles, stream);
+  } else if (bm == 64) {
+    launch_mx<64, 128, 2, 2, 3, 2, MM_SWIGLU_Q, true>(up, tiles, stream);
+    launch_mx<64, 128, 4, 2, 3, 2, MM_PLAIN, true>(down, tiles, stream);
+  } else if (bm == 128) {
+    launch_mx<128, 256, 2, 4, 3, 2, MM_SWIGLU_Q, true>(up, tiles, stream);
+    launch_mx<128, 256, 2, 4, 3, 2, MM_PLAIN, true>(down, tiles, stream);
   } else {
-    launch_mx<128, 256, 2, 4, 3, MM_SWIGLU_Q, true>(up, tiles, stream);
-    launch_mx<128, 256, 2, 4, 3, MM_PLAIN, true>(down, tiles, stream);
+    launch_mx<256, 256, 2, 4, 2, 2, MM_SWIGLU_Q, true>(up, tiles, stream);
+    launch_mx<256, 256, 2, 4, 2, 2, MM_PLAIN, true>(down, tiles, stream);
   }
 }
 
@@ -103,7 +118,7 @@ extern "C" gr_status_t gr_expert_mlp_mxfp4(void* out, int64_t out_stride, const 
     return GR_ERR_UNSUPPORTED;
   const int bm = mx_tile_rows((int64_t)T * top_k, num_experts);
   const MxWorkspace l = plan_mx_workspace(T, top_k, num_experts, H, F, bm);
-  const int cols = bm == 16 ? 16 : 128;  // results of a workgroup, in the narrower product
+  const int cols = bm == 16 ? 32 : bm == 64 ? 64 : 128;  // results of a workgroup, in the narrower product
   if (l.max_tiles * ((std::max(F, H) + cols - 1) / cols) > GRID_MAX - 8 || T > GRID_MAX) return GR_ERR_UNSUPPORTED;
   if (!workspace || !aligned(workspace, 256) || workspace_bytes < (size_t)l.bytes) return GR_ERR_WORKSPACE;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
@@ -174,7 +189,7 @@ extern "C" gr_status_t gr_expert_mlp_mxfp4(void* out, int64_t out_stride, const 
   dn.scatter = 1;
   launch_mx_experts(up, dn, (int)l.max_tiles, bm, stream);
 
-  const CombineArgs c{out, out_stride, ws + l.y, dn.out_exp, mx_wave_cols(bm), weights, ids, T, top_k, num_experts, H};
+  const CombineArgs c{out, out_stride, ws + l.y, dn.out_exp, MX_WAVE_COLS, weights, ids, T, top_k, num_experts, H};
   const dim3 grid((unsigned)T, (unsigned)((H + 2047) / 2048));
   auto go = [&](auto k) { hipLaunchKernelGGL(k, grid, dim3(256), 0, stream, c); };
   if (dtype == GR_DTYPE_BF16) go(expert_combine_k<GR_DTYPE_BF16, true>);

@@ -15,6 +15,8 @@
 // of row r, so that a stage's scales are two neighbouring bytes of that row.
 #pragma once
 
+#include <type_traits>
+
 #include "gr_block_mm.h"
 
 namespace gr {
@@ -50,29 +52,39 @@ struct MxArgs : MmArgs {  // kbytes: in_features / 2; strides of x and w in byte
 };
 
 // BM rows by BN weight rows, WM x WN waves (SwiGLU: 16 gate rows and their 16 up rows alternate)
-template <int BM, int BN, int WM, int WN, int MODE, bool EXPERTS>
+template <int BM, int BN, int WM, int WN, int CH, int MODE, bool EXPERTS>
 struct Mx {
   static constexpr bool GATED = MODE == MM_SWIGLU || MODE == MM_SWIGLU_Q;
   static constexpr bool QUANT = MODE == MM_SWIGLU_Q || MODE == MM_PLAIN_Q;
   using M = Mm<GR_DTYPE_BF16, BM, BN, WM, WN, GATED ? MM_SWIGLU : MM_PLAIN, EXPERTS, false>;  // rows of bytes
   static constexpr int NW = WM * WN, ROWS = BM + BN, TILE = M::TILE, LPS = M::LPS, FM = M::FM, FN = M::FN, OC = M::OC;
-  static constexpr int SPS = (2 * ROWS + 64 * NW - 1) / (64 * NW);  // transfers of scales a wave and stage, a dword a lane
-  static constexpr int OPS = LPS + SPS, SCALES = NW * SPS * 256;
-  static_assert(ROWS % (8 * NW) == 0 && NW % 2 == 0, "whole transfers; a wave's rows keep their parity of 8");
+  // Scales come CH stages at a time: what a transfer of them costs is its rows' lines,
+  // whatever it takes of each (a dword a lane: 4 CH / 2 lanes a row).
+  static constexpr int LANES = 2 * CH, PER = 64 / LANES, SPS = (ROWS + PER * NW - 1) / (PER * NW), SCALES = NW * SPS * 256;
+  static_assert(BM % (8 * NW) == 0 && BN % (8 * NW) == 0 && NW % 2 == 0, "whole transfers; a wave's rows keep their parity of 8");
   static_assert(!QUANT || OC / WN % 32 == 0, "a block of the result is one wave's");
   using Acc = typename M::Acc;
 
-  // Chunks of 16 bytes in LDS are XORed with the row's bits 1 to 3: 16 rows of one
-  // logical chunk, which a fragment reads at once, lie on all 64 banks.
-  __device__ static __forceinline__ int swizzle(int row) { return row >> 1 & 7; }
+  // Chunks of 16 bytes in LDS are XORed so that the four chunks of 16 rows that a
+  // fragment reads at once meet no bank twice (5.2 clocks a read of 64 lanes; with the
+  // row's low bits alone, or its bits 1 to 3, 8.5).
+  __device__ static __forceinline__ int swizzle(int row) { return (row & 7) ^ (row >> 3 & 1); }
+  // The same for the 8 bytes of scales of a stage, of which a row has CH side by side
+  // (u16 reads of 16 rows 16 bytes apart take 4.3 clocks, so 2.8).
+  static_assert(CH == 1 || CH == 2 || CH == 4, "stages of scales");
+  __device__ static __forceinline__ int scale_swizzle(int row) { return row >> (CH == 4 ? 2 : 3) & (CH - 1); }
 
   struct Source {
     typename M::Source rows;
-    const uint8_t* scale[SPS];
+    const uint8_t* ws;
+    int scale_row[SPS];  // of x, or (past BM) of the weights
   };
   __device__ static __forceinline__ int w_row(const MmTile& t, int b, int N) {  // weight row of tile row BM + b
     if constexpr (GATED) return min(t.n0 + (b >> 5) * 16 + (b & 15), N - 1) + (b >> 4 & 1) * N;
     else return min(t.n0 + b, N - 1);
+  }
+  __device__ static __forceinline__ int tile_row(int i, int wave, int lane) {  // of transfer i of scales
+    return (wave * SPS + i) * PER + lane / LANES;
   }
   __device__ static __forceinline__ void source(const MxArgs& a, const MmTile& t, int wave, int lane, Source& s) {
     s.rows.ch = ((lane & 7) ^ swizzle(wave * 8 + (lane >> 3))) * 16;
@@ -83,7 +95,7 @@ struct Mx {
 #pragma unroll
     for (int i = 0; i < LPS; ++i) {
       const int r8 = 8 * (wave + NW * i), row = r8 + (lane >> 3);
-      if (r8 < BM) {
+      if (8 * NW * i < BM) {
         s.rows.buf[i] = xb;
         s.rows.off[i] = (uint32_t)((M::x_row(a, t, row) - first) * (uint32_t)a.x_stride) + s.rows.ch;
       } else {
@@ -93,39 +105,46 @@ struct Mx {
         s.rows.off[i] = (uint32_t)((w_row(t, b, a.N) - (up ? a.N : 0) - t.n0) * (uint32_t)a.w_stride) + s.rows.ch;
       }
     }
-    const uint8_t* ws = a.ws4;
-    if constexpr (EXPERTS) ws += __builtin_amdgcn_readfirstlane(a.tiles[t.mt].x) * a.ws4_expert;
+    s.ws = a.ws4;
+    if constexpr (EXPERTS) s.ws += __builtin_amdgcn_readfirstlane(a.tiles[t.mt].x) * a.ws4_expert;
 #pragma unroll
-    for (int i = 0; i < SPS; ++i) {  // entry: a row's first or second four blocks of the stage
-      const int r = min(((wave * SPS + i) * 64 + lane) >> 1, ROWS - 1);
-      s.scale[i] = r < BM ? a.xs4 + M::x_row(a, t, r) * a.xs4_row : ws + w_row(t, r - BM, a.N) * a.ws4_row;
+    for (int i = 0; i < SPS; ++i) {
+      const int r = min(tile_row(i, wave, lane), ROWS - 1);
+      s.scale_row[i] = r < BM ? M::x_row(a, t, r) : w_row(t, r - BM, a.N);
     }
   }
 
-  // Stage k into the buffers at LDS bytes `rows` and `scales` of lds.  Past a row's
+  // Scales of stages CH c .. into the buffer at LDS byte `at` of lds.  Past a row's
   // last block its last four scales stand (a NaN there is the row's anyway); the
   // numbers there are zeros.
-  __device__ static __forceinline__ void fetch(const MxArgs& a, const Source& s, int k, uint8_t* lds, int rows, int scales,
-                                               int wave, int lane) {
-    const uint32_t lds0 = (uint32_t)reinterpret_cast<uintptr_t>(lds);
-    if (a.loose) {  // (its loads are waited for before anything below is sent: the transfers' count stays an upper bound)
+  __device__ static __forceinline__ void fetch_scales(const MxArgs& a, const Source& s, int c, uint8_t* lds, int at, int wave,
+                                                      int lane) {
 #pragma unroll
-      for (int i = 0; i < SPS; ++i) {
+    for (int i = 0; i < SPS; ++i) {
+      const int r = tile_row(i, wave, lane);
+      const int b0 = 8 * CH * c + 4 * ((lane & (LANES - 1)) ^ 2 * scale_swizzle(r));
+      const bool x = r < BM;
+      const uint8_t* row = (x ? a.xs4 : s.ws) + s.scale_row[i] * (x ? a.xs4_row : a.ws4_row);
+      const int to = at + (wave * SPS + i) * 256;
+      if (a.loose) {
         uint32_t v = 0;
 #pragma unroll
-        for (int b = 0; b < 4; ++b) v |= (uint32_t)s.scale[i][min(8 * k + 4 * (lane & 1) + b, a.blocks - 1)] << (8 * b);
-        *reinterpret_cast<uint32_t*>(lds + scales + ((wave * SPS + i) * 64 + lane) * 4) = v;
+        for (int b = 0; b < 4; ++b) v |= (uint32_t)row[min(b0 + b, a.blocks - 1)] << (8 * b);
+        *reinterpret_cast<uint32_t*>(lds + to + lane * 4) = v;
+      } else {
+        dma_v1((uint32_t)reinterpret_cast<uintptr_t>(lds) + to, row + min(b0, a.blocks - 4));
       }
-    } else {
-      const int at = min(8 * k + 4 * (lane & 1), a.blocks - 4);
-#pragma unroll
-      for (int i = 0; i < SPS; ++i) dma_v1(lds0 + scales + (wave * SPS + i) * 256, s.scale[i] + at);
     }
-    M::fetch(a, s.rows, k, lds0 + rows, 0, wave);
+  }
+
+  // Transfer i of stage k's rows into the buffer at LDS byte `lds`.
+  __device__ static __forceinline__ void fetch_rows(const MxArgs& a, const Source& s, int i, int k, uint32_t lds, int wave) {
+    const bool in = k * 128 + (int)s.rows.ch < a.kbytes;  // (a short last stage: zeros behind its end)
+    dma_b(lds + (uint32_t)(wave + NW * i) * 1024, s.rows.buf[i], in ? s.rows.off[i] : MM_NOWHERE, (uint32_t)k * 128);
   }
 
   struct Lane {
-    int xo, wo, fch[2], xso, wso;
+    int xo, wo, fch[2], xso, wso, ssw;
   };
   __device__ static __forceinline__ Lane lane_of(int wm, int wn, int lane) {
     const int r16 = lane & 15, q = lane >> 4;
@@ -135,8 +154,9 @@ struct Mx {
     const int xr = wm * (BM / WM) + r16, wr = BM + wn * (BN / WN) + r16;
     l.xo = xr * 128;
     l.wo = wr * 128;
-    l.xso = xr * 8 + 2 * q;
-    l.wso = wr * 8 + 2 * q;
+    l.ssw = scale_swizzle(r16) * 8;
+    l.xso = xr * (8 * CH) + 2 * q;
+    l.wso = wr * (8 * CH) + 2 * q;
     return l;
   }
   struct Frag {  // a lane's two blocks of a fragment of 16 rows
@@ -175,15 +195,23 @@ template <typename M> __device__ __forceinline__ uint32_t mx_block(const typenam
 }
 
 // ST stages of LDS, one barrier a stage, as block_mm: stage s has landed when all but the
-// ST - 2 younger ones' transfers have; past its barrier nobody reads stage s - 1, whose
-// buffer takes stage s + ST - 1.
-template <int BM, int BN, int WM, int WN, int ST, int MODE, bool EXPERTS>
-__global__ __launch_bounds__(64 * WM * WN, 2) void mx_mm(MxArgs a) {
-  using X = Mx<BM, BN, WM, WN, MODE, EXPERTS>;
+// ST - 2 younger ones' transfers of rows have (scales are sent ahead of their first stage's
+// rows, so they have too); past its barrier nobody reads stage s - 1, whose buffer takes
+// stage s + ST - 1, nor the scales before the current ones.
+template <int BM, int BN, int WM, int WN, int ST, int CH, int MODE, bool EXPERTS> struct MxLds {
+  using X = Mx<BM, BN, WM, WN, CH, MODE, EXPERTS>;
+  static constexpr int NS = (ST - 1 + CH - 1) / CH + 1;  // buffers of scales
+  static constexpr int BYTES = ST * X::TILE + NS * X::SCALES;
+  static constexpr int WAVES = X::NW / 4 * (BYTES <= 80 * 1024 ? 2 : 1);  // of a SIMD: two workgroups, where LDS has room
+};
+template <int BM, int BN, int WM, int WN, int ST, int CH, int MODE, bool EXPERTS>
+__global__ __launch_bounds__(64 * WM * WN, (MxLds<BM, BN, WM, WN, ST, CH, MODE, EXPERTS>::WAVES)) void mx_mm(MxArgs a) {
+  using X = Mx<BM, BN, WM, WN, CH, MODE, EXPERTS>;
   using M = typename X::M;
   constexpr int BLOCKS = X::OC / 32, PITCH = X::OC / 2 + 16;  // of a row in 4 bits
+  constexpr int NS = MxLds<BM, BN, WM, WN, ST, CH, MODE, EXPERTS>::NS;
   static_assert(!X::QUANT || BM * (PITCH + BLOCKS) <= ST * X::TILE, "the results' rows fit");
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[ST * (X::TILE + X::SCALES)];
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[MxLds<BM, BN, WM, WN, ST, CH, MODE, EXPERTS>::BYTES];
   MmTile t;
   if (!M::tile(a, t)) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -192,8 +220,12 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mx_mm(MxArgs a) {
   X::source(a, t, wave, lane, src);
   const typename X::Lane l = X::lane_of(wm, wn, lane);
   const int n = __builtin_amdgcn_readfirstlane((a.kbytes + 127) >> 7);
-  auto fetch = [&](int s, int buf) __attribute__((always_inline)) {
-    X::fetch(a, src, s, lds, buf * X::TILE, ST * X::TILE + buf * X::SCALES, wave, lane);
+  const uint32_t lds0 = (uint32_t)reinterpret_cast<uintptr_t>(lds);
+  auto scales = [&](int s) __attribute__((always_inline)) {
+    if (s % CH == 0) X::fetch_scales(a, src, s / CH, lds, ST * X::TILE + s / CH % NS * X::SCALES, wave, lane);
+  };
+  auto scales_at = [&](int s) __attribute__((always_inline)) {
+    return lds + ST * X::TILE + s / CH % NS * X::SCALES + (s % CH * 8 ^ l.ssw);
   };
   typename X::Acc acc;
 #pragma unroll
@@ -202,25 +234,49 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mx_mm(MxArgs a) {
     for (int j = 0; j < X::FM; ++j) acc[i][j] = mm4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int s = 0; s < ST - 1; ++s)
-    if (s < n) fetch(s, s);
-  int buf = 0;
-  for (int s = 0; s < n; ++s) {
-    if (s + ST - 1 <= n) mm_wait_barrier<(ST - 2) * X::OPS>();
-    else mm_wait_barrier<0>();
-    if (s + ST - 1 < n) fetch(s + ST - 1, buf == 0 ? ST - 1 : buf - 1);
-    const uint8_t *p = lds + buf * X::TILE, *sc = lds + ST * X::TILE + buf * X::SCALES;
-    typename X::Frag w[X::FN];
+    if (s < n) {
+      scales(s);
 #pragma unroll
-    for (int i = 0; i < X::FN; ++i) w[i] = X::read(p + l.wo + i * 2048, sc + l.wso + i * 128, l);
+      for (int i = 0; i < X::LPS; ++i) X::fetch_rows(a, src, i, s, lds0 + s * X::TILE, wave);
+    }
+  int buf = 0;
+  // The transfers of a stage ahead are sent between the first products: sent in one go
+  // they keep their wave from its products until the last is taken (512 x 2048 of 6144
+  // features, 64 x 128 tiles, 17.2 us and 15.4).
+  auto step = [&](int s, auto ahead) __attribute__((always_inline)) {
+    constexpr bool AHEAD = decltype(ahead)::value;
+    constexpr int SLOTS = X::FM * X::FN, EACH = (X::LPS + SLOTS - 1) / SLOTS;
+    const uint8_t *p = lds + buf * X::TILE, *sc = scales_at(s);
+    const uint32_t to = lds0 + (buf == 0 ? ST - 1 : buf - 1) * X::TILE;
+    typename X::Frag w[X::FN], x, next;
+#pragma unroll
+    for (int i = 0; i < X::FN; ++i) w[i] = X::read(p + l.wo + i * 2048, sc + l.wso + i * (128 * CH), l);
+    x = X::read(p + l.xo, sc + l.xso, l);
+    if constexpr (AHEAD) scales(s + ST - 1);
 #pragma unroll
     for (int j = 0; j < X::FM; ++j) {
-      const typename X::Frag x = X::read(p + l.xo + j * 2048, sc + l.xso + j * 128, l);
+      if (j + 1 < X::FM) next = X::read(p + l.xo + (j + 1) * 2048, sc + l.xso + (j + 1) * (128 * CH), l);
 #pragma unroll
-      for (int i = 0; i < X::FN; ++i) acc[i][j] = mx_mma<0>(w[i].v[0], w[i].s, x.v[0], x.s, acc[i][j]);
+      for (int i = 0; i < X::FN; ++i) {
+        if constexpr (AHEAD)
 #pragma unroll
-      for (int i = 0; i < X::FN; ++i) acc[i][j] = mx_mma<1>(w[i].v[1], w[i].s, x.v[1], x.s, acc[i][j]);
+          for (int c = 0; c < EACH; ++c)
+            if ((j * X::FN + i) * EACH + c < X::LPS) X::fetch_rows(a, src, (j * X::FN + i) * EACH + c, s + ST - 1, to, wave);
+        acc[i][j] = mx_mma<0>(w[i].v[0], w[i].s, x.v[0], x.s, acc[i][j]);
+        acc[i][j] = mx_mma<1>(w[i].v[1], w[i].s, x.v[1], x.s, acc[i][j]);
+      }
+      x = next;
     }
     buf = buf + 1 == ST ? 0 : buf + 1;
+  };
+  int s = 0;
+  for (; s + ST - 1 < n; ++s) {
+    mm_wait_barrier<(ST - 2) * X::LPS>();
+    step(s, std::true_type());
+  }
+  for (; s < n; ++s) {
+    mm_wait_barrier<0>();
+    step(s, std::false_type());
   }
   __syncthreads();
   if constexpr (X::QUANT) {
@@ -297,8 +353,8 @@ __global__ __launch_bounds__(64 * WK) void mx_few(MxArgs a) {
     Piece f{{{0, 0, 0, 0}, {0, 0, 0, 0}}, 0};
     const int left = a.blocks - 8 * s - 2 * q;
     if (left > 0) f.v[0] = *reinterpret_cast<const mm4i_t*>(p + (int64_t)s * 128);
-    if (left > 1) f.v[1] = *reinterpret_cast<const mm4i_t*>(p + (int64_t)s * 128 + 16);
     if (left > 1) {
+      f.v[1] = *reinterpret_cast<const mm4i_t*>(p + (int64_t)s * 128 + 16);
       uint16_t two;
       __builtin_memcpy(&two, sp + (int64_t)s * 8, 2);
       f.s = two;
@@ -315,12 +371,13 @@ __global__ __launch_bounds__(64 * WK) void mx_few(MxArgs a) {
   for (int s0 = wave; s0 < n; s0 += WK * U) {
     Piece w[U][FN], x[U][FM];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
+    for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int i = 0; i < FN; ++i) w[u][i] = load(w0[i], ws[i], s0 + u * WK);
 #pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
       for (int j = 0; j < FM; ++j) x[u][j] = load(x0[j], xs[j], s0 + u * WK);
-    }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (u && s0 + u * WK >= n) break;
@@ -370,13 +427,13 @@ __global__ __launch_bounds__(64 * WK) void mx_few(MxArgs a) {
   }
 }
 
-template <int BM, int BN, int WM, int WN, int ST, int MODE, bool EXPERTS>
+template <int BM, int BN, int WM, int WN, int ST, int CH, int MODE, bool EXPERTS>
 void launch_mx(MxArgs a, int tiles_m, hipStream_t stream) {
-  using X = Mx<BM, BN, WM, WN, MODE, EXPERTS>;
+  using X = Mx<BM, BN, WM, WN, CH, MODE, EXPERTS>;
   a.tiles_m = tiles_m;
   a.tiles_n = (a.N + X::OC - 1) / X::OC;
   const int64_t total = (int64_t)tiles_m * a.tiles_n;
-  hipLaunchKernelGGL((mx_mm<BM, BN, WM, WN, ST, MODE, EXPERTS>), dim3((unsigned)((total + 7) / 8 * 8)), dim3(64 * WM * WN),
+  hipLaunchKernelGGL((mx_mm<BM, BN, WM, WN, ST, CH, MODE, EXPERTS>), dim3((unsigned)((total + 7) / 8 * 8)), dim3(64 * WM * WN),
                      0, stream, a);
 }
 template <int FM, int NF, int WK, int MODE, bool EXPERTS>

@@ -92,9 +92,10 @@ class LLM:
     (the reference keeps it as a -inf-score beam, serving_engine.py:504-506,
     which only reaches the output when fewer than beam_width valid sequences
     exist).  ``quantization="fp8"`` serves the layers' projections and experts in
-    e4m3 (``quantize_weights``); weights that come with their scales are served so
-    in any case.  Sizes that the 8-bit products do not take are refused here.  It
-    halves the layers' memory; a step is faster with experts, not without."""
+    e4m3, ``"mxfp4"`` in 4 bits (``quantize_weights``); weights that come with their
+    scales are served so in any case.  Sizes that these products do not take are
+    refused here.  e4m3 halves the layers' memory; a step is faster with experts, not
+    without.  4 bits take 27 % of it."""
 
     def __init__(self, cfg: DecoderConfig = SID_DECODER_1P7B, *, seed: int = 0, device="cuda",
                  num_blocks: int = 4096, block_size: int = 16, eos_token_id: int | None = None,
@@ -104,12 +105,12 @@ class LLM:
         dev = torch.device(device)
         if dev.type != "cuda":
             raise ValueError("the beam path runs on a HIP device (torch 'cuda')")
-        if quantization not in (None, "fp8"):
-            raise ValueError("quantization must be None or 'fp8'")
+        if quantization not in (None, "fp8", "mxfp4"):
+            raise ValueError("quantization must be None, 'fp8' or 'mxfp4'")
         if weights is None:
             weights = init_weights(cfg, seed, dev)
         if quantization:
-            weights = quantize_weights(weights)
+            weights = quantize_weights(weights, quantization)
         self.cfg = cfg
         self.model = SidDecoder(cfg, weights, max_position=max_position)
         self.runner = SidModelRunner(self.model, num_blocks, block_size, use_graphs=use_graphs)

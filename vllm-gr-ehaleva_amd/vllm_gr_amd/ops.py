@@ -955,25 +955,36 @@ _MX_CODES = (torch.uint8, torch.float4_e2m1fn_x2)
 _MX_SCALES = (torch.uint8, torch.float8_e8m0fnu)
 
 
-def _mx_rows(name: str, t: torch.Tensor, scale: torch.Tensor) -> int:
-    """Features of the rows of a 4-bit matrix."""
-    _rows(name, t)
-    K = 2 * t.shape[1]
-    if t.dtype not in _MX_CODES or K % MXFP4_BLOCK or K > _INT_MAX:
-        raise ValueError(f"{name} must hold two codes a byte (uint8 or float4_e2m1fn_x2), 16 bytes a block of 32")
-    _mx_scales(f"{name}_scale" if name != "out" else "out_scale", scale, t.shape[0], K)
-    return K
+def _mx_rows(name: str, t: torch.Tensor, scale: torch.Tensor) -> tuple[int, int, int, int]:
+    """Rows and features of a 4-bit matrix, and the bytes from row to row of its codes and of its scales."""
+    if t.dim() != 2 or t.stride(1) != 1 or t.dtype not in _MX_CODES:
+        raise ValueError(f"{name} must be a [tokens, features / 2] tensor of two codes a byte (uint8 or "
+                         "float4_e2m1fn_x2), a row's side by side")
+    rows, half = t.shape
+    blocks = half // 16
+    if half != 16 * blocks or half > _INT_MAX // 2 or rows > _INT_MAX:
+        raise ValueError(f"{name} must have a multiple of 32 features, and at most 2^31 - 1 rows or features")
+    if scale.shape != (rows, blocks) or scale.dtype not in _MX_SCALES or (blocks > 1 and scale.stride(1) != 1):
+        raise ValueError(f"{name}'s scale must be a uint8 or float8_e8m0fnu [rows, features / 32] tensor, a row's bytes "
+                         "side by side")
+    if rows > 1:
+        return rows, 2 * half, t.stride(0), scale.stride(0)
+    return rows, 2 * half, half, blocks
 
 
-def _mx_scales(name: str, t: torch.Tensor, rows: int, features: int) -> None:
-    if (t.dtype not in _MX_SCALES or t.shape != (rows, features // MXFP4_BLOCK)
-            or (t.shape[1] > 1 and t.stride(1) != 1)):
-        raise ValueError(f"{name} must be a uint8 or float8_e8m0fnu [rows, features / 32] tensor, a row's bytes side by side")
-
-
-def _mx_new(rows: int, features: int, dev):
-    return (torch.empty((rows, features // 2), dtype=torch.uint8, device=dev),
-            torch.empty((rows, features // MXFP4_BLOCK), dtype=torch.uint8, device=dev))
+def _mx_out(out: torch.Tensor | None, scale: torch.Tensor | None, rows: int, features: int, dev):
+    """A 4-bit result and its scales, new where None, and the bytes from row to row of both."""
+    given = out is not None or scale is not None
+    if out is None:
+        out = torch.empty((rows, features // 2), dtype=torch.uint8, device=dev)
+    if scale is None:
+        scale = torch.empty((rows, features // MXFP4_BLOCK), dtype=torch.uint8, device=dev)
+    if not given:
+        return out, scale, features // 2, features // MXFP4_BLOCK
+    got_rows, got_features, pitch, scale_pitch = _mx_rows("out", out, scale)
+    if got_rows != rows or got_features != features:
+        raise ValueError("out must be a [tokens, features / 2] tensor of as many tokens and features as the result")
+    return out, scale, pitch, scale_pitch
 
 
 def quant_mxfp4(x: torch.Tensor, *, out: torch.Tensor | None = None, scale: torch.Tensor | None = None):
@@ -986,13 +997,9 @@ def quant_mxfp4(x: torch.Tensor, *, out: torch.Tensor | None = None, scale: torc
     T, K = x.shape
     if K % MXFP4_BLOCK:
         raise ValueError("x must have a multiple of 32 features")
-    new = _mx_new(T, K, dev) if out is None or scale is None else (None, None)
-    out = new[0] if out is None else out
-    scale = new[1] if scale is None else scale
-    if _mx_rows("out", out, scale) != K or out.shape[0] != T:
-        raise ValueError("out must be a [tokens, features / 2] tensor")
-    _launch(dev, "gr_quant_mxfp4", out.data_ptr(), _row_stride(out, T, K // 2), scale.data_ptr(),
-            _row_stride(scale, T, K // MXFP4_BLOCK), x.data_ptr(), _row_stride(x, T, K), T, K, _dtype_code(x), _stream(dev))
+    out, scale, pitch, scale_pitch = _mx_out(out, scale, T, K, dev)
+    _launch(dev, "gr_quant_mxfp4", out.data_ptr(), pitch, scale.data_ptr(), scale_pitch, x.data_ptr(),
+            _row_stride(x, T, K), T, K, _dtype_code(x), _stream(dev))
     return out, scale
 
 
@@ -1001,16 +1008,15 @@ def dequant_mxfp4(x: torch.Tensor, scale: torch.Tensor, *, dtype: torch.dtype = 
     """The values ``[T, K]`` of 4-bit rows ``x [T, K / 2]`` with ``scale [T, K / 32]``, in
     ``dtype`` (float32, fp16, bf16); see ``gr_dequant_mxfp4`` in gr_mxfp4.h."""
     dev = _need_cuda(x, scale, out)
-    K = _mx_rows("x", x, scale)
-    T = x.shape[0]
+    T, K, pitch, scale_pitch = _mx_rows("x", x, scale)
     if out is None:
         out = torch.empty((T, K), dtype=dtype, device=dev)
     else:
         _rows("out", out)
         if out.shape != (T, K) or out.dtype != dtype:
             raise ValueError("out must be a [tokens, features] tensor of dtype")
-    _launch(dev, "gr_dequant_mxfp4", out.data_ptr(), _row_stride(out, T, K), x.data_ptr(), _row_stride(x, T, K // 2),
-            scale.data_ptr(), _row_stride(scale, T, K // MXFP4_BLOCK), T, K, _dtype_code(out), _stream(dev))
+    _launch(dev, "gr_dequant_mxfp4", out.data_ptr(), _row_stride(out, T, K), x.data_ptr(), pitch, scale.data_ptr(),
+            scale_pitch, T, K, _dtype_code(out), _stream(dev))
     return out
 
 
@@ -1024,34 +1030,30 @@ def linear_mxfp4(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scal
     with ``quantized`` the pair ``quant_mxfp4`` would give of the float32 results.
     ``out`` is aligned to 16 bytes (float32), 8 (16 bits) or, each of its rows, 16 (4 bits)."""
     dev = _need_cuda(x, x_scale, w, w_scale, out, out_scale)
-    K = _mx_rows("x", x, x_scale)
-    T, rows = x.shape[0], w.shape[0]
-    if _mx_rows("w", w, w_scale) != K or (swiglu and rows % 2):
+    T, K, x_pitch, xs_pitch = _mx_rows("x", x, x_scale)
+    N, w_features, w_pitch, ws_pitch = _mx_rows("w", w, w_scale)
+    if w_features != K or (swiglu and N % 2):
         raise ValueError("w must be [out_features, in_features / 2] (twice the rows with swiglu)")
-    N = rows // 2 if swiglu else rows
+    if swiglu:
+        N //= 2
     if quantized:
         if N % MXFP4_BLOCK:
             raise ValueError("a quantized result needs a multiple of 32 columns")
-        new = _mx_new(T, N, dev) if out is None or out_scale is None else (None, None)
-        out = new[0] if out is None else out
-        out_scale = new[1] if out_scale is None else out_scale
-        if _mx_rows("out", out, out_scale) != N or out.shape[0] != T:
-            raise ValueError("out must be a [tokens, out_features / 2] tensor")
-        pitch, odt = _row_stride(out, T, N // 2), _C.GR_DTYPE_MXFP4
+        out, out_scale, pitch, os_pitch = _mx_out(out, out_scale, T, N, dev)
+        odt, os_at = _C.GR_DTYPE_MXFP4, out_scale.data_ptr()
     else:
         if out_scale is not None:
             raise ValueError("out_scale goes with quantized=True")
         if out is None:
-            out = torch.empty((T, N), dtype=out_dtype, device=dev)
+            out, pitch = torch.empty((T, N), dtype=out_dtype, device=dev), N
         else:
             _rows("out", out)
             if out.shape != (T, N) or out.dtype != out_dtype:
                 raise ValueError("out must be [tokens, out_features] of the result's type")
-        pitch, odt = _row_stride(out, T, N), _dtype_code(out)
-    _launch(dev, "gr_linear_mxfp4", out.data_ptr(), pitch, _ptr(out_scale),
-            _row_stride(out_scale, T, N // MXFP4_BLOCK) if quantized else 0, x.data_ptr(), _row_stride(x, T, K // 2),
-            x_scale.data_ptr(), _row_stride(x_scale, T, K // MXFP4_BLOCK), w.data_ptr(), _row_stride(w, rows, K // 2),
-            w_scale.data_ptr(), _row_stride(w_scale, rows, K // MXFP4_BLOCK), T, N, K, int(swiglu), odt, _stream(dev))
+            pitch = _row_stride(out, T, N)
+        odt, os_at, os_pitch = _dtype_code(out), None, 0
+    _launch(dev, "gr_linear_mxfp4", out.data_ptr(), pitch, os_at, os_pitch, x.data_ptr(), x_pitch, x_scale.data_ptr(),
+            xs_pitch, w.data_ptr(), w_pitch, w_scale.data_ptr(), ws_pitch, T, N, K, 1 if swiglu else 0, odt, _stream(dev))
     return (out, out_scale) if quantized else out
 
 

@@ -144,19 +144,43 @@ def quantize_blocks(w: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     return x.to(torch.float8_e4m3fn).contiguous(), scale.contiguous()
 
 
+def quantize_mxfp4(w: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """``w [..., N, K]`` in 4 bits as ops.quant_mxfp4 makes them, two codes a byte
+    ``[..., N, K / 2]`` and a scale byte for each 32 of a row ``[..., N, K / 32]``, both
+    uint8; on any device.  ``K`` is a multiple of 32, and ``w`` finite."""
+    if w.shape[-1] % ops.MXFP4_BLOCK:
+        raise ValueError(f"4-bit weights need a multiple of 32 features, not {list(w.shape)}")
+    x = w.double().unflatten(-1, (-1, ops.MXFP4_BLOCK))
+    top = x.abs().amax(-1)
+    half, power = torch.frexp(top)  # half in [0.5, 1) times 2^power
+    # the least power of two with top < 7 times it: from 1.75 times one on the next
+    e = torch.where(top > 0, power - 3 + (half >= 0.875).int(), -127).clamp(-127, 127)
+    x = x * ((1023 - e).long() << 52).view(torch.float64)[..., None]  # 2^-e by its bits
+    a = x.abs()
+    # e2m1 numbers lie 0.5 apart up to 2, 1 up to 4 and then 2: their codes count them from 0, 2 and 4 on
+    code = torch.where(a < 2, (2 * a).round(), torch.where(a < 4, a.round() + 2, (a / 2).round() + 4)).clamp_max(7)
+    code = (code + 8 * torch.signbit(x)).to(torch.uint8).flatten(-2)
+    return code[..., 0::2] | code[..., 1::2] << 4, (e + 127).to(torch.uint8)
+
+
 _QUANTIZED = ("qkv", "o", "gate_up", "down", "expert_gate_up", "expert_down")
 
 
-def quantize_weights(weights: dict[str, torch.Tensor]) -> dict[str, torch.Tensor]:
-    """A decoder's weights with every layer's projections and experts in e4m3 and
-    their scales beside them (``<name>_scale``); gate and up are scaled apart.
+def quantize_weights(weights: dict[str, torch.Tensor], quantization: str = "fp8") -> dict[str, torch.Tensor]:
+    """A decoder's weights with every layer's projections and experts in 8 or 4 bits
+    and their scales beside them (``<name>_scale``): ``"fp8"``, e4m3 in blocks of 128 x
+    128 with gate and up scaled apart, or ``"mxfp4"``, e2m1 in blocks of 32 of a row.
     Embedding, lm_head, norms and router stay as they are, and so does what has its
     scales already."""
+    if quantization not in ("fp8", "mxfp4"):
+        raise ValueError("quantization must be 'fp8' or 'mxfp4'")
     out = {}
     for name, w in weights.items():
         kind = name.rsplit(".", 1)[-1]
         if not name.startswith("layers.") or kind not in _QUANTIZED or name + "_scale" in weights:
             out[name] = w
+        elif quantization == "mxfp4":
+            out[name], out[name + "_scale"] = quantize_mxfp4(w)
         elif kind.endswith("gate_up"):
             w8, scale = quantize_blocks(w.unflatten(-2, (2, w.shape[-2] // 2)))
             out[name], out[name + "_scale"] = w8.flatten(-3, -2), scale.flatten(-3, -2).contiguous()
@@ -257,26 +281,33 @@ def _check_experts(cfg: DecoderConfig) -> None:
 
 
 def _check_quantized(cfg: DecoderConfig, weights: dict[str, torch.Tensor]) -> None:
-    """Refuses 8-bit weights that the products would refuse in the first forward."""
+    """Refuses 8- and 4-bit weights that the products would refuse in the first forward."""
     names = ("expert_gate_up", "expert_down") if cfg.num_experts else ("gate_up", "down")
     for i in range(cfg.num_layers):
         p = f"layers.{i}."
         for name in (p + "qkv", p + "o", p + names[0], p + names[1]):
             w, scale = weights.get(name), weights.get(name + "_scale")
-            if w is None or (scale is None and w.dtype != torch.float8_e4m3fn):
+            if w is None or (scale is None and w.dtype not in (torch.float8_e4m3fn, torch.uint8)):
                 continue
-            if scale is None or w.dtype != torch.float8_e4m3fn:
-                raise ValueError(f"{name}: float8_e4m3fn weights and {name}_scale go together")
+            if scale is None or w.dtype not in (torch.float8_e4m3fn, torch.uint8):
+                raise ValueError(f"{name}: float8_e4m3fn or uint8 weights and {name}_scale go together")
+            four = w.dtype == torch.uint8
             parts = 2 if name.endswith("gate_up") else 1  # gate's rows, then up's
-            N, K = w.shape[-2] // parts, w.shape[-1]
-            if K % 16 or w.shape[-2] % parts or (parts == 2 and N % 16):
-                raise ValueError(f"{name}: 8-bit weights need sizes in multiples of 16, not {list(w.shape)}")
-            blocks = [-(-n // ops.FP8_BLOCK) for n in (N, K)]
-            shape = (*w.shape[:-2], parts * blocks[0], blocks[1])
-            if scale.shape != shape or scale.dtype != torch.float32 or not scale.is_contiguous():
-                raise ValueError(f"{name}_scale must be a contiguous float32 {list(shape)} tensor")
-        if (p + names[0] + "_scale" in weights) != (p + names[1] + "_scale" in weights):
-            raise ValueError(f"{p}{names[0]} and {p}{names[1]} are 8-bit together or not at all")
+            N, K = w.shape[-2] // parts, w.shape[-1] * (2 if four else 1)
+            each = ops.MXFP4_BLOCK if four else 16
+            if K % each or w.shape[-2] % parts or (parts == 2 and N % each):
+                raise ValueError(f"{name}: {4 if four else 8}-bit weights need sizes in multiples of {each}, not "
+                                 f"{[*w.shape[:-1], K]}")
+            if four:
+                shape, dtype = (*w.shape[:-1], K // ops.MXFP4_BLOCK), torch.uint8
+            else:
+                blocks = [-(-n // ops.FP8_BLOCK) for n in (N, K)]
+                shape, dtype = (*w.shape[:-2], parts * blocks[0], blocks[1]), torch.float32
+            if scale.shape != shape or scale.dtype != dtype or not scale.is_contiguous():
+                raise ValueError(f"{name}_scale must be a contiguous {dtype} {list(shape)} tensor")
+        types = {weights[p + n].dtype for n in names if p + n + "_scale" in weights}
+        if len(types) > 1 or (p + names[0] + "_scale" in weights) != (p + names[1] + "_scale" in weights):
+            raise ValueError(f"{p}{names[0]} and {p}{names[1]} are 8-bit together, 4-bit together or neither")
 
 
 class SidDecoder:
@@ -312,6 +343,8 @@ class SidDecoder:
         w, scale = self.w[name], self.w.get(name + "_scale")
         if scale is None:
             return _linear(x, w)
+        if w.dtype == torch.uint8:
+            return ops.linear_mxfp4(*ops.quant_mxfp4(x), w, scale, out_dtype=x.dtype)
         return ops.linear_fp8(*ops.quant_fp8(x), w, scale, out_dtype=x.dtype)
 
     def _mlp(self, x: torch.Tensor, p: str) -> torch.Tensor:
@@ -325,12 +358,18 @@ class SidDecoder:
                 logits, cfg.experts_per_token, score=cfg.router_score, bias=w.get(p + "router_bias"),
                 num_groups=cfg.router_groups, top_groups=cfg.router_top_groups,
                 renormalize=cfg.router_renormalize, scale=cfg.router_scale)
+            if w[p + "expert_gate_up"].dtype == torch.uint8:
+                return ops.expert_mlp_mxfp4(x, w[p + "expert_gate_up"], w[p + "expert_gate_up_scale"], w[p + "expert_down"],
+                                            w[p + "expert_down_scale"], weights, ids)
             return ops.expert_mlp(x, w[p + "expert_gate_up"], w[p + "expert_down"], weights, ids,
                                   gate_up_scale=w.get(p + "expert_gate_up_scale"),
                                   down_scale=w.get(p + "expert_down_scale"))
         scale = w.get(p + "gate_up_scale")
         if scale is None:
             return _linear(_swiglu(x, w[p + "gate_up"]), w[p + "down"])
+        if w[p + "gate_up"].dtype == torch.uint8:
+            act = ops.linear_mxfp4(*ops.quant_mxfp4(x), w[p + "gate_up"], scale, swiglu=True, quantized=True)
+            return ops.linear_mxfp4(*act, w[p + "down"], w[p + "down_scale"], out_dtype=x.dtype)
         act = ops.linear_fp8(*ops.quant_fp8(x), w[p + "gate_up"], scale, swiglu=True, quantized=True)
         return ops.linear_fp8(*act, w[p + "down"], w[p + "down_scale"], out_dtype=x.dtype)
 

@@ -75,7 +75,8 @@ def check(got, y, err):
 
 
 # tokens: one, a few rows an expert, tiles of every size, more choices than one workgroup sorts
-CASES = [(1, 1, 1, 32, 32), (1, 8, 2, 256, 128), (3, 4, 4, 96, 160), (8, 64, 8, 2048, 768), (33, 5, 3, 416, 96),
+CASES = [(1, 1, 1, 32, 32), (1, 8, 2, 256, 128), (3, 4, 4, 96, 160), (8, 64, 8, 2048, 768), (16, 20, 8, 544, 288),
+         (5, 40, 25, 288, 96), (17, 100, 8, 256, 128), (40, 64, 2, 544, 288), (33, 5, 3, 416, 96),
          (100, 8, 2, 544, 288), (257, 6, 4, 512, 256), (640, 4, 2, 288, 352), (1500, 16, 8, 256, 64), (700, 2, 1, 1024, 512)]
 
 
@@ -109,8 +110,25 @@ def test_absent_bad_and_repeated_experts(device):
     assert (ops.expert_mlp_mxfp4(*a) == 0).all()
 
 
-def test_strided_tensors_and_workspace(device):
-    T, E, k, H, F = 40, 4, 2, 160, 96
+def test_few_tokens_absent_bad_and_repeated_experts(device):
+    """The same for 16 tokens: more rows of one expert than a fragment holds among them."""
+    T, E, k, H, F = 16, 5, 8, 288, 96
+    a, gu, dn, x, w, ids = make(T, E + 3, k, H, F, torch.float16, device, seed=6, away=0.3)
+    ids[0] = -1
+    ids[1] = torch.tensor([2, 2, 4, 0, -1, E + 3, 2 ** 31 - 1, 1], dtype=torch.int32)
+    for choices in (ids, torch.full_like(ids, 3), torch.full_like(ids, -7)):
+        a[6] = choices.to(device)
+        status = torch.zeros(1, dtype=torch.int32, device=device)
+        y, err = reference(x, gu, dn, w, torch.where(choices >= E + 3, -1, choices))
+        got = ops.expert_mlp_mxfp4(*a, status=status)
+        check(got, y, err)
+        assert status.item() == (_C.GR_DEV_BAD_EXPERT if choices is ids else 0)
+    assert (got == 0).all()
+
+
+@pytest.mark.parametrize("T", [9, 40])
+def test_strided_tensors_and_workspace(device, T):
+    E, k, H, F = 4, 2, 160, 96
     a, gu, dn, x, w, ids = make(T, E, k, H, F, torch.float16, device)
     y, err = reference(x, gu, dn, w, ids)
     wide = torch.zeros(T, H + 24, dtype=torch.float16, device=device)

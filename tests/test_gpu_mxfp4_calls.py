@@ -24,10 +24,11 @@ def random_rows(g, rows, K, device):
     return x4, s, v * POWERS.to(device)[s.long()].repeat_interleave(32, -1)
 
 
-# from a few rows over tiles of 64 x 64, 64 x 128, 128 x 128 and 128 x 256 to 256 x 256, rows
+# from a few rows over tiles of 64 x 64 to 256 x 256, rows
 # and columns left over
 @pytest.mark.parametrize("M,N,K", [(8, 8192, 6144), (20, 4000, 160), (64, 4096, 2048), (200, 2000, 96), (511, 8184, 2048),
-                                   (1001, 2048, 6144), (512, 12280, 2048), (2047, 12300, 288), (8190, 12280, 512)])
+                                   (1001, 2048, 6144), (512, 12280, 2048), (2047, 12300, 288), (8190, 12280, 512),
+                                   (4090, 8190, 1056)])
 def test_large_tiles(device, M, N, K):
     g = torch.Generator(device=device).manual_seed(M + N + K)
     x4, xs, x = random_rows(g, M, K, device)
@@ -40,7 +41,8 @@ def test_large_tiles(device, M, N, K):
         assert (out[M:] == -7).all()
 
 
-@pytest.mark.parametrize("M,N,K", [(20, 2016, 160), (200, 1024, 96), (511, 4096, 544), (520, 6144, 2048), (4100, 6112, 96)])
+@pytest.mark.parametrize("M,N,K", [(20, 2016, 160), (200, 1024, 96), (511, 4096, 544), (520, 6144, 2048), (4100, 6112, 96),
+                                   (4100, 2080, 1056)])
 def test_large_gated_tiles(device, M, N, K):
     g = torch.Generator(device=device).manual_seed(M + N + K)
     x4, xs, x = random_rows(g, M, K, device)

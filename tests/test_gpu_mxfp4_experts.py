@@ -77,7 +77,7 @@ def check(got, y, err):
 # tokens: one, a few rows an expert, tiles of every size, more choices than one workgroup sorts
 CASES = [(1, 1, 1, 32, 32), (1, 8, 2, 256, 128), (3, 4, 4, 96, 160), (8, 64, 8, 2048, 768), (16, 20, 8, 544, 288),
          (5, 40, 25, 288, 96), (17, 100, 8, 256, 128), (40, 64, 2, 544, 288), (33, 5, 3, 416, 96),
-         (100, 8, 2, 544, 288), (257, 6, 4, 512, 256), (640, 4, 2, 288, 352), (1500, 16, 8, 256, 64), (700, 2, 1, 1024, 512)]
+         (100, 8, 2, 544, 288), (257, 6, 4, 512, 256), (640, 4, 2, 288, 352), (1500, 16, 8, 256, 64), (700, 2, 1, 1024, 512), (16, 60, 8, 2080, 800)]
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])

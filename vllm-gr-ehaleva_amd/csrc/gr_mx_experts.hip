@@ -2,6 +2,7 @@
 // tokens are quantised once, each expert's gated product is written in 4 bits, and its
 // result waits for the sum over a token's experts as scaled fp16.
 #include <algorithm>
+#include <cmath>
 
 #include "gr_expert_rows.h"
 #include "gr_mx_mm.h"
@@ -32,14 +33,13 @@ struct MxWorkspace {
 // Rows of a tile, by the rows an expert gets on average: few rows are bound by the weights'
 // way from memory, many by the products and the results.  Measured (64 experts of 768
 // features, hidden 2048, 8 of them a token; us of both products, by tile rows):
-//   rows an expert    1     2     8    16    32    64   128   256   375   625  1024
-//   16             25.4  31.4  40.3
-//   32                   29.9  35.8  42.5  50.6  59.2  97.5
-//   64                   33.8  41.0  42.3  45.6  53.0  77.5
-//   128                                    55.3  66.2  79.9   115   155   233   346
-//   256                                    70.5  75.8  90.3   119   135   205   303
+//   rows an expert    8    16    28    32    48    64    96   128   192   256   300   375   625  1024
+//    32            33.2  39.8  42.9  50.5  56.2  60.5
+//    64            40.3  42.0  43.3  45.0  46.9  52.7  67.7  84.4   108   136
+//   128                                          59.9  64.2  76.9  94.0   111   136   159   242   357
+//   256                                                      93.7   101   123   136   141   212   312
 int mx_tile_rows(int64_t rows, int E) {
-  return 2 * rows <= 3ll * E ? 16 : rows <= 20ll * E ? 32 : rows <= 144ll * E ? 64 : rows <= 300ll * E ? 128 : 256;
+  return rows <= 28ll * E ? 32 : rows <= 88ll * E ? 64 : rows <= 300ll * E ? 128 : 256;
 }
 constexpr int MX_WAVE_COLS = 64;  // columns of a wave of the down product, whatever its tiles
 
@@ -66,19 +66,32 @@ MxWorkspace plan_mx_workspace(int T, int k, int E, int H, int F, int bm) {
   return w;
 }
 
-void launch_mx_experts(const MxArgs& up, const MxArgs& down, int tiles, int bm, hipStream_t stream) {
-  if (bm == 16) {
-    launch_mx_few<1, 2, 4, MM_SWIGLU_Q, true>(up, tiles, stream);
-    launch_mx_few<1, 4, 2, MM_PLAIN, true>(down, tiles, stream);
-  } else if (bm == 32) {
-    launch_mx<32, 256, 1, 4, 2, 1, MM_SWIGLU_Q, true>(up, tiles, stream);
-    launch_mx<32, 256, 1, 4, 2, 1, MM_PLAIN, true>(down, tiles, stream);
+void launch_mx_experts(const MxArgs& up, const MxArgs& down, int tiles, int E, int bm, hipStream_t stream) {
+  if (bm == 32) {
+    // Few rows: what counts is that all workgroups of a product are on the CUs at once.  Of the experts, choices
+    // that fall evenly reach `reached`.  Up: 64 results a workgroup, two workgroups a CU with three stages each, or
+    // three with two.  Down: 64 columns, six a CU, or 256, two a CU.  Where all fit in the second form only it is
+    // taken, else the first (64 experts of 768 features, hidden 2048, 8 a token; us):
+    //   tokens                     1     8    12    16    64    80    96   128
+    //   workgroups up             96   492   587   664   768   768   ...
+    //   three stages             7.4  12.6  18.8  20.3  25.2  25.6  25.6  25.9
+    //   two                      9.2  13.1  16.2  17.2  21.0  23.8  28.3  28.5
+    //   down 64                  4.6   8.2   9.9  11.8  13.4  13.3  13.2  13.9
+    //   down 256                 5.7   9.2   9.5  10.0  12.2  13.4  15.4  16.2
+    const double reached = E * (1.0 - std::exp(-(double)up.M / E));
+    const double wgs = reached * ((up.N + 63) / 64), wide = reached * ((down.N + 255) / 256);
+    const bool once = up.M <= 10ll * E;  // (more rows give some experts a second tile)
+    if (once && wgs > 512 && wgs <= 768) launch_mx<32, 128, 2, 2, 2, 2, MM_SWIGLU_Q, true>(up, tiles, stream);
+    else launch_mx<32, 128, 2, 2, 3, 2, MM_SWIGLU_Q, true>(up, tiles, stream);
+    if (once && wide <= 512 && reached * ((down.N + 63) / 64) > 1536)
+      launch_mx<32, 256, 1, 4, 2, 1, MM_PLAIN, true>(down, tiles, stream);
+    else launch_mx<32, 64, 2, 1, 2, 1, MM_PLAIN, true>(down, tiles, stream);
   } else if (bm == 64) {
     launch_mx<64, 128, 2, 2, 3, 2, MM_SWIGLU_Q, true>(up, tiles, stream);
-    launch_mx<64, 128, 4, 2, 3, 2, MM_PLAIN, true>(down, tiles, stream);
+    launch_mx<64, 128, 2, 2, 2, 1, MM_PLAIN, true>(down, tiles, stream);
   } else if (bm == 128) {
     launch_mx<128, 256, 2, 4, 3, 2, MM_SWIGLU_Q, true>(up, tiles, stream);
-    launch_mx<128, 256, 2, 4, 3, 2, MM_PLAIN, true>(down, tiles, stream);
+    launch_mx<128, 128, 4, 2, 2, 1, MM_PLAIN, true>(down, tiles, stream);
   } else {
     launch_mx<256, 256, 2, 4, 2, 2, MM_SWIGLU_Q, true>(up, tiles, stream);
     launch_mx<256, 256, 2, 4, 2, 2, MM_PLAIN, true>(down, tiles, stream);
@@ -118,7 +131,7 @@ extern "C" gr_status_t gr_expert_mlp_mxfp4(void* out, int64_t out_stride, const 
     return GR_ERR_UNSUPPORTED;
   const int bm = mx_tile_rows((int64_t)T * top_k, num_experts);
   const MxWorkspace l = plan_mx_workspace(T, top_k, num_experts, H, F, bm);
-  const int cols = bm == 16 ? 32 : bm == 64 ? 64 : 128;  // results of a workgroup, in the narrower product
+  const int cols = bm <= 64 ? 64 : 128;  // results of a workgroup, in the narrower product
   if (l.max_tiles * ((std::max(F, H) + cols - 1) / cols) > GRID_MAX - 8 || T > GRID_MAX) return GR_ERR_UNSUPPORTED;
   if (!workspace || !aligned(workspace, 256) || workspace_bytes < (size_t)l.bytes) return GR_ERR_WORKSPACE;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
@@ -187,7 +200,7 @@ extern "C" gr_status_t gr_expert_mlp_mxfp4(void* out, int64_t out_stride, const 
   dn.num_tiles = p.num_tiles;
   dn.slot = p.slot;
   dn.scatter = 1;
-  launch_mx_experts(up, dn, (int)l.max_tiles, bm, stream);
+  launch_mx_experts(up, dn, (int)l.max_tiles, num_experts, bm, stream);
 
   const CombineArgs c{out, out_stride, ws + l.y, dn.out_exp, MX_WAVE_COLS, weights, ids, T, top_k, num_experts, H};
   const dim3 grid((unsigned)T, (unsigned)((H + 2047) / 2048));

@@ -96,8 +96,10 @@ struct Mx {
     for (int i = 0; i < LPS; ++i) {
       const int r8 = 8 * (wave + NW * i), row = r8 + (lane >> 3);
       if (8 * NW * i < BM) {
+        // (rows behind an expert's last: zeros, that nothing is read for)
         s.rows.buf[i] = xb;
-        s.rows.off[i] = (uint32_t)((M::x_row(a, t, row) - first) * (uint32_t)a.x_stride) + s.rows.ch;
+        s.rows.off[i] = EXPERTS && t.m0 + row >= t.m_end ? MM_NOWHERE
+                                                         : (uint32_t)((M::x_row(a, t, row) - first) * (uint32_t)a.x_stride) + s.rows.ch;
       } else {
         const int b = row - BM;
         const bool up = GATED && ((r8 - BM) >> 4 & 1);
@@ -310,40 +312,31 @@ __global__ __launch_bounds__(64 * WM * WN, (MxLds<BM, BN, WM, WN, ST, CH, MODE, 
   }
 }
 
-// Few rows: BM = 16 FM, 16 NF columns.  Bound by the weights' way from memory, or by one
-// round trip: each weight is loaded once, by the wave that multiplies it, into the
-// registers of the operand, and the WK waves split the depth (wave k takes stages k,
-// k + WK, ...).  Their partial sums meet in LDS.  The rows are read by every workgroup,
-// from L2.
-template <int FM, int NF, int WK, int MODE, bool EXPERTS>
-__global__ __launch_bounds__(64 * WK) void mx_few(MxArgs a) {
+// 16 rows, 16 NF columns.  Bound by the weights' way from memory, or by one round trip:
+// each weight is loaded once, by the wave that multiplies it, into the registers of the
+// operand, and the WK waves split the depth (wave k takes stages k, k + WK, ...).  Their
+// partial sums meet in LDS.  The rows are read by every workgroup, from L2.
+template <int NF, int WK, int MODE> __global__ __launch_bounds__(64 * WK) void mx_few(MxArgs a) {
   constexpr bool GATED = MODE == MM_SWIGLU || MODE == MM_SWIGLU_Q, QUANT = MODE == MM_SWIGLU_Q || MODE == MM_PLAIN_Q;
-  constexpr int FN = NF * (GATED ? 2 : 1), U = FM * FN <= 2 ? 4 : 2;
-  using M = Mm<GR_DTYPE_BF16, 16 * FM, 16 * FN, 1, 1, GATED ? MM_SWIGLU : MM_PLAIN, EXPERTS, false>;
-  using M1 = Mm<GR_DTYPE_BF16, 16, 16 * FN, 1, 1, GATED ? MM_SWIGLU : MM_PLAIN, EXPERTS, false>;  // one fragment row
-  static_assert(FM <= WK && (!QUANT || NF == 2), "a wave finishes a fragment row; a block of the result is 32 columns");
-  constexpr int PART = WK * FM * FN * 1024, ROOM = 16 * (16 * NF * 4 + 16);
-  __shared__ __attribute__((aligned(16))) uint8_t lds[PART + (QUANT ? 0 : FM * ROOM)];
+  constexpr int FN = NF * (GATED ? 2 : 1), U = FN <= 2 ? 4 : 2;
+  using M = Mm<GR_DTYPE_BF16, 16, 16 * FN, 1, 1, GATED ? MM_SWIGLU : MM_PLAIN, false, false>;
+  static_assert(!QUANT || NF == 2, "a block of the result is 32 columns");
+  constexpr int PART = WK * FN * 1024, ROOM = 16 * (16 * NF * 4 + 16);
+  __shared__ __attribute__((aligned(16))) uint8_t lds[PART + (QUANT ? 0 : ROOM)];
   MmTile t;
   if (!M::tile(a, t)) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r16 = lane & 15, q = lane >> 4;
   const int n = (a.kbytes + 127) >> 7;
-  const uint8_t *w0[FN], *ws[FN], *x0[FM], *xs[FM];
-  const uint8_t* ws4 = a.ws4;
-  if constexpr (EXPERTS) ws4 += __builtin_amdgcn_readfirstlane(a.tiles[t.mt].x) * a.ws4_expert;
+  const uint8_t *w0[FN], *ws[FN];
 #pragma unroll
   for (int i = 0; i < FN; ++i) {
     const int64_t r = min(t.n0 + 16 * (GATED ? i >> 1 : i) + r16, a.N - 1) + (GATED && (i & 1) ? a.N : 0);
     w0[i] = t.w + r * a.w_stride + q * 32;
-    ws[i] = ws4 + r * a.ws4_row + q * 2;
+    ws[i] = a.ws4 + r * a.ws4_row + q * 2;
   }
-#pragma unroll
-  for (int j = 0; j < FM; ++j) {
-    const int64_t r = M::x_row(a, t, 16 * j + r16);
-    x0[j] = a.x + r * a.x_stride + q * 32;
-    xs[j] = a.xs4 + r * a.xs4_row + q * 2;
-  }
+  const int64_t xr = M::x_row(a, t, r16);
+  const uint8_t *x0 = a.x + xr * a.x_stride + q * 32, *xs = a.xs4 + xr * a.xs4_row + q * 2;
   struct Piece {
     mm4i_t v[2];
     int s;
@@ -365,64 +358,50 @@ __global__ __launch_bounds__(64 * WK) void mx_few(MxArgs a) {
   };
   typename M::Acc acc;
 #pragma unroll
-  for (int i = 0; i < FN; ++i)
-#pragma unroll
-    for (int j = 0; j < FM; ++j) acc[i][j] = mm4_t{0.f, 0.f, 0.f, 0.f};
+  for (int i = 0; i < FN; ++i) acc[i][0] = mm4_t{0.f, 0.f, 0.f, 0.f};
   for (int s0 = wave; s0 < n; s0 += WK * U) {
-    Piece w[U][FN], x[U][FM];
+    Piece w[U][FN], x[U];
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int i = 0; i < FN; ++i) w[u][i] = load(w0[i], ws[i], s0 + u * WK);
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int j = 0; j < FM; ++j) x[u][j] = load(x0[j], xs[j], s0 + u * WK);
+    for (int u = 0; u < U; ++u) x[u] = load(x0, xs, s0 + u * WK);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (u && s0 + u * WK >= n) break;
 #pragma unroll
-      for (int j = 0; j < FM; ++j)
-#pragma unroll
-        for (int i = 0; i < FN; ++i) {
-          acc[i][j] = mx_mma<0>(w[u][i].v[0], w[u][i].s, x[u][j].v[0], x[u][j].s, acc[i][j]);
-          acc[i][j] = mx_mma<1>(w[u][i].v[1], w[u][i].s, x[u][j].v[1], x[u][j].s, acc[i][j]);
-        }
-    }
-  }
-  mm4_t* part = reinterpret_cast<mm4_t*>(lds);  // [wave][FM][FN][64]
-#pragma unroll
-  for (int j = 0; j < FM; ++j)
-#pragma unroll
-    for (int i = 0; i < FN; ++i) part[((wave * FM + j) * FN + i) * 64 + lane] = acc[i][j];
-  __syncthreads();
-  if (const int j = wave; j < FM) {
-    typename M1::Acc sum;
-#pragma unroll
-    for (int i = 0; i < FN; ++i) {
-      sum[i][0] = part[(j * FN + i) * 64 + lane];
-#pragma unroll
-      for (int k = 1; k < WK; ++k) {
-        const mm4_t v = part[((k * FM + j) * FN + i) * 64 + lane];
-#pragma unroll
-        for (int u = 0; u < 4; ++u) sum[i][0][u] += v[u];
+      for (int i = 0; i < FN; ++i) {
+        acc[i][0] = mx_mma<0>(w[u][i].v[0], w[u][i].s, x[u].v[0], x[u].s, acc[i][0]);
+        acc[i][0] = mx_mma<1>(w[u][i].v[1], w[u][i].s, x[u].v[1], x[u].s, acc[i][0]);
       }
     }
-    MmTile tj = t;
-    tj.m0 += 16 * j;
-    if (tj.m0 >= tj.m_end) return;
+  }
+  mm4_t* part = reinterpret_cast<mm4_t*>(lds);  // [wave][FN][64]
+#pragma unroll
+  for (int i = 0; i < FN; ++i) part[(wave * FN + i) * 64 + lane] = acc[i][0];
+  __syncthreads();
+  if (wave == 0) {
+#pragma unroll
+    for (int i = 0; i < FN; ++i)
+#pragma unroll
+      for (int k = 1; k < WK; ++k) {
+        const mm4_t v = part[(k * FN + i) * 64 + lane];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) acc[i][0][u] += v[u];
+      }
     if constexpr (QUANT) {
       uint32_t codes;
-      const uint32_t s = mx_block<M1>(sum, 0, 0, codes);
-      if (tj.m0 + r16 < tj.m_end) {
-        const int64_t row = M1::out_row(a, tj, r16);
+      const uint32_t s = mx_block<M>(acc, 0, 0, codes);
+      if (t.m0 + r16 < t.m_end) {
+        const int64_t row = M::out_row(a, t, r16);
         uint16_t* o = reinterpret_cast<uint16_t*>(static_cast<uint8_t*>(a.out) + row * a.out_stride + t.n0 / 2) + q;
         o[0] = (uint16_t)codes;
         o[4] = (uint16_t)(codes >> 16);
         if (q == 0) a.os4[row * a.os4_row + t.n0 / 32] = (uint8_t)s;
       }
     } else {
-      M1::store_any(a, tj, sum, wave, 0, 0, lane, lds + PART);
+      M::store_any(a, t, acc, wave, 0, 0, lane, lds + PART);
     }
   }
 }
@@ -436,12 +415,11 @@ void launch_mx(MxArgs a, int tiles_m, hipStream_t stream) {
   hipLaunchKernelGGL((mx_mm<BM, BN, WM, WN, ST, CH, MODE, EXPERTS>), dim3((unsigned)((total + 7) / 8 * 8)), dim3(64 * WM * WN),
                      0, stream, a);
 }
-template <int FM, int NF, int WK, int MODE, bool EXPERTS>
-void launch_mx_few(MxArgs a, int tiles_m, hipStream_t stream) {
-  a.tiles_m = tiles_m;
+template <int NF, int WK, int MODE> void launch_mx_few(MxArgs a, hipStream_t stream) {
+  a.tiles_m = (a.M + 15) / 16;
   a.tiles_n = (a.N + 16 * NF - 1) / (16 * NF);
-  const int64_t total = (int64_t)tiles_m * a.tiles_n;
-  hipLaunchKernelGGL((mx_few<FM, NF, WK, MODE, EXPERTS>), dim3((unsigned)((total + 7) / 8 * 8)), dim3(64 * WK), 0, stream, a);
+  const int64_t total = (int64_t)a.tiles_m * a.tiles_n;
+  hipLaunchKernelGGL((mx_few<NF, WK, MODE>), dim3((unsigned)((total + 7) / 8 * 8)), dim3(64 * WK), 0, stream, a);
 }
 
 // ---- rows to 4 bits ------------------------------------------------------------

@@ -72,23 +72,24 @@ template <int DT, int ROWS> __global__ __launch_bounds__(MXQ_THREADS) void mx_de
 // of the XCD that gets the most of them, whose 32 CUs take one or two each, a round costs
 // a fixed part and its stages of 256 features, `one` ns each alone on a CU, `two` with a
 // neighbour.  Fitted to 250 measured sizes of 48 to 8192 rows, 512 to 12288 weight rows
-// and 512 to 6144 features: the pick is 0.8 % slower than the best tile in the mean and
-// 10 % at most.  (us; rows x weight rows x features, the picked tile's and the next one's)
-//   64 x 4096 x 2048     64 x 64     5.1,   64 x 128   6.4
-//   1001 x 2048 x 6144   64 x 64    15.3,   64 x 128  15.5
-//   512 x 8192 x 2048   128 x 128    9.7,   64 x 128  10.3
-//   2048 x 2048 x 6144  128 x 128   19.3,   64 x 128  23.8
-//   512 x 12288 x 2048  128 x 256   13.0,  128 x 128  15.1
-//   8192 x 12288 x 2048 256 x 256    134,  128 x 256   178
+// and 512 to 6144 features: the pick is 1.1 % slower than the best tile in the mean, more
+// than 10 % in 3 of 100.  (us; rows x weight rows x features, the picked tile's and the next one's)
+//   64 x 4096 x 2048     64 x 64     5.1,   64 x 128          6.4
+//   1001 x 2048 x 6144   64 x 64    15.3,   64 x 128         15.5
+//   512 x 8192 x 2048   128 x 128    9.7,   64 x 128         10.3
+//   2048 x 2048 x 6144  128 x 128   19.3,   64 x 128         23.8
+//   8192 x 12288 x 512  128 x 128 of two stages, two a CU: 57 (in 4 bits), 256 x 256  63
+//   512 x 12288 x 2048  128 x 256   13.0,  128 x 128         15.1
+//   8192 x 12288 x 2048 256 x 256    134,  128 x 256          178
 struct MxChoice { int bm, bn, per_cu, launch, fixed1, one, fixed2, two; };
-constexpr MxChoice kMx[] = {{64, 64, 2, 1920, 900, 307, 1530, 443}, {64, 128, 2, 2000, 1270, 449, 1890, 758},
-                            {128, 128, 1, 480, 3040, 591, 0, 0}, {128, 256, 1, -640, 4980, 908, 0, 0},
-                            {256, 256, 1, -3560, 9140, 1435, 0, 0}};
+constexpr MxChoice kMx[] = {{64, 64, 2, 1800, 1010, 308, 1520, 462},   {64, 128, 2, 1960, 1330, 471, 1960, 747},
+                            {128, 128, 1, 840, 2840, 626, 0, 0},        {128, 128, 2, 1960, 820, 873, 2510, 1268},
+                            {128, 256, 1, 430, 4240, 1017, 0, 0},       {256, 256, 1, -1200, 7990, 1657, 0, 0}};
 
 int pick_mx(int M, int rows_w, int stages, bool quant) {
   int best = -1;
   int64_t least = 0;
-  for (int i = quant ? 1 : 0; i < 5; ++i) {  // (a wave of a 64 x 64 tile has 16 gated results of a row, half a block)
+  for (int i = quant ? 1 : 0; i < 6; ++i) {  // (a wave of a 64 x 64 tile has 16 gated results of a row, half a block)
     const MxChoice& c = kMx[i];
     const int64_t tiles = ((int64_t)((M + c.bm - 1) / c.bm) * ((rows_w + c.bn - 1) / c.bn) + 7) / 8;
     const int64_t one = c.fixed1 + (int64_t)stages * c.one, two = c.per_cu == 2 ? c.fixed2 + (int64_t)stages * c.two : one;
@@ -109,16 +110,17 @@ template <int MODE> void launch_linear_mx(const MxArgs& a, hipStream_t stream) {
   // 6144 8.5 us in 32 columns a workgroup, 9.5 in 16 (64 x 64 tiles 9.9; 32 x 8192 x 2048, twice that many, 7.4 and 5.2)
   const int64_t few = (int64_t)((M + 15) / 16) * ((a.N + 15) / 16);
   if constexpr (!QUANT) {
-    if (few <= 256) return launch_mx_few<1, 1, 8, MODE, false>(a, (M + 15) / 16, stream);
+    if (few <= 256) return launch_mx_few<1, 8, MODE>(a, stream);
   }
-  if (few <= 512) return launch_mx_few<1, 2, 8, MODE, false>(a, (M + 15) / 16, stream);
+  if (few <= 512) return launch_mx_few<2, 8, MODE>(a, stream);
   switch (pick_mx(M, rows_w, (a.kbytes + 127) / 128, QUANT)) {
     case 0:
       if constexpr (!QUANT) launch_mx<64, 64, 2, 2, 4, 4, MODE, false>(a, (M + 63) / 64, stream);
       break;
     case 1: launch_mx<64, 128, 2, 2, 3, 2, MODE, false>(a, (M + 63) / 64, stream); break;
     case 2: launch_mx<128, 128, 4, 2, 3, 4, MODE, false>(a, (M + 127) / 128, stream); break;
-    case 3: launch_mx<128, 256, 2, 4, 3, 2, MODE, false>(a, (M + 127) / 128, stream); break;
+    case 3: launch_mx<128, 128, 4, 2, 2, 1, MODE, false>(a, (M + 127) / 128, stream); break;
+    case 4: launch_mx<128, 256, 2, 4, 3, 2, MODE, false>(a, (M + 127) / 128, stream); break;
     default: launch_mx<256, 256, 2, 4, 2, 2, MODE, false>(a, (M + 255) / 256, stream);
   }
 }

@@ -20,7 +20,7 @@ def _rows(ins):
 
 
 def _scales(ins):
-    return ins.startswith("global_load_lds_dword ")
+    return ins.startswith(("global_load_lds_dword ", "global_load_lds_dwordx4 "))
 
 
 def _late(code):

@@ -33,13 +33,13 @@ struct MxWorkspace {
 // Rows of a tile, by the rows an expert gets on average: few rows are bound by the weights'
 // way from memory, many by the products and the results.  Measured (64 experts of 768
 // features, hidden 2048, 8 of them a token; us of both products, by tile rows):
-//   rows an expert    8    16    28    32    48    64    96   128   192   256   300   375   625  1024
-//    32            33.2  39.8  42.9  50.5  56.2  60.5
-//    64            40.3  42.0  43.3  45.0  46.9  52.7  67.7  84.4   108   136
-//   128                                          59.9  64.2  76.9  94.0   111   136   159   242   357
-//   256                                                      93.7   101   123   136   141   212   312
+//   rows an expert    8    16    24    28    32    48    64    80    96   128   192   224   256   300   375   625
+//    32            33.3  40.0  40.5  43.4  45.7  51.1
+//    64            39.8  42.0  42.9  43.3  43.5  45.6  51.8  59.8  64.3  79.8
+//   128                                    48.6  51.9  54.3  56.1  57.6  74.4  94.1   107   113   131   155   233
+//   256                                                                  87.2  95.3   111   114   126   131   199
 int mx_tile_rows(int64_t rows, int E) {
-  return rows <= 28ll * E ? 32 : rows <= 88ll * E ? 64 : rows <= 300ll * E ? 128 : 256;
+  return rows <= 28ll * E ? 32 : rows <= 72ll * E ? 64 : rows <= 260ll * E ? 128 : 256;
 }
 constexpr int MX_WAVE_COLS = 64;  // columns of a wave of the down product, whatever its tiles
 
@@ -73,11 +73,11 @@ void launch_mx_experts(const MxArgs& up, const MxArgs& down, int tiles, int E, i
     // three with two.  Down: 64 columns, six a CU, or 256, two a CU.  Where all fit in the second form only it is
     // taken, else the first (64 experts of 768 features, hidden 2048, 8 a token; us):
     //   tokens                     1     8    12    16    64    80    96   128
-    //   workgroups up             96   492   587   664   768   768   ...
-    //   three stages             7.4  12.6  18.8  20.3  25.2  25.6  25.6  25.9
-    //   two                      9.2  13.1  16.2  17.2  21.0  23.8  28.3  28.5
-    //   down 64                  4.6   8.2   9.9  11.8  13.4  13.3  13.2  13.9
-    //   down 256                 5.7   9.2   9.5  10.0  12.2  13.4  15.4  16.2
+    //   workgroups up             96   483   619   680   768   768   768   768
+    //   three stages             7.1  12.7  18.5  20.0  25.5  26.5  26.4  26.5
+    //   two                      8.8  12.4  15.3  16.7  21.5  24.1  27.7  28.1
+    //   down 64                  4.6   8.3   9.9  11.9  12.9  13.1  13.2  13.5
+    //   down 256                 5.6   9.1   9.5   9.8  11.8  13.2  15.5  16.0
     const double reached = E * (1.0 - std::exp(-(double)up.M / E));
     const double wgs = reached * ((up.N + 63) / 64), wide = reached * ((down.N + 255) / 256);
     const bool once = up.M <= 10ll * E;  // (more rows give some experts a second tile)
@@ -170,7 +170,7 @@ extern "C" gr_status_t gr_expert_mlp_mxfp4(void* out, int64_t out_stride, const 
   up.N = F;
   up.kbytes = H / 2;
   up.blocks = H / 32;
-  up.loose = up.blocks % 4 != 0 || !aligned(gate_up_scale, 4);
+  up.scale_piece = mx_scale_piece(up);
   up.tiles = p.tiles;
   up.num_tiles = p.num_tiles;
   up.slot = p.slot;
@@ -192,7 +192,7 @@ extern "C" gr_status_t gr_expert_mlp_mxfp4(void* out, int64_t out_stride, const 
   dn.N = H;
   dn.kbytes = F / 2;
   dn.blocks = F / 32;
-  dn.loose = dn.blocks % 4 != 0 || !aligned(down_scale, 4);
+  dn.scale_piece = mx_scale_piece(dn);
   // (up to 2^-11 of each expert's result: half a step of an fp16 output, little beside the 2^-2 of its 4-bit operands)
   dn.out_type = MM_OUT_SCALED;
   dn.out_exp = reinterpret_cast<int8_t*>(ws + l.y_exp);

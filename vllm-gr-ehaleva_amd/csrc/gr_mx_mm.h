@@ -48,8 +48,22 @@ struct MxArgs : MmArgs {  // kbytes: in_features / 2; strides of x and w in byte
   uint8_t* os4;  // *_Q
   int64_t os4_row;
   int blocks;  // of a row: in_features / 32
-  int loose;   // scales are not whole, aligned dwords: blocks or a row's stride % 4 != 0
+  int scale_piece;  // bytes of a row's scales that a lane can take: 16, 4 or 1 (mx_scale_piece)
 };
+// What rows and their strides are whole, aligned multiples of.
+inline int mx_scale_piece(const MxArgs& a) {
+  const uint64_t all = (uint64_t)a.blocks | reinterpret_cast<uint64_t>(a.xs4) | (uint64_t)a.xs4_row |
+                       reinterpret_cast<uint64_t>(a.ws4) | (uint64_t)a.ws4_row;
+  return all % 16 == 0 ? 16 : all % 4 == 0 ? 4 : 1;
+}
+
+// 16 bytes a lane from global memory into LDS: lane i's land at lds + 16 i.
+__device__ __forceinline__ void dma_v4(uint32_t lds, const void* addr) {
+  const uint32_t m = __builtin_amdgcn_readfirstlane(lds);
+  uint32_t save;
+  __asm__ volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, off\n\ts_mov_b32 m0, %0"
+                   : "=&s"(save) : "s"(m), "v"(addr) : "memory");
+}
 
 // BM rows by BN weight rows, WM x WN waves (SwiGLU: 16 gate rows and their 16 up rows alternate)
 template <int BM, int BN, int WM, int WN, int CH, int MODE, bool EXPERTS>
@@ -58,9 +72,14 @@ struct Mx {
   static constexpr bool QUANT = MODE == MM_SWIGLU_Q || MODE == MM_PLAIN_Q;
   using M = Mm<GR_DTYPE_BF16, BM, BN, WM, WN, GATED ? MM_SWIGLU : MM_PLAIN, EXPERTS, false>;  // rows of bytes
   static constexpr int NW = WM * WN, ROWS = BM + BN, TILE = M::TILE, LPS = M::LPS, FM = M::FM, FN = M::FN, OC = M::OC;
-  // Scales come CH stages at a time: what a transfer of them costs is its rows' lines,
-  // whatever it takes of each (a dword a lane: 4 CH / 2 lanes a row).
-  static constexpr int LANES = 2 * CH, PER = 64 / LANES, SPS = (ROWS + PER * NW - 1) / (PER * NW), SCALES = NW * SPS * 256;
+  // Scales come CH stages at a time, 16 bytes a lane or (WORDS) 4, as linear rows of 8 CH
+  // bytes: a transfer costs as much as one of rows does, however little it brings (experts
+  // of 5001 tokens, 256 x 256 tiles: up product 114 us by words, 99 us by 16 bytes).
+  static constexpr int LANES = 2 * CH, PER = 64 / LANES, SPS = (ROWS + PER * NW - 1) / (PER * NW);
+  static constexpr bool WIDE = CH >= 2;
+  static constexpr int WIDE_LANES = WIDE ? CH / 2 : 1, WIDE_PER = 64 / WIDE_LANES, WIDE_ALL = (ROWS + WIDE_PER - 1) / WIDE_PER,
+                       WIDE_SPS = (WIDE_ALL + NW - 1) / NW;
+  static constexpr int SCALES = WIDE && WIDE_ALL * 1024 > NW * SPS * 256 ? WIDE_ALL * 1024 : NW * SPS * 256;
   static_assert(BM % (8 * NW) == 0 && BN % (8 * NW) == 0 && NW % 2 == 0, "whole transfers; a wave's rows keep their parity of 8");
   static_assert(!QUANT || OC / WN % 32 == 0, "a block of the result is one wave's");
   using Acc = typename M::Acc;
@@ -69,10 +88,9 @@ struct Mx {
   // fragment reads at once meet no bank twice (5.2 clocks a read of 64 lanes; with the
   // row's low bits alone, or its bits 1 to 3, 8.5).
   __device__ static __forceinline__ int swizzle(int row) { return (row & 7) ^ (row >> 3 & 1); }
-  // The same for the 8 bytes of scales of a stage, of which a row has CH side by side
-  // (u16 reads of 16 rows 16 bytes apart take 4.3 clocks, so 2.8).
+  // The same for a stage's 8 bytes of scales, by 16 bytes.
   static_assert(CH == 1 || CH == 2 || CH == 4, "stages of scales");
-  __device__ static __forceinline__ int scale_swizzle(int row) { return row >> (CH == 4 ? 2 : 3) & (CH - 1); }
+  __device__ static __forceinline__ int scale_swizzle(int row) { return CH == 4 ? row >> 2 & 1 : 0; }
 
   struct Source {
     typename M::Source rows;
@@ -83,8 +101,9 @@ struct Mx {
     if constexpr (GATED) return min(t.n0 + (b >> 5) * 16 + (b & 15), N - 1) + (b >> 4 & 1) * N;
     else return min(t.n0 + b, N - 1);
   }
-  __device__ static __forceinline__ int tile_row(int i, int wave, int lane) {  // of transfer i of scales
-    return (wave * SPS + i) * PER + lane / LANES;
+  __device__ static __forceinline__ bool wide(const MxArgs& a) { return WIDE && a.scale_piece == 16; }
+  __device__ static __forceinline__ int tile_row(bool wide, int i, int wave, int lane) {  // of transfer i of scales
+    return wide ? (wave + NW * i) * WIDE_PER + lane / WIDE_LANES : (wave * SPS + i) * PER + lane / LANES;
   }
   __device__ static __forceinline__ void source(const MxArgs& a, const MmTile& t, int wave, int lane, Source& s) {
     s.rows.ch = ((lane & 7) ^ swizzle(wave * 8 + (lane >> 3))) * 16;
@@ -111,30 +130,43 @@ struct Mx {
     if constexpr (EXPERTS) s.ws += __builtin_amdgcn_readfirstlane(a.tiles[t.mt].x) * a.ws4_expert;
 #pragma unroll
     for (int i = 0; i < SPS; ++i) {
-      const int r = min(tile_row(i, wave, lane), ROWS - 1);
+      const int r = min(tile_row(wide(a), i, wave, lane), ROWS - 1);
       s.scale_row[i] = r < BM ? M::x_row(a, t, r) : w_row(t, r - BM, a.N);
     }
   }
 
   // Scales of stages CH c .. into the buffer at LDS byte `at` of lds.  Past a row's
-  // last block its last four scales stand (a NaN there is the row's anyway); the
+  // last block its last scales stand (a NaN there is the row's anyway); the
   // numbers there are zeros.
   __device__ static __forceinline__ void fetch_scales(const MxArgs& a, const Source& s, int c, uint8_t* lds, int at, int wave,
                                                       int lane) {
+    const uint32_t lds0 = (uint32_t)reinterpret_cast<uintptr_t>(lds);
+    auto row = [&](int i, int r) __attribute__((always_inline)) {
+      return (r < BM ? a.xs4 : s.ws) + s.scale_row[i] * (r < BM ? a.xs4_row : a.ws4_row);
+    };
+    if (wide(a)) {
+#pragma unroll
+      for (int i = 0; i < WIDE_SPS; ++i) {
+        if (wave + NW * i >= WIDE_ALL) break;
+        const int r = tile_row(true, i, wave, lane);
+        const int b0 = 8 * CH * c + 16 * ((lane & (WIDE_LANES - 1)) ^ scale_swizzle(r));
+        dma_v4(lds0 + at + (wave + NW * i) * 1024, row(i, r) + min(b0, a.blocks - 16));
+      }
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < SPS; ++i) {
-      const int r = tile_row(i, wave, lane);
-      const int b0 = 8 * CH * c + 4 * ((lane & (LANES - 1)) ^ 2 * scale_swizzle(r));
-      const bool x = r < BM;
-      const uint8_t* row = (x ? a.xs4 : s.ws) + s.scale_row[i] * (x ? a.xs4_row : a.ws4_row);
+      const int r = tile_row(false, i, wave, lane);
+      const int b0 = 8 * CH * c + 4 * ((lane & (LANES - 1)) ^ 4 * scale_swizzle(r));
+      const uint8_t* p = row(i, r);
       const int to = at + (wave * SPS + i) * 256;
-      if (a.loose) {
+      if (a.scale_piece == 1) {
         uint32_t v = 0;
 #pragma unroll
-        for (int b = 0; b < 4; ++b) v |= (uint32_t)row[min(b0 + b, a.blocks - 1)] << (8 * b);
+        for (int b = 0; b < 4; ++b) v |= (uint32_t)p[min(b0 + b, a.blocks - 1)] << (8 * b);
         *reinterpret_cast<uint32_t*>(lds + to + lane * 4) = v;
       } else {
-        dma_v1((uint32_t)reinterpret_cast<uintptr_t>(lds) + to, row + min(b0, a.blocks - 4));
+        dma_v1(lds0 + to, p + min(b0, a.blocks - 4));
       }
     }
   }
@@ -156,7 +188,7 @@ struct Mx {
     const int xr = wm * (BM / WM) + r16, wr = BM + wn * (BN / WN) + r16;
     l.xo = xr * 128;
     l.wo = wr * 128;
-    l.ssw = scale_swizzle(r16) * 8;
+    l.ssw = scale_swizzle(r16) * 16;
     l.xso = xr * (8 * CH) + 2 * q;
     l.wso = wr * (8 * CH) + 2 * q;
     return l;

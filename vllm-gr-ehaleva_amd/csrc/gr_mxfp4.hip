@@ -82,9 +82,9 @@ template <int DT, int ROWS> __global__ __launch_bounds__(MXQ_THREADS) void mx_de
 //   512 x 12288 x 2048  128 x 256   13.0,  128 x 128         15.1
 //   8192 x 12288 x 2048 256 x 256    134,  128 x 256          178
 struct MxChoice { int bm, bn, per_cu, launch, fixed1, one, fixed2, two; };
-constexpr MxChoice kMx[] = {{64, 64, 2, 1800, 1010, 308, 1520, 462},   {64, 128, 2, 1960, 1330, 471, 1960, 747},
-                            {128, 128, 1, 840, 2840, 626, 0, 0},        {128, 128, 2, 1960, 820, 873, 2510, 1268},
-                            {128, 256, 1, 430, 4240, 1017, 0, 0},       {256, 256, 1, -1200, 7990, 1657, 0, 0}};
+constexpr MxChoice kMx[] = {{64, 64, 2, 1910, 950, 291, 1500, 454},   {64, 128, 2, 2130, 1210, 450, 1910, 728},
+                            {128, 128, 1, 910, 2740, 609, 0, 0},      {128, 128, 2, 2250, 520, 863, 2370, 1196},
+                            {128, 256, 1, 760, 4070, 953, 0, 0},      {256, 256, 1, 200, 6510, 1563, 0, 0}};
 
 int pick_mx(int M, int rows_w, int stages, bool quant) {
   int best = -1;
@@ -118,7 +118,7 @@ template <int MODE> void launch_linear_mx(const MxArgs& a, hipStream_t stream) {
       if constexpr (!QUANT) launch_mx<64, 64, 2, 2, 4, 4, MODE, false>(a, (M + 63) / 64, stream);
       break;
     case 1: launch_mx<64, 128, 2, 2, 3, 2, MODE, false>(a, (M + 63) / 64, stream); break;
-    case 2: launch_mx<128, 128, 4, 2, 3, 4, MODE, false>(a, (M + 127) / 128, stream); break;
+    case 2: launch_mx<128, 128, 4, 2, 3, 2, MODE, false>(a, (M + 127) / 128, stream); break;
     case 3: launch_mx<128, 128, 4, 2, 2, 1, MODE, false>(a, (M + 127) / 128, stream); break;
     case 4: launch_mx<128, 256, 2, 4, 3, 2, MODE, false>(a, (M + 127) / 128, stream); break;
     default: launch_mx<256, 256, 2, 4, 2, 2, MODE, false>(a, (M + 255) / 256, stream);
@@ -211,7 +211,7 @@ extern "C" gr_status_t gr_linear_mxfp4(void* out, int64_t out_stride, uint8_t* o
   a.N = out_features;
   a.kbytes = in_features / 2;
   a.blocks = in_features / 32;
-  a.loose = a.blocks % 4 != 0 || !aligned(x_scale, 4) || x_scale_stride % 4 != 0 || !aligned(w_scale, 4) || w_scale_stride % 4 != 0;
+  a.scale_piece = mx_scale_piece(a);
   a.out_type = out_dtype;
   if (quant) {
     if (swiglu) launch_linear_mx<MM_SWIGLU_Q>(a, stream);

@@ -59,7 +59,6 @@ def operand(g, rows, K, spread=1.0):
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
 @pytest.mark.parametrize("T,K", [(1, 32), (3, 96), (5, 160), (17, 2048), (300, 6144), (1025, 416), (4099, 4096)])
 def test_quant_and_back(device, dtype, T, K):
-    """The last size takes the kernels that have several rows a lane, with rows left over."""
     g = torch.Generator().manual_seed(T + K)
     x = (torch.randn(T, K + 32, generator=g) * torch.exp(2 * torch.randn(T, 1, generator=g))).to(dtype)
     x[0, :K // 2] = 0

@@ -14,10 +14,10 @@ namespace {
 
 // The tokens are quantised by the workgroups behind those that sort (or count, where
 // several do).
-template <int DT, int ROWS> __global__ __launch_bounds__(PLAN_THREADS) void mx_expert_start_k(PlanArgs a, MxQuantArgs q) {
+template <int DT> __global__ __launch_bounds__(PLAN_THREADS) void mx_expert_start_k(PlanArgs a, MxQuantArgs q) {
   __shared__ int next[MAX_EXPERTS], part[PLAN_THREADS / 64];
   if ((int)blockIdx.x >= a.blocks)
-    mx_quant_item<DT, ROWS>(q, (blockIdx.x - a.blocks) * PLAN_THREADS + threadIdx.x);
+    mx_quant_item<DT>(q, (blockIdx.x - a.blocks) * PLAN_THREADS + threadIdx.x);
   else if (a.blocks > 1)
     expert_count(a, next);
   else
@@ -141,14 +141,11 @@ extern "C" gr_status_t gr_expert_mlp_mxfp4(void* out, int64_t out_stride, const 
                    reinterpret_cast<int32_t*>(ws + l.slot), reinterpret_cast<int4*>(ws + l.tiles),
                    reinterpret_cast<int32_t*>(ws + l.num_tiles), dev_status};
   const MxQuantArgs q{ws + l.x4, H / 2, ws + l.xs, H / 32, x, x_stride, T, H};
-  const int quant = mx_quant_rows(T, H, dtype);
-  const int64_t items = ((int64_t)T + quant - 1) / quant * (H / 16);
+  const int64_t items = (int64_t)T * (H / 16);
   const dim3 start((unsigned)(l.blocks + (items + PLAN_THREADS - 1) / PLAN_THREADS));
-  auto first = [&](auto one, auto two) {
-    hipLaunchKernelGGL(quant == 2 ? two : one, start, dim3(PLAN_THREADS), 0, stream, p, q);
-  };
-  if (dtype == GR_DTYPE_F16) first(mx_expert_start_k<GR_DTYPE_F16, 1>, mx_expert_start_k<GR_DTYPE_F16, 2>);
-  else first(mx_expert_start_k<GR_DTYPE_BF16, 1>, mx_expert_start_k<GR_DTYPE_BF16, 2>);
+  auto first = [&](auto k) { hipLaunchKernelGGL(k, start, dim3(PLAN_THREADS), 0, stream, p, q); };
+  if (dtype == GR_DTYPE_F16) first(mx_expert_start_k<GR_DTYPE_F16>);
+  else first(mx_expert_start_k<GR_DTYPE_BF16>);
   if (l.blocks > 1) hipLaunchKernelGGL(expert_plan_k, dim3(l.blocks), dim3(PLAN_THREADS), 0, stream, p);
 
   MxArgs up{};

@@ -121,6 +121,8 @@ def test_zeros_of_every_scale(device):
             assert (o4 & 0x77 == 0).all() and (os == 0).all()
     none = ops.linear_mxfp4(x4[:0], xs[:0], w4, ws)
     assert none.shape == (0, 256)
+    a, *_ = make(4, 3, 2, 64, 32, torch.bfloat16, device)
+    assert ops.expert_mlp_mxfp4(a[0][:0], *a[1:5], a[5][:0], a[6][:0]).shape == (0, 64)
     o4, s = ops.quant_mxfp4(torch.zeros(0, 64, device=device))
     assert o4.shape == (0, 32) and s.shape == (0, 2) and ops.dequant_mxfp4(o4, s).shape == (0, 64)
 

@@ -73,16 +73,17 @@ template <int DT> __global__ __launch_bounds__(MXQ_THREADS) void mx_dequant_k(Mx
 // The tile with the least estimated time (as for the 8-bit products): over the workgroups
 // of the XCD that gets the most of them, whose 32 CUs take one or two each, a round costs
 // a fixed part and its stages of 256 features, `one` ns each alone on a CU, `two` with a
-// neighbour.  Fitted to 250 measured sizes of 48 to 8192 rows, 512 to 12288 weight rows
-// and 512 to 6144 features: the pick is 1.1 % slower than the best tile in the mean, more
-// than 10 % in 3 of 100.  (us; rows x weight rows x features, the picked tile's and the next one's)
-//   64 x 4096 x 2048     64 x 64     5.1,   64 x 128          6.4
-//   1001 x 2048 x 6144   64 x 64    15.3,   64 x 128         15.5
-//   512 x 8192 x 2048   128 x 128    9.7,   64 x 128         10.3
-//   2048 x 2048 x 6144  128 x 128   19.3,   64 x 128         23.8
-//   8192 x 12288 x 512  128 x 128 of two stages, two a CU: 57 (in 4 bits), 256 x 256  63
-//   512 x 12288 x 2048  128 x 256   13.0,  128 x 128         15.1
-//   8192 x 12288 x 2048 256 x 256    134,  128 x 256          178
+// neighbour.  Fitted to 339 measured sizes of 48 to 8192 rows, 512 to 12288 weight rows
+// and 512 to 6144 features: the pick is 0.7 % slower than the best tile in the mean and
+// 10 % at most.  (us; rows x weight rows x features, the picked tile's and the next one's)
+//   48 x 4096 x 2048     64 x 64     5.1,   64 x 128   6.5
+//   1024 x 2048 x 6144   64 x 128   15.9,   64 x 64   15.3
+//   400 x 4096 x 2048    64 x 128    7.1,  128 x 128   8.1
+//   512 x 8192 x 2048   128 x 128   10.0,   64 x 128  10.3
+//   2048 x 2048 x 6144  128 x 128   21.0,   64 x 128  25.1
+//   3000 x 12288 x 512  128 x 128 of two stages, two a CU  22.0, 256 x 256  25.2
+//   512 x 12288 x 2048  128 x 256   12.9,  128 x 128  13.9
+//   8192 x 12288 x 2048 256 x 256    131,  128 x 128   174
 struct MxChoice { int bm, bn, per_cu, launch, fixed1, one, fixed2, two; };
 constexpr MxChoice kMx[] = {{64, 64, 2, 1910, 950, 291, 1500, 454},   {64, 128, 2, 2130, 1210, 450, 1910, 728},
                             {128, 128, 1, 910, 2740, 609, 0, 0},      {128, 128, 2, 2250, 520, 863, 2370, 1196},

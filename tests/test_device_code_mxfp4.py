@@ -40,8 +40,8 @@ def test_transfers_are_what_the_waits_count():
     kernels = _kernels(_disassembly(), "mx_mm")
     assert len(kernels) >= 20
     for name, code in kernels.items():
-        bm, bn, wm, wn, st = map(int, re.search(r"mx_mmILi(\d+)ELi(\d+)ELi(\d+)ELi(\d+)ELi(\d+)E", name).groups())
-        per = (bm + bn) // 8 // (wm * wn)
+        bm, bn, wm, wn, kg, st = map(int, re.search(r"mx_mmI" + r"Li(\d+)E" * 6, name).groups())
+        per = (bm + bn) // 8 // (wm * wn)  # of a wave: kg groups of them send kg stages
         # the first stages, then the loop's body, sent once each
         assert sum(map(_rows, code)) == st * per and _late(code) == 0, name
         waits = [code[i - 1] for i, ins in enumerate(code) if ins.startswith("s_barrier")]

@@ -28,7 +28,8 @@ def random_rows(g, rows, K, device):
 # and columns left over
 @pytest.mark.parametrize("M,N,K", [(8, 8192, 6144), (20, 4000, 160), (64, 4096, 2048), (200, 2000, 96), (511, 8184, 2048),
                                    (1001, 2048, 6144), (512, 12280, 2048), (2047, 12300, 288), (8190, 12280, 512),
-                                   (4090, 8190, 1056)])
+                                   (4090, 8190, 1056), (500, 2040, 6144), (250, 2000, 1056), (700, 2300, 2080),
+                                   (300, 4128, 2304)])
 def test_large_tiles(device, M, N, K):
     g = torch.Generator(device=device).manual_seed(M + N + K)
     x4, xs, x = random_rows(g, M, K, device)
@@ -42,7 +43,7 @@ def test_large_tiles(device, M, N, K):
 
 
 @pytest.mark.parametrize("M,N,K", [(20, 2016, 160), (200, 1024, 96), (511, 4096, 544), (520, 6144, 2048), (4100, 6112, 96),
-                                   (4100, 2080, 1056)])
+                                   (4100, 2080, 1056), (500, 1024, 2336), (300, 2048, 2304), (4100, 6144, 1056)])
 def test_large_gated_tiles(device, M, N, K):
     g = torch.Generator(device=device).manual_seed(M + N + K)
     x4, xs, x = random_rows(g, M, K, device)

@@ -65,13 +65,13 @@ __device__ __forceinline__ void dma_v4(uint32_t lds, const void* addr) {
                    : "=&s"(save) : "s"(m), "v"(addr) : "memory");
 }
 
-// BM rows by BN weight rows, WM x WN waves (SwiGLU: 16 gate rows and their 16 up rows alternate)
-template <int BM, int BN, int WM, int WN, int CH, int MODE, bool EXPERTS>
+// BM rows by BN weight rows, KG groups of WM x WN waves (SwiGLU: 16 gate rows and their 16 up rows alternate)
+template <int BM, int BN, int WM, int WN, int KG, int CH, int MODE, bool EXPERTS>
 struct Mx {
   static constexpr bool GATED = MODE == MM_SWIGLU || MODE == MM_SWIGLU_Q;
   static constexpr bool QUANT = MODE == MM_SWIGLU_Q || MODE == MM_PLAIN_Q;
   using M = Mm<GR_DTYPE_BF16, BM, BN, WM, WN, GATED ? MM_SWIGLU : MM_PLAIN, EXPERTS, false>;  // rows of bytes
-  static constexpr int NW = WM * WN, ROWS = BM + BN, TILE = M::TILE, LPS = M::LPS, FM = M::FM, FN = M::FN, OC = M::OC;
+  static constexpr int NW = WM * WN * KG, ROWS = BM + BN, TILE = M::TILE, LPS = ROWS / 8 / NW, FM = M::FM, FN = M::FN, OC = M::OC;
   // Scales come CH stages at a time, 16 bytes a lane or (WORDS) 4, as linear rows of 8 CH
   // bytes: a transfer costs as much as one of rows does, however little it brings (experts
   // of 5001 tokens, 256 x 256 tiles: up product 114 us by words, 99 us by 16 bytes).
@@ -228,60 +228,69 @@ template <typename M> __device__ __forceinline__ uint32_t mx_block(const typenam
   return s;
 }
 
-// ST stages of LDS, one barrier a stage, as block_mm: stage s has landed when all but the
-// ST - 2 younger ones' transfers of rows have (scales are sent ahead of their first stage's
-// rows, so they have too); past its barrier nobody reads stage s - 1, whose buffer takes
-// stage s + ST - 1, nor the scales before the current ones.
-template <int BM, int BN, int WM, int WN, int ST, int CH, int MODE, bool EXPERTS> struct MxLds {
-  using X = Mx<BM, BN, WM, WN, CH, MODE, EXPERTS>;
-  static constexpr int NS = (ST - 1 + CH - 1) / CH + 1;  // buffers of scales
-  static constexpr int BYTES = ST * X::TILE + NS * X::SCALES;
+// A step is a stage, or one for each of KG groups of waves, whose sums meet in LDS: where a
+// CU has one workgroup, a group's reads and products go on while the other waits (512 x
+// 2048 of 6144 features, 64 x 64 tiles 10.8 us and 9.9, 64 x 128 14.2 and 12.5).
+// ST steps of LDS, one barrier a step, as block_mm: step s has landed when all but the
+// ST - 2 younger ones' transfers of rows have (scales are sent ahead of their first step's
+// rows, so they have too); past its barrier nobody reads step s - 1, whose buffer takes
+// step s + ST - 1, nor the scales before the current ones.
+template <int BM, int BN, int WM, int WN, int KG, int ST, int CH, int MODE, bool EXPERTS> struct MxLds {
+  using X = Mx<BM, BN, WM, WN, KG, CH, MODE, EXPERTS>;
+  static_assert(CH % KG == 0, "whole steps");
+  static constexpr int STEPS = CH / KG, NS = (ST - 1 + STEPS - 1) / STEPS + 1;  // that a buffer of scales is for, and buffers
+  static constexpr int BYTES = ST * KG * X::TILE + NS * X::SCALES;
   static constexpr int WAVES = X::NW / 4 * (BYTES <= 80 * 1024 ? 2 : 1);  // of a SIMD: two workgroups, where LDS has room
 };
-template <int BM, int BN, int WM, int WN, int ST, int CH, int MODE, bool EXPERTS>
-__global__ __launch_bounds__(64 * WM * WN, (MxLds<BM, BN, WM, WN, ST, CH, MODE, EXPERTS>::WAVES)) void mx_mm(MxArgs a) {
-  using X = Mx<BM, BN, WM, WN, CH, MODE, EXPERTS>;
+template <int BM, int BN, int WM, int WN, int KG, int ST, int CH, int MODE, bool EXPERTS>
+__global__ __launch_bounds__(64 * WM * WN * KG, (MxLds<BM, BN, WM, WN, KG, ST, CH, MODE, EXPERTS>::WAVES)) void mx_mm(MxArgs a) {
+  using X = Mx<BM, BN, WM, WN, KG, CH, MODE, EXPERTS>;
+  using L = MxLds<BM, BN, WM, WN, KG, ST, CH, MODE, EXPERTS>;
   using M = typename X::M;
   constexpr int BLOCKS = X::OC / 32, PITCH = X::OC / 2 + 16;  // of a row in 4 bits
-  constexpr int NS = MxLds<BM, BN, WM, WN, ST, CH, MODE, EXPERTS>::NS;
-  static_assert(!X::QUANT || BM * (PITCH + BLOCKS) <= ST * X::TILE, "the results' rows fit");
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[MxLds<BM, BN, WM, WN, ST, CH, MODE, EXPERTS>::BYTES];
+  constexpr int AT_SCALES = ST * KG * X::TILE;
+  static_assert(!X::QUANT || BM * (PITCH + BLOCKS) <= AT_SCALES, "the results' rows fit");
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[L::BYTES];
   MmTile t;
   if (!M::tile(a, t)) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int wm = wave / WN, wn = wave % WN;
+  const int kg = wave / (WM * WN), wt = wave % (WM * WN), wm = wt / WN, wn = wt % WN;
   typename X::Source src;
   X::source(a, t, wave, lane, src);
   const typename X::Lane l = X::lane_of(wm, wn, lane);
-  const int n = __builtin_amdgcn_readfirstlane((a.kbytes + 127) >> 7);
+  const int n = __builtin_amdgcn_readfirstlane((a.kbytes + 128 * KG - 1) / (128 * KG));
   const uint32_t lds0 = (uint32_t)reinterpret_cast<uintptr_t>(lds);
   auto scales = [&](int s) __attribute__((always_inline)) {
-    if (s % CH == 0) X::fetch_scales(a, src, s / CH, lds, ST * X::TILE + s / CH % NS * X::SCALES, wave, lane);
+    if (s % L::STEPS == 0) X::fetch_scales(a, src, s / L::STEPS, lds, AT_SCALES + s / L::STEPS % L::NS * X::SCALES, wave, lane);
   };
   auto scales_at = [&](int s) __attribute__((always_inline)) {
-    return lds + ST * X::TILE + s / CH % NS * X::SCALES + (s % CH * 8 ^ l.ssw);
+    return lds + AT_SCALES + s / L::STEPS % L::NS * X::SCALES + ((s % L::STEPS * KG + kg) * 8 ^ l.ssw);
   };
   typename X::Acc acc;
 #pragma unroll
   for (int i = 0; i < X::FN; ++i)
 #pragma unroll
     for (int j = 0; j < X::FM; ++j) acc[i][j] = mm4_t{0.f, 0.f, 0.f, 0.f};
+  constexpr int SENDS = KG * X::LPS;  // of a wave and step
+  auto send = [&](int c, int s, uint32_t to) __attribute__((always_inline)) {
+    X::fetch_rows(a, src, c % X::LPS, s * KG + c / X::LPS, to + c / X::LPS * X::TILE, wave);
+  };
 #pragma unroll
   for (int s = 0; s < ST - 1; ++s)
     if (s < n) {
       scales(s);
 #pragma unroll
-      for (int i = 0; i < X::LPS; ++i) X::fetch_rows(a, src, i, s, lds0 + s * X::TILE, wave);
+      for (int c = 0; c < SENDS; ++c) send(c, s, lds0 + s * KG * X::TILE);
     }
   int buf = 0;
-  // The transfers of a stage ahead are sent between the first products: sent in one go
+  // The transfers of a step ahead are sent between the first products: sent in one go
   // they keep their wave from its products until the last is taken (512 x 2048 of 6144
   // features, 64 x 128 tiles, 17.2 us and 15.4).
   auto step = [&](int s, auto ahead) __attribute__((always_inline)) {
     constexpr bool AHEAD = decltype(ahead)::value;
-    constexpr int SLOTS = X::FM * X::FN, EACH = (X::LPS + SLOTS - 1) / SLOTS;
-    const uint8_t *p = lds + buf * X::TILE, *sc = scales_at(s);
-    const uint32_t to = lds0 + (buf == 0 ? ST - 1 : buf - 1) * X::TILE;
+    constexpr int SLOTS = X::FM * X::FN, EACH = (SENDS + SLOTS - 1) / SLOTS;
+    const uint8_t *p = lds + (buf * KG + kg) * X::TILE, *sc = scales_at(s);
+    const uint32_t to = lds0 + (buf == 0 ? ST - 1 : buf - 1) * KG * X::TILE;
     typename X::Frag w[X::FN], x, next;
 #pragma unroll
     for (int i = 0; i < X::FN; ++i) w[i] = X::read(p + l.wo + i * 2048, sc + l.wso + i * (128 * CH), l);
@@ -295,7 +304,7 @@ __global__ __launch_bounds__(64 * WM * WN, (MxLds<BM, BN, WM, WN, ST, CH, MODE, 
         if constexpr (AHEAD)
 #pragma unroll
           for (int c = 0; c < EACH; ++c)
-            if ((j * X::FN + i) * EACH + c < X::LPS) X::fetch_rows(a, src, (j * X::FN + i) * EACH + c, s + ST - 1, to, wave);
+            if ((j * X::FN + i) * EACH + c < SENDS) send((j * X::FN + i) * EACH + c, s + ST - 1, to);
         acc[i][j] = mx_mma<0>(w[i].v[0], w[i].s, x.v[0], x.s, acc[i][j]);
         acc[i][j] = mx_mma<1>(w[i].v[1], w[i].s, x.v[1], x.s, acc[i][j]);
       }
@@ -305,7 +314,7 @@ __global__ __launch_bounds__(64 * WM * WN, (MxLds<BM, BN, WM, WN, ST, CH, MODE, 
   };
   int s = 0;
   for (; s + ST - 1 < n; ++s) {
-    mm_wait_barrier<(ST - 2) * X::LPS>();
+    mm_wait_barrier<(ST - 2) * SENDS>();
     step(s, std::true_type());
   }
   for (; s < n; ++s) {
@@ -313,12 +322,35 @@ __global__ __launch_bounds__(64 * WM * WN, (MxLds<BM, BN, WM, WN, ST, CH, MODE, 
     step(s, std::false_type());
   }
   __syncthreads();
+  if constexpr (KG > 1) {  // the groups' sums meet
+    static_assert(KG == 2 && WM * WN * X::FM * X::FN * 1024 <= AT_SCALES, "room for a group's");
+    mm4_t* part = reinterpret_cast<mm4_t*>(lds) + wt * X::FM * X::FN * 64 + lane;
+    if (kg == 1)
+#pragma unroll
+      for (int i = 0; i < X::FN; ++i)
+#pragma unroll
+        for (int j = 0; j < X::FM; ++j) part[(i * X::FM + j) * 64] = acc[i][j];
+    __syncthreads();
+    if (kg == 0)
+#pragma unroll
+      for (int i = 0; i < X::FN; ++i)
+#pragma unroll
+        for (int j = 0; j < X::FM; ++j) {
+          const mm4_t v = part[(i * X::FM + j) * 64];
+#pragma unroll
+          for (int u = 0; u < 4; ++u) acc[i][j][u] += v[u];
+        }
+    __syncthreads();
+    if constexpr (!X::QUANT)
+      if (kg == 1) return;
+  }
   if constexpr (X::QUANT) {
     // through LDS, so that a row's blocks of the tile are written side by side
     const int r16 = lane & 15, q = lane >> 4, c0 = wn * (X::OC / WN);
     uint8_t* scale = lds + BM * PITCH;
 #pragma unroll
     for (int j = 0; j < X::FM; ++j) {
+      if (kg > 0) break;
       const int r = wm * (BM / WM) + j * 16 + r16;
 #pragma unroll
       for (int g = 0; g < M::FO / 2; ++g) {
@@ -340,7 +372,7 @@ __global__ __launch_bounds__(64 * WM * WN, (MxLds<BM, BN, WM, WN, ST, CH, MODE, 
       a.os4[row * a.os4_row + t.n0 / 32 + b] = scale[c];
     }
   } else {
-    M::store_any(a, t, acc, wave, wm, wn, lane, lds);
+    M::store_any(a, t, acc, wt, wm, wn, lane, lds);
   }
 }
 
@@ -438,13 +470,13 @@ template <int NF, int WK, int MODE> __global__ __launch_bounds__(64 * WK) void m
   }
 }
 
-template <int BM, int BN, int WM, int WN, int ST, int CH, int MODE, bool EXPERTS>
+template <int BM, int BN, int WM, int WN, int ST, int CH, int MODE, bool EXPERTS, int KG = 1>
 void launch_mx(MxArgs a, int tiles_m, hipStream_t stream) {
-  using X = Mx<BM, BN, WM, WN, CH, MODE, EXPERTS>;
+  using X = Mx<BM, BN, WM, WN, KG, CH, MODE, EXPERTS>;
   a.tiles_m = tiles_m;
   a.tiles_n = (a.N + X::OC - 1) / X::OC;
   const int64_t total = (int64_t)tiles_m * a.tiles_n;
-  hipLaunchKernelGGL((mx_mm<BM, BN, WM, WN, ST, CH, MODE, EXPERTS>), dim3((unsigned)((total + 7) / 8 * 8)), dim3(64 * WM * WN),
+  hipLaunchKernelGGL((mx_mm<BM, BN, WM, WN, KG, ST, CH, MODE, EXPERTS>), dim3((unsigned)((total + 7) / 8 * 8)), dim3(64 * X::NW),
                      0, stream, a);
 }
 template <int NF, int WK, int MODE> void launch_mx_few(MxArgs a, hipStream_t stream) {

@@ -74,25 +74,26 @@ template <int DT> __global__ __launch_bounds__(MXQ_THREADS) void mx_dequant_k(Mx
 // of the XCD that gets the most of them, whose 32 CUs take one or two each, a round costs
 // a fixed part and its stages of 256 features, `one` ns each alone on a CU, `two` with a
 // neighbour.  Fitted to 339 measured sizes of 48 to 8192 rows, 512 to 12288 weight rows
-// and 512 to 6144 features: the pick is 0.7 % slower than the best tile in the mean and
-// 10 % at most.  (us; rows x weight rows x features, the picked tile's and the next one's)
-//   48 x 4096 x 2048     64 x 64     5.1,   64 x 128   6.5
-//   1024 x 2048 x 6144   64 x 128   15.9,   64 x 64   15.3
-//   400 x 4096 x 2048    64 x 128    7.1,  128 x 128   8.1
+// and 512 to 6144 features: the pick is 0.4 % slower than the best tile in the mean and
+// 9 % at most.  (us; rows x weight rows x features, the picked tile's and the next one's)
+//   400 x 4096 x 2048    64 x 64     6.9,   64 x 128   7.1
+//   256 x 2048 x 6144    64 x 64, two groups  9.4, one  10.1
+//   400 x 4096 x 6144    64 x 128, two groups  13.1, one  14.3
 //   512 x 8192 x 2048   128 x 128   10.0,   64 x 128  10.3
 //   2048 x 2048 x 6144  128 x 128   21.0,   64 x 128  25.1
 //   3000 x 12288 x 512  128 x 128 of two stages, two a CU  22.0, 256 x 256  25.2
 //   512 x 12288 x 2048  128 x 256   12.9,  128 x 128  13.9
 //   8192 x 12288 x 2048 256 x 256    131,  128 x 128   174
 struct MxChoice { int bm, bn, per_cu, launch, fixed1, one, fixed2, two; };
-constexpr MxChoice kMx[] = {{64, 64, 2, 1910, 950, 291, 1500, 454},   {64, 128, 2, 2130, 1210, 450, 1910, 728},
-                            {128, 128, 1, 910, 2740, 609, 0, 0},      {128, 128, 2, 2250, 520, 863, 2370, 1196},
-                            {128, 256, 1, 760, 4070, 953, 0, 0},      {256, 256, 1, 200, 6510, 1563, 0, 0}};
+constexpr MxChoice kMx[] = {{64, 64, 2, 1840, 980, 296, 1500, 448},   {64, 64, 1, 1060, 1980, 249, 0, 0},  // (the second in two groups)
+                            {64, 128, 2, 2060, 1310, 442, 1960, 703}, {64, 128, 1, 1240, 2560, 366, 0, 0},
+                            {128, 128, 1, 910, 2690, 616, 0, 0},      {128, 128, 2, 2150, 650, 863, 2490, 1198},
+                            {128, 256, 1, 550, 4290, 961, 0, 0},      {256, 256, 1, -90, 6880, 1607, 0, 0}};
 
 int pick_mx(int M, int rows_w, int stages, bool quant) {
   int best = -1;
   int64_t least = 0;
-  for (int i = quant ? 1 : 0; i < 6; ++i) {  // (a wave of a 64 x 64 tile has 16 gated results of a row, half a block)
+  for (int i = quant ? 2 : 0; i < 8; ++i) {  // (a wave of a 64 x 64 tile has 16 gated results of a row, half a block)
     const MxChoice& c = kMx[i];
     const int64_t tiles = ((int64_t)((M + c.bm - 1) / c.bm) * ((rows_w + c.bn - 1) / c.bn) + 7) / 8;
     const int64_t one = c.fixed1 + (int64_t)stages * c.one, two = c.per_cu == 2 ? c.fixed2 + (int64_t)stages * c.two : one;
@@ -120,10 +121,14 @@ template <int MODE> void launch_linear_mx(const MxArgs& a, hipStream_t stream) {
     case 0:
       if constexpr (!QUANT) launch_mx<64, 64, 2, 2, 4, 4, MODE, false>(a, (M + 63) / 64, stream);
       break;
-    case 1: launch_mx<64, 128, 2, 2, 3, 2, MODE, false>(a, (M + 63) / 64, stream); break;
-    case 2: launch_mx<128, 128, 4, 2, 3, 2, MODE, false>(a, (M + 127) / 128, stream); break;
-    case 3: launch_mx<128, 128, 4, 2, 2, 1, MODE, false>(a, (M + 127) / 128, stream); break;
-    case 4: launch_mx<128, 256, 2, 4, 3, 2, MODE, false>(a, (M + 127) / 128, stream); break;
+    case 1:
+      if constexpr (!QUANT) launch_mx<64, 64, 2, 2, 3, 4, MODE, false, 2>(a, (M + 63) / 64, stream);
+      break;
+    case 2: launch_mx<64, 128, 2, 2, 3, 2, MODE, false>(a, (M + 63) / 64, stream); break;
+    case 3: launch_mx<64, 128, 2, 2, 3, 4, MODE, false, 2>(a, (M + 63) / 64, stream); break;
+    case 4: launch_mx<128, 128, 4, 2, 3, 2, MODE, false>(a, (M + 127) / 128, stream); break;
+    case 5: launch_mx<128, 128, 4, 2, 2, 1, MODE, false>(a, (M + 127) / 128, stream); break;
+    case 6: launch_mx<128, 256, 2, 4, 3, 2, MODE, false>(a, (M + 127) / 128, stream); break;
     default: launch_mx<256, 256, 2, 4, 2, 2, MODE, false>(a, (M + 255) / 256, stream);
   }
 }

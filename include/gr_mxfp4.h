@@ -70,9 +70,8 @@ gr_status_t gr_linear_mxfp4(void* out, int64_t out_stride, uint8_t* out_scale, i
  * hidden, ffn] with their scales, all contiguous; weights float32, ids int32
  * [num_tokens, top_k] contiguous.  An id below 0 adds nothing (an expert of another
  * rank), one >= num_experts flags GR_DEV_BAD_EXPERT and adds nothing; an expert named
- * twice counts twice.  Sums are float32; each expert's result is rounded to fp16 times a
- * power of two (2^-11 of a value, 2^-39 of the largest of its row's 64 neighbouring
- * columns) before the sum over j, which is float32 and in the order of j.  As for
+ * twice counts twice.  Sums are float32, the one over j too, which is in the order of j
+ * and rounded once.  As for
  * gr_linear_mxfp4, a token's last bits may differ between calls of other sizes.
  * hidden % 32 == 0, ffn % 32 == 0; rows of x, and weights, 16-byte aligned; out rows
  * 8-byte aligned.  num_experts <= 1024, num_tokens < 2^23, num_tokens * hidden <

@@ -1,6 +1,6 @@
 // The chosen experts' SwiGLU layers with 4-bit microscaled weights (gr_mx_mm.h): the
 // tokens are quantised once, each expert's gated product is written in 4 bits, and its
-// result waits for the sum over a token's experts as scaled fp16.
+// result waits for the sum over a token's experts in float32.
 #include <algorithm>
 #include <cmath>
 
@@ -25,7 +25,7 @@ template <int DT> __global__ __launch_bounds__(PLAN_THREADS) void mx_expert_star
 }
 
 struct MxWorkspace {
-  int64_t hist, slot, tiles, num_tiles, x4, xs, act, act_scale, y, y_exp, bytes;
+  int64_t hist, slot, tiles, num_tiles, x4, xs, act, act_scale, y, bytes;
   int64_t max_tiles;
   int blocks;
 };
@@ -34,14 +34,13 @@ struct MxWorkspace {
 // way from memory, many by the products and the results.  Measured (64 experts of 768
 // features, hidden 2048, 8 of them a token; us of both products, by tile rows):
 //   rows an expert    8    16    24    28    32    48    64    80    96   128   192   224   256   300   375   625
-//    32            33.3  40.0  40.5  43.4  45.7  51.1
-//    64            39.8  42.0  42.9  43.3  43.5  45.6  51.8  59.8  64.3  79.8
-//   128                                    48.6  51.9  54.3  56.1  57.6  74.4  94.1   107   113   131   155   233
-//   256                                                                  87.2  95.3   111   114   126   131   199
+//    32            33.1  40.8  42.2  45.5  47.3  51.8  66.0
+//    64            40.0  42.2  43.8  44.5  45.1  47.7  55.2  65.0  69.4  82.6
+//   128                        49.9  50.8  50.9  55.3  58.8  64.5  67.3  81.5  99.1   112   119   139   163   252
+//   256                                                                  93.0  99.4   119   125   137   143   222
 int mx_tile_rows(int64_t rows, int E) {
   return rows <= 28ll * E ? 32 : rows <= 72ll * E ? 64 : rows <= 260ll * E ? 128 : 256;
 }
-constexpr int MX_WAVE_COLS = 64;  // columns of a wave of the down product, whatever its tiles
 
 MxWorkspace plan_mx_workspace(int T, int k, int E, int H, int F, int bm) {
   MxWorkspace w{};
@@ -61,8 +60,7 @@ MxWorkspace plan_mx_workspace(int T, int k, int E, int H, int F, int bm) {
   w.xs = take((int64_t)T * ((H + 31) / 32));
   w.act = take(rows * ((F + 1) / 2));
   w.act_scale = take(rows * ((F + 31) / 32));
-  w.y = take(2 * rows * H);
-  w.y_exp = take(rows * ((H + 15) / 16));
+  w.y = take(4 * rows * H);
   return w;
 }
 
@@ -74,10 +72,10 @@ void launch_mx_experts(const MxArgs& up, const MxArgs& down, int tiles, int E, i
     // taken, else the first (64 experts of 768 features, hidden 2048, 8 a token; us):
     //   tokens                     1     8    12    16    64    80    96   128
     //   workgroups up             96   483   619   680   768   768   768   768
-    //   three stages             7.1  12.7  18.5  20.0  25.5  26.5  26.4  26.5
-    //   two                      8.8  12.4  15.3  16.7  21.5  24.1  27.7  28.1
-    //   down 64                  4.6   8.3   9.9  11.9  12.9  13.1  13.2  13.5
-    //   down 256                 5.6   9.1   9.5   9.8  11.8  13.2  15.5  16.0
+    //   three stages             7.3  12.9  19.1  20.3  25.9  27.0  26.9  26.4
+    //   two                      9.7  12.7  15.8  16.8  21.0  24.2  27.8  28.4
+    //   down 64                  4.3   8.1   9.7  11.8  13.5  13.5  13.7  14.4
+    //   down 256                 5.7   9.4   9.5   9.8  12.2  13.6  15.9  16.6
     const double reached = E * (1.0 - std::exp(-(double)up.M / E));
     const double wgs = reached * ((up.N + 63) / 64), wide = reached * ((down.N + 255) / 256);
     const bool once = up.M <= 10ll * E;  // (more rows give some experts a second tile)
@@ -190,19 +188,19 @@ extern "C" gr_status_t gr_expert_mlp_mxfp4(void* out, int64_t out_stride, const 
   dn.kbytes = F / 2;
   dn.blocks = F / 32;
   dn.scale_piece = mx_scale_piece(dn);
-  // (up to 2^-11 of each expert's result: half a step of an fp16 output, little beside the 2^-2 of its 4-bit operands)
-  dn.out_type = MM_OUT_SCALED;
-  dn.out_exp = reinterpret_cast<int8_t*>(ws + l.y_exp);
+  // (fp16 multiples of a power of two would halve what the sum reads, 5001 tokens 246 us for 291, but a token's sum would
+  // be off by 2^-11 of each of its terms, however near its terms' opposites bring it to 0)
+  dn.out_type = GR_DTYPE_F32;
   dn.tiles = p.tiles;
   dn.num_tiles = p.num_tiles;
   dn.slot = p.slot;
   dn.scatter = 1;
   launch_mx_experts(up, dn, (int)l.max_tiles, num_experts, bm, stream);
 
-  const CombineArgs c{out, out_stride, ws + l.y, dn.out_exp, MX_WAVE_COLS, weights, ids, T, top_k, num_experts, H};
+  const CombineArgs c{out, out_stride, ws + l.y, nullptr, 0, weights, ids, T, top_k, num_experts, H};
   const dim3 grid((unsigned)T, (unsigned)((H + 2047) / 2048));
   auto go = [&](auto k) { hipLaunchKernelGGL(k, grid, dim3(256), 0, stream, c); };
-  if (dtype == GR_DTYPE_BF16) go(expert_combine_k<GR_DTYPE_BF16, true>);
-  else go(expert_combine_k<GR_DTYPE_F16, true>);
+  if (dtype == GR_DTYPE_BF16) go(expert_combine_k<GR_DTYPE_BF16, false>);
+  else go(expert_combine_k<GR_DTYPE_F16, false>);
   return launch_status();
 }

@@ -147,7 +147,8 @@ def quantize_blocks(w: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
 def quantize_mxfp4(w: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """``w [..., N, K]`` in 4 bits as ops.quant_mxfp4 makes them, two codes a byte
     ``[..., N, K / 2]`` and a scale byte for each 32 of a row ``[..., N, K / 32]``, both
-    uint8; on any device.  ``K`` is a multiple of 32, and ``w`` finite."""
+    uint8; on any device.  ``K`` is a multiple of 32.  A block with an infinity or a
+    NaN has the scale byte 255: it reads back as NaN, and so does what is made of it."""
     if w.shape[-1] % ops.MXFP4_BLOCK:
         raise ValueError(f"4-bit weights need a multiple of 32 features, not {list(w.shape)}")
     x = w.double().unflatten(-1, (-1, ops.MXFP4_BLOCK))
@@ -155,7 +156,9 @@ def quantize_mxfp4(w: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     half, power = torch.frexp(top)  # half in [0.5, 1) times 2^power
     # the least power of two with top < 7 times it: from 1.75 times one on the next
     e = torch.where(top > 0, power - 3 + (half >= 0.875).int(), -127).clamp(-127, 127)
-    x = x * ((1023 - e).long() << 52).view(torch.float64)[..., None]  # 2^-e by its bits
+    finite = top < 2.0 ** 128
+    e = torch.where(finite, e, 128)
+    x = torch.where(finite[..., None], x, 0.0) * ((1023 - e).long() << 52).view(torch.float64)[..., None]  # 2^-e by its bits
     a = x.abs()
     # e2m1 numbers lie 0.5 apart up to 2, 1 up to 4 and then 2: their codes count them from 0, 2 and 4 on
     code = torch.where(a < 2, (2 * a).round(), torch.where(a < 4, a.round() + 2, (a / 2).round() + 4)).clamp_max(7)

@@ -22,3 +22,31 @@ def test_weights_that_are_not_finite_stay_visible(dtype):
     codes[bad.repeat_interleave(32, -1)], byte[bad] = 0, 255
     for w4, scale in (quantize_mxfp4(w), list(quantize_weights({"layers.0.expert_down": w}, "mxfp4").values())):
         assert torch.equal(scale, byte) and torch.equal(w4, pack(codes))
+
+
+def test_weights_are_taken_piece_by_piece():
+    """Temporaries stay at 2^22 weights at a time, whatever the tensor, and give the definition's codes and scales."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    largest = 0
+
+    class Watch(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            nonlocal largest
+            out = func(*args, **(kwargs or {}))
+            for t in out if isinstance(out, (list, tuple)) else (out,):
+                if isinstance(t, torch.Tensor) and not t._is_view():
+                    largest = max(largest, t.numel() * t.element_size())
+            return out
+
+    w = torch.randn(5, 1000, 2080, generator=torch.Generator().manual_seed(6)).bfloat16()
+    with Watch():
+        w4, scale = quantize_mxfp4(w)
+    assert largest <= 8 * 2 ** 22
+    codes, byte = quantise(w.double())
+    assert torch.equal(scale, byte) and torch.equal(w4, pack(codes))
+    w = w.transpose(1, 2)[:, :, :992]
+    w4, scale = quantize_mxfp4(w)
+    codes, byte = quantise(w.double())
+    assert torch.equal(scale, byte) and torch.equal(w4, pack(codes))
+    assert [t.shape for t in quantize_mxfp4(w[:0])] == [(0, 2080, 496), (0, 2080, 31)]

@@ -149,8 +149,28 @@ def quantize_mxfp4(w: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     ``[..., N, K / 2]`` and a scale byte for each 32 of a row ``[..., N, K / 32]``, both
     uint8; on any device.  ``K`` is a multiple of 32.  A block with an infinity or a
     NaN has the scale byte 255: it reads back as NaN, and so does what is made of it."""
-    if w.shape[-1] % ops.MXFP4_BLOCK:
+    K = w.shape[-1]
+    if K < 1 or K % ops.MXFP4_BLOCK:
         raise ValueError(f"4-bit weights need a multiple of 32 features, not {list(w.shape)}")
+    codes = torch.empty((*w.shape[:-1], K // 2), dtype=torch.uint8, device=w.device)
+    scale = torch.empty((*w.shape[:-1], K // ops.MXFP4_BLOCK), dtype=torch.uint8, device=w.device)
+    kernel = w.is_cuda and w.dtype in (torch.float32, torch.bfloat16, torch.float16)
+    step = max(1, (1 << (28 if kernel else 22)) // K)  # rows at a time
+    for part, c, s in zip(*(t.flatten(0, -3) if t.dim() > 2 else t[None] for t in (w, codes, scale))):
+        for r in range(0, len(part), step):
+            rows = part[r:r + step]
+            if not kernel:
+                c[r:r + step], s[r:r + step] = _mxfp4_rows(rows)
+                continue
+            pitch = rows.stride(0)
+            if rows.stride(1) != 1 or pitch < K or pitch * rows.element_size() % 16 or rows.data_ptr() % 16:
+                rows = rows.clone(memory_format=torch.contiguous_format)
+            ops.quant_mxfp4(rows, out=c[r:r + step], scale=s[r:r + step])
+    return codes, scale
+
+
+def _mxfp4_rows(w: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """Codes and scales of ``w [N, K]`` in float64, some 50 bytes a weight."""
     x = w.double().unflatten(-1, (-1, ops.MXFP4_BLOCK))
     top = x.abs().amax(-1)
     half, power = torch.frexp(top)  # half in [0.5, 1) times 2^power

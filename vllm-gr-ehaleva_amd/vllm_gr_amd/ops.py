@@ -951,20 +951,21 @@ def expert_mlp_workspace_bytes(num_tokens: int, top_k: int, num_experts: int, hi
 
 #: features of a row that share a scale byte
 MXFP4_BLOCK = 32
-_MX_CODES = (torch.uint8, torch.float4_e2m1fn_x2)
-_MX_SCALES = (torch.uint8, torch.float8_e8m0fnu)
+#: types of codes and of scales (older torch has uint8 alone)
+MXFP4_CODES = tuple(getattr(torch, n) for n in ("uint8", "float4_e2m1fn_x2") if hasattr(torch, n))
+MXFP4_SCALES = tuple(getattr(torch, n) for n in ("uint8", "float8_e8m0fnu") if hasattr(torch, n))
 
 
 def _mx_rows(name: str, t: torch.Tensor, scale: torch.Tensor) -> tuple[int, int, int, int]:
     """Rows and features of a 4-bit matrix, and the bytes from row to row of its codes and of its scales."""
-    if t.dim() != 2 or t.stride(1) != 1 or t.dtype not in _MX_CODES:
+    if t.dim() != 2 or t.stride(1) != 1 or t.dtype not in MXFP4_CODES:
         raise ValueError(f"{name} must be a [tokens, features / 2] tensor of two codes a byte (uint8 or "
                          "float4_e2m1fn_x2), a row's side by side")
     rows, half = t.shape
     blocks = half // 16
     if half != 16 * blocks or half > _INT_MAX // 2 or rows > _INT_MAX:
         raise ValueError(f"{name} must have a multiple of 32 features, and at most 2^31 - 1 rows or features")
-    if scale.shape != (rows, blocks) or scale.dtype not in _MX_SCALES or (blocks > 1 and scale.stride(1) != 1):
+    if scale.shape != (rows, blocks) or scale.dtype not in MXFP4_SCALES or (blocks > 1 and scale.stride(1) != 1):
         raise ValueError(f"{name}'s scale must be a uint8 or float8_e8m0fnu [rows, features / 32] tensor, a row's bytes "
                          "side by side")
     if rows > 1:
@@ -1074,10 +1075,10 @@ def expert_mlp_mxfp4(x: torch.Tensor, gate_up: torch.Tensor, gate_up_scale: torc
     E, F = gate_up.shape[0], gate_up.shape[1] // 2
     if H % MXFP4_BLOCK or F % MXFP4_BLOCK:
         raise ValueError("4-bit experts need multiples of 32 features")
-    for name, t, types, shape in (("gate_up", gate_up, _MX_CODES, (E, 2 * F, H // 2)),
-                                  ("down", down, _MX_CODES, (E, H, F // 2)),
-                                  ("gate_up_scale", gate_up_scale, _MX_SCALES, (E, 2 * F, H // MXFP4_BLOCK)),
-                                  ("down_scale", down_scale, _MX_SCALES, (E, H, F // MXFP4_BLOCK))):
+    for name, t, types, shape in (("gate_up", gate_up, MXFP4_CODES, (E, 2 * F, H // 2)),
+                                  ("down", down, MXFP4_CODES, (E, H, F // 2)),
+                                  ("gate_up_scale", gate_up_scale, MXFP4_SCALES, (E, 2 * F, H // MXFP4_BLOCK)),
+                                  ("down_scale", down_scale, MXFP4_SCALES, (E, H, F // MXFP4_BLOCK))):
         if t.dtype not in types or t.shape != shape or not t.is_contiguous():
             raise ValueError(f"{name} must be a contiguous {list(shape)} tensor of {' or '.join(map(str, types))}")
     if ids.dim() != 2 or ids.shape[0] != T or ids.dtype != torch.int32 or not ids.is_contiguous():

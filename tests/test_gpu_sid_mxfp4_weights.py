@@ -4,7 +4,9 @@ import pytest
 import torch
 
 from tests.test_gpu_mxfp4 import pack, quantise
-from vllm_gr_amd.v1.sid_decoder import quantize_mxfp4
+from tests.test_gpu_sid_experts import BF16, EXPERTS
+from tests.test_sid_mxfp4_types_host import typed
+from vllm_gr_amd.v1.sid_decoder import SidDecoder, init_weights, quantize_mxfp4, quantize_weights
 
 pytestmark = pytest.mark.gpu
 
@@ -34,3 +36,14 @@ def test_layouts(device):
             assert torch.equal(scale.cpu(), byte) and torch.equal(w4.cpu(), pack(codes))
             assert w4.is_contiguous() and scale.is_contiguous()
     assert [t.shape for t in quantize_mxfp4(flat[:0])] == [(0, 70, 208), (0, 70, 13)]
+
+
+@pytest.mark.parametrize("cfg", [BF16, EXPERTS], ids=["dense", "experts"])
+def test_types_of_codes_and_scales(device, cfg):
+    """A layer gives the same bits with torch's own types of 4-bit codes and scales as with uint8."""
+    w = {k: v.to(device) for k, v in quantize_weights(init_weights(cfg, 2), "mxfp4").items()}
+    models = [SidDecoder(cfg, t, max_position=8) for t in (w, typed(w))]
+    x = torch.randn(40, cfg.hidden, generator=torch.Generator().manual_seed(3)).to(device).to(cfg.dtype)
+    for f in (lambda m: m._project(x, "layers.1.qkv"), lambda m: m._mlp(x, "layers.1.")):
+        a, b = map(f, models)
+        assert torch.equal(a, b) and a.isfinite().all() and (a != 0).any()

@@ -310,11 +310,11 @@ def _check_quantized(cfg: DecoderConfig, weights: dict[str, torch.Tensor]) -> No
         p = f"layers.{i}."
         for name in (p + "qkv", p + "o", p + names[0], p + names[1]):
             w, scale = weights.get(name), weights.get(name + "_scale")
-            if w is None or (scale is None and w.dtype not in (torch.float8_e4m3fn, torch.uint8)):
+            four = w is not None and w.dtype in ops.MXFP4_CODES
+            if w is None or (scale is None and w.dtype != torch.float8_e4m3fn and not four):
                 continue
-            if scale is None or w.dtype not in (torch.float8_e4m3fn, torch.uint8):
-                raise ValueError(f"{name}: float8_e4m3fn or uint8 weights and {name}_scale go together")
-            four = w.dtype == torch.uint8
+            if scale is None or (w.dtype != torch.float8_e4m3fn and not four):
+                raise ValueError(f"{name}: float8_e4m3fn, uint8 or float4_e2m1fn_x2 weights and {name}_scale go together")
             parts = 2 if name.endswith("gate_up") else 1  # gate's rows, then up's
             N, K = w.shape[-2] // parts, w.shape[-1] * (2 if four else 1)
             each = ops.MXFP4_BLOCK if four else 16
@@ -322,14 +322,14 @@ def _check_quantized(cfg: DecoderConfig, weights: dict[str, torch.Tensor]) -> No
                 raise ValueError(f"{name}: {4 if four else 8}-bit weights need sizes in multiples of {each}, not "
                                  f"{[*w.shape[:-1], K]}")
             if four:
-                shape, dtype = (*w.shape[:-1], K // ops.MXFP4_BLOCK), torch.uint8
+                shape, dtypes = (*w.shape[:-1], K // ops.MXFP4_BLOCK), ops.MXFP4_SCALES
             else:
                 blocks = [-(-n // ops.FP8_BLOCK) for n in (N, K)]
-                shape, dtype = (*w.shape[:-2], parts * blocks[0], blocks[1]), torch.float32
-            if scale.shape != shape or scale.dtype != dtype or not scale.is_contiguous():
-                raise ValueError(f"{name}_scale must be a contiguous {dtype} {list(shape)} tensor")
-        types = {weights[p + n].dtype for n in names if p + n + "_scale" in weights}
-        if len(types) > 1 or (p + names[0] + "_scale" in weights) != (p + names[1] + "_scale" in weights):
+                shape, dtypes = (*w.shape[:-2], parts * blocks[0], blocks[1]), (torch.float32,)
+            if scale.shape != shape or scale.dtype not in dtypes or not scale.is_contiguous():
+                raise ValueError(f"{name}_scale must be a contiguous {' or '.join(map(str, dtypes))} {list(shape)} tensor")
+        fours = {weights[p + n].dtype in ops.MXFP4_CODES for n in names if p + n + "_scale" in weights}
+        if len(fours) > 1 or (p + names[0] + "_scale" in weights) != (p + names[1] + "_scale" in weights):
             raise ValueError(f"{p}{names[0]} and {p}{names[1]} are 8-bit together, 4-bit together or neither")
 
 
@@ -366,7 +366,7 @@ class SidDecoder:
         w, scale = self.w[name], self.w.get(name + "_scale")
         if scale is None:
             return _linear(x, w)
-        if w.dtype == torch.uint8:
+        if w.dtype in ops.MXFP4_CODES:
             return ops.linear_mxfp4(*ops.quant_mxfp4(x), w, scale, out_dtype=x.dtype)
         return ops.linear_fp8(*ops.quant_fp8(x), w, scale, out_dtype=x.dtype)
 
@@ -381,7 +381,7 @@ class SidDecoder:
                 logits, cfg.experts_per_token, score=cfg.router_score, bias=w.get(p + "router_bias"),
                 num_groups=cfg.router_groups, top_groups=cfg.router_top_groups,
                 renormalize=cfg.router_renormalize, scale=cfg.router_scale)
-            if w[p + "expert_gate_up"].dtype == torch.uint8:
+            if w[p + "expert_gate_up"].dtype in ops.MXFP4_CODES:
                 return ops.expert_mlp_mxfp4(x, w[p + "expert_gate_up"], w[p + "expert_gate_up_scale"], w[p + "expert_down"],
                                             w[p + "expert_down_scale"], weights, ids)
             return ops.expert_mlp(x, w[p + "expert_gate_up"], w[p + "expert_down"], weights, ids,
@@ -390,7 +390,7 @@ class SidDecoder:
         scale = w.get(p + "gate_up_scale")
         if scale is None:
             return _linear(_swiglu(x, w[p + "gate_up"]), w[p + "down"])
-        if w[p + "gate_up"].dtype == torch.uint8:
+        if w[p + "gate_up"].dtype in ops.MXFP4_CODES:
             act = ops.linear_mxfp4(*ops.quant_mxfp4(x), w[p + "gate_up"], scale, swiglu=True, quantized=True)
             return ops.linear_mxfp4(*act, w[p + "down"], w[p + "down_scale"], out_dtype=x.dtype)
         act = ops.linear_fp8(*ops.quant_fp8(x), w[p + "gate_up"], scale, swiglu=True, quantized=True)

@@ -85,6 +85,13 @@ gr_status_t gr_expert_mlp_mxfp4(void* out, int64_t out_stride, const void* x, in
                                 int hidden, int ffn, int dtype, void* workspace, size_t workspace_bytes,
                                 int32_t* dev_status, hipStream_t stream);
 
+/*
+ * The tiles that gr_expert_mlp_mxfp4 takes for these sizes: 1000000 * stages of the gated
+ * product on their way + 1000 * rows + columns of the down product; 0 for sizes that
+ * are not positive, and for features above 2^21.
+ */
+int gr_expert_mlp_mxfp4_tile(int num_tokens, int top_k, int num_experts, int hidden, int ffn);
+
 #ifdef __cplusplus
 }
 #endif

@@ -30,7 +30,7 @@ struct MxWorkspace {
   int blocks;
 };
 
-// Rows of a tile, by the rows an expert gets on average: few rows are bound by the weights'
+// Rows of a tile.  By the rows an expert gets on average: few rows are bound by the weights'
 // way from memory, many by the products and the results.  Measured (64 experts of 768
 // features, hidden 2048, 8 of them a token; us of both products, by tile rows):
 //   rows an expert    8    16    24    28    32    48    64    80    96   128   192   224   256   300   375   625
@@ -38,8 +38,22 @@ struct MxWorkspace {
 //    64            40.0  42.2  43.8  44.5  45.1  47.7  55.2  65.0  69.4  82.6
 //   128                        49.9  50.8  50.9  55.3  58.8  64.5  67.3  81.5  99.1   112   119   139   163   252
 //   256                                                                  93.0  99.4   119   125   137   143   222
-int mx_tile_rows(int64_t rows, int E) {
-  return rows <= 28ll * E ? 32 : rows <= 72ll * E ? 64 : rows <= 260ll * E ? 128 : 256;
+// A tall tile is for many workgroups: where the gated product has fewer than 136 (some more than half the CUs),
+// the next lower one is taken.  Over 76 sizes of 1 to 160 experts of 128 to 6144 features, hidden 512 to 4096, the pick
+// is 1.3 % slower than the best tile in the mean and 17 % at most; by the rows alone 12 % and 131 % (us; E experts of F
+// features, hidden H: tiles of 256, 128, 64 and 32 rows):
+//   1200 rows, E 4, F 256, H 512     20.4  12.5  10.5   9.5    32 taken
+//   1000 rows, E 8, F 512, H 2048    31.4  20.4  16.0  15.8    64
+//   4000 rows, E 8, F 512, H 2048    35.5  27.9  31.4  33.4   128
+//   4096 rows, E 8, F 1024, H 4096   67.9  72.2  69.2  93.0   256
+int mx_up_cols(int bm) { return bm <= 64 ? 64 : 128; }  // results of the gated product that a workgroup has
+int mx_tile_rows(int64_t rows, int E, int F) {
+  int bm = rows <= 28ll * E ? 32 : rows <= 72ll * E ? 64 : rows <= 260ll * E ? 128 : 256;
+  auto workgroups = [&] {  // (half of each expert's last tile is empty)
+    return (rows / bm + (std::min<int64_t>(rows, E) + 1) / 2) * (((int64_t)F + mx_up_cols(bm) - 1) / mx_up_cols(bm));
+  };
+  while (bm > 32 && workgroups() < 136) bm /= 2;
+  return bm;
 }
 
 MxWorkspace plan_mx_workspace(int T, int k, int E, int H, int F, int bm) {
@@ -64,30 +78,37 @@ MxWorkspace plan_mx_workspace(int T, int k, int E, int H, int F, int bm) {
   return w;
 }
 
-void launch_mx_experts(const MxArgs& up, const MxArgs& down, int tiles, int E, int bm, hipStream_t stream) {
-  if (bm == 32) {
-    // Few rows: what counts is that all workgroups of a product are on the CUs at once.  Of the experts, choices
-    // that fall evenly reach `reached`.  Up: 64 results a workgroup, two workgroups a CU with three stages each, or
-    // three with two.  Down: 64 columns, six a CU, or 256, two a CU.  Where all fit in the second form only it is
-    // taken, else the first (64 experts of 768 features, hidden 2048, 8 a token; us):
-    //   tokens                     1     8    12    16    64    80    96   128
-    //   workgroups up             96   483   619   680   768   768   768   768
-    //   three stages             7.3  12.9  19.1  20.3  25.9  27.0  26.9  26.4
-    //   two                      9.7  12.7  15.8  16.8  21.0  24.2  27.8  28.4
-    //   down 64                  4.3   8.1   9.7  11.8  13.5  13.5  13.7  14.4
-    //   down 256                 5.7   9.4   9.5   9.8  12.2  13.6  15.9  16.6
-    const double reached = E * (1.0 - std::exp(-(double)up.M / E));
-    const double wgs = reached * ((up.N + 63) / 64), wide = reached * ((down.N + 255) / 256);
-    const bool once = up.M <= 10ll * E;  // (more rows give some experts a second tile)
-    if (once && wgs > 512 && wgs <= 768) launch_mx<32, 128, 2, 2, 2, 2, MM_SWIGLU_Q, true>(up, tiles, stream);
+// The products' forms: rows of a tile, the gated product's stages on their way, the down product's columns.
+struct MxForm { int bm, up_stages, down_cols; };
+MxForm pick_mx_experts(int64_t rows, int E, int H, int F) {
+  const int bm = mx_tile_rows(rows, E, F);
+  if (bm > 32) return {bm, bm == 256 ? 2 : 3, bm == 256 ? 256 : 128};
+  // Few rows: what counts is that all workgroups of a product are on the CUs at once.  Of the experts, choices
+  // that fall evenly reach `reached`.  Up: 64 results a workgroup, two workgroups a CU with three stages each, or
+  // three with two.  Down: 64 columns, six a CU, or 256, two a CU.  Where all fit in the second form only it is
+  // taken, else the first (64 experts of 768 features, hidden 2048, 8 a token; us):
+  //   tokens                     1     8    12    16    64    80    96   128
+  //   workgroups up             96   483   619   680   768   768   768   768
+  //   three stages             7.3  12.9  19.1  20.3  25.9  27.0  26.9  26.4
+  //   two                      9.7  12.7  15.8  16.8  21.0  24.2  27.8  28.4
+  //   down 64                  4.3   8.1   9.7  11.8  13.5  13.5  13.7  14.4
+  //   down 256                 5.7   9.4   9.5   9.8  12.2  13.6  15.9  16.6
+  const double reached = E * (1.0 - std::exp(-(double)rows / E));
+  const double wgs = reached * ((F + 63) / 64), wide = reached * ((H + 255) / 256);
+  const bool once = rows <= 10ll * E;  // (more rows give some experts a second tile)
+  return {32, once && wgs > 512 && wgs <= 768 ? 2 : 3, once && wide <= 512 && reached * ((H + 63) / 64) > 1536 ? 256 : 64};
+}
+
+void launch_mx_experts(const MxArgs& up, const MxArgs& down, int tiles, const MxForm& f, hipStream_t stream) {
+  if (f.bm == 32) {
+    if (f.up_stages == 2) launch_mx<32, 128, 2, 2, 2, 2, MM_SWIGLU_Q, true>(up, tiles, stream);
     else launch_mx<32, 128, 2, 2, 3, 2, MM_SWIGLU_Q, true>(up, tiles, stream);
-    if (once && wide <= 512 && reached * ((down.N + 63) / 64) > 1536)
-      launch_mx<32, 256, 1, 4, 2, 1, MM_PLAIN, true>(down, tiles, stream);
+    if (f.down_cols == 256) launch_mx<32, 256, 1, 4, 2, 1, MM_PLAIN, true>(down, tiles, stream);
     else launch_mx<32, 64, 2, 1, 2, 1, MM_PLAIN, true>(down, tiles, stream);
-  } else if (bm == 64) {
+  } else if (f.bm == 64) {
     launch_mx<64, 128, 2, 2, 3, 2, MM_SWIGLU_Q, true>(up, tiles, stream);
     launch_mx<64, 128, 2, 2, 2, 1, MM_PLAIN, true>(down, tiles, stream);
-  } else if (bm == 128) {
+  } else if (f.bm == 128) {
     launch_mx<128, 256, 2, 4, 3, 2, MM_SWIGLU_Q, true>(up, tiles, stream);
     launch_mx<128, 128, 4, 2, 2, 1, MM_PLAIN, true>(down, tiles, stream);
   } else {
@@ -105,8 +126,14 @@ using namespace gr;
 
 extern "C" size_t gr_expert_mlp_mxfp4_workspace_size(int num_tokens, int top_k, int num_experts, int hidden, int ffn) {
   if (num_tokens < 1 || top_k < 1 || num_experts < 1 || hidden < 1 || ffn < 1) return 0;
-  const int bm = mx_tile_rows((int64_t)num_tokens * top_k, num_experts);
+  const int bm = mx_tile_rows((int64_t)num_tokens * top_k, num_experts, ffn);
   return (size_t)plan_mx_workspace(num_tokens, top_k, num_experts, hidden, ffn, bm).bytes;
+}
+
+extern "C" int gr_expert_mlp_mxfp4_tile(int num_tokens, int top_k, int num_experts, int hidden, int ffn) {
+  if (num_tokens < 1 || top_k < 1 || num_experts < 1 || hidden < 1 || ffn < 1 || hidden > (1 << 21) || ffn > (1 << 21)) return 0;
+  const MxForm f = pick_mx_experts((int64_t)num_tokens * top_k, num_experts, hidden, ffn);
+  return 1000000 * f.up_stages + 1000 * f.bm + f.down_cols;
 }
 
 extern "C" gr_status_t gr_expert_mlp_mxfp4(void* out, int64_t out_stride, const void* x, int64_t x_stride,
@@ -127,9 +154,10 @@ extern "C" gr_status_t gr_expert_mlp_mxfp4(void* out, int64_t out_stride, const 
       !aligned(gate_up, 16) || !aligned(down, 16) || !aligned(out, 8) || out_stride % 4 != 0 ||
       (int64_t)T * H > (1ll << 32) - (1 << 24))
     return GR_ERR_UNSUPPORTED;
-  const int bm = mx_tile_rows((int64_t)T * top_k, num_experts);
+  const MxForm form = pick_mx_experts((int64_t)T * top_k, num_experts, H, F);
+  const int bm = form.bm;
   const MxWorkspace l = plan_mx_workspace(T, top_k, num_experts, H, F, bm);
-  const int cols = bm <= 64 ? 64 : 128;  // results of a workgroup, in the narrower product
+  const int cols = mx_up_cols(bm);  // (the down product's workgroups have as many or more)
   if (l.max_tiles * ((std::max(F, H) + cols - 1) / cols) > GRID_MAX - 8 || T > GRID_MAX) return GR_ERR_UNSUPPORTED;
   if (!workspace || !aligned(workspace, 256) || workspace_bytes < (size_t)l.bytes) return GR_ERR_WORKSPACE;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
@@ -195,7 +223,7 @@ extern "C" gr_status_t gr_expert_mlp_mxfp4(void* out, int64_t out_stride, const 
   dn.num_tiles = p.num_tiles;
   dn.slot = p.slot;
   dn.scatter = 1;
-  launch_mx_experts(up, dn, (int)l.max_tiles, num_experts, bm, stream);
+  launch_mx_experts(up, dn, (int)l.max_tiles, form, stream);
 
   const CombineArgs c{out, out_stride, ws + l.y, nullptr, 0, weights, ids, T, top_k, num_experts, H};
   const dim3 grid((unsigned)T, (unsigned)((H + 2047) / 2048));

@@ -131,6 +131,7 @@ SIGNATURES = {
         _I, _I, _I, _I, _I, _P,         # tokens, out_features, in_features, swiglu, out_dtype, stream
     ]),
     "gr_expert_mlp_mxfp4_workspace_size": (_SZ, [_I, _I, _I, _I, _I]),
+    "gr_expert_mlp_mxfp4_tile": (_I, [_I, _I, _I, _I, _I]),
     "gr_expert_mlp_mxfp4": (_I, [
         _P, _L, _P, _L, _P, _P, _P, _P, # out, out_stride, x, x_stride, gate_up, its scale, down, its scale
         _P, _P,                         # weights, ids

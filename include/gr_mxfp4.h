@@ -76,7 +76,8 @@ gr_status_t gr_linear_mxfp4(void* out, int64_t out_stride, uint8_t* out_scale, i
  * hidden % 32 == 0, ffn % 32 == 0; rows of x, and weights, 16-byte aligned; out rows
  * 8-byte aligned.  num_experts <= 1024, num_tokens < 2^23, num_tokens * hidden <
  * 2^32 - 2^24.  workspace: gr_expert_mlp_mxfp4_workspace_size bytes, 256-byte aligned,
- * no initial contents; calls that may overlap need one each.
+ * no initial contents; one for more tokens does for fewer; calls that may overlap need
+ * one each.
  */
 size_t gr_expert_mlp_mxfp4_workspace_size(int num_tokens, int top_k, int num_experts, int hidden, int ffn);
 gr_status_t gr_expert_mlp_mxfp4(void* out, int64_t out_stride, const void* x, int64_t x_stride, const void* gate_up,

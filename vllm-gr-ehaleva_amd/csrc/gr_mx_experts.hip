@@ -26,7 +26,6 @@ template <int DT> __global__ __launch_bounds__(PLAN_THREADS) void mx_expert_star
 
 struct MxWorkspace {
   int64_t hist, slot, tiles, num_tiles, x4, xs, act, act_scale, y, bytes;
-  int64_t max_tiles;
   int blocks;
 };
 
@@ -56,7 +55,10 @@ int mx_tile_rows(int64_t rows, int E, int F) {
   return bm;
 }
 
-MxWorkspace plan_mx_workspace(int T, int k, int E, int H, int F, int bm) {
+int64_t mx_most_tiles(int64_t rows, int E, int bm) { return rows / bm + std::min<int64_t>(rows, E); }
+
+// (H and F: sizes of which a call is refused too)
+MxWorkspace plan_mx_workspace(int T, int k, int E, int64_t H, int64_t F) {
   MxWorkspace w{};
   const int64_t rows = (int64_t)T * k;
   auto take = [&](int64_t bytes) {
@@ -65,11 +67,10 @@ MxWorkspace plan_mx_workspace(int T, int k, int E, int H, int F, int bm) {
     return at;
   };
   w.blocks = (int)((rows + PLAN_ROWS - 1) / PLAN_ROWS);
-  w.max_tiles = rows / bm + (rows < E ? rows : E);
   w.num_tiles = take(4);
   w.hist = take(4ll * w.blocks * E);
   w.slot = take(4 * rows);
-  w.tiles = take(16 * w.max_tiles);
+  w.tiles = take(16 * mx_most_tiles(rows, E, 32));  // (of the lowest ones: more tokens, of taller tiles, need no less)
   w.x4 = take((int64_t)T * ((H + 1) / 2));
   w.xs = take((int64_t)T * ((H + 31) / 32));
   w.act = take(rows * ((F + 1) / 2));
@@ -126,8 +127,7 @@ using namespace gr;
 
 extern "C" size_t gr_expert_mlp_mxfp4_workspace_size(int num_tokens, int top_k, int num_experts, int hidden, int ffn) {
   if (num_tokens < 1 || top_k < 1 || num_experts < 1 || hidden < 1 || ffn < 1) return 0;
-  const int bm = mx_tile_rows((int64_t)num_tokens * top_k, num_experts, ffn);
-  return (size_t)plan_mx_workspace(num_tokens, top_k, num_experts, hidden, ffn, bm).bytes;
+  return (size_t)plan_mx_workspace(num_tokens, top_k, num_experts, hidden, ffn).bytes;
 }
 
 extern "C" int gr_expert_mlp_mxfp4_tile(int num_tokens, int top_k, int num_experts, int hidden, int ffn) {
@@ -156,9 +156,10 @@ extern "C" gr_status_t gr_expert_mlp_mxfp4(void* out, int64_t out_stride, const 
     return GR_ERR_UNSUPPORTED;
   const MxForm form = pick_mx_experts((int64_t)T * top_k, num_experts, H, F);
   const int bm = form.bm;
-  const MxWorkspace l = plan_mx_workspace(T, top_k, num_experts, H, F, bm);
+  const MxWorkspace l = plan_mx_workspace(T, top_k, num_experts, H, F);
+  const int64_t tiles = mx_most_tiles((int64_t)T * top_k, num_experts, bm);
   const int cols = mx_up_cols(bm);  // (the down product's workgroups have as many or more)
-  if (l.max_tiles * ((std::max(F, H) + cols - 1) / cols) > GRID_MAX - 8 || T > GRID_MAX) return GR_ERR_UNSUPPORTED;
+  if (tiles * ((std::max(F, H) + cols - 1) / cols) > GRID_MAX - 8 || T > GRID_MAX) return GR_ERR_UNSUPPORTED;
   if (!workspace || !aligned(workspace, 256) || workspace_bytes < (size_t)l.bytes) return GR_ERR_WORKSPACE;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   const int rows = T * top_k;
@@ -223,7 +224,7 @@ extern "C" gr_status_t gr_expert_mlp_mxfp4(void* out, int64_t out_stride, const 
   dn.num_tiles = p.num_tiles;
   dn.slot = p.slot;
   dn.scatter = 1;
-  launch_mx_experts(up, dn, (int)l.max_tiles, form, stream);
+  launch_mx_experts(up, dn, (int)tiles, form, stream);
 
   const CombineArgs c{out, out_stride, ws + l.y, nullptr, 0, weights, ids, T, top_k, num_experts, H};
   const dim3 grid((unsigned)T, (unsigned)((H + 2047) / 2048));

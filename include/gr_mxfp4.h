@@ -52,10 +52,15 @@ gr_status_t gr_dequant_mxfp4(void* out, int64_t out_stride, const void* x, int64
  * Sums are float32: a block's 32 products are added exactly, four blocks are joined
  * within 2^-24 of their sum of magnitudes.  A pair of scales whose product is above
  * 2^127 or below 2^-126 gives infinities or flushed results as float32 does.  The
- * sizes of a call choose its kernel, and with it the order of the sums: a row's last
- * bits may differ between calls of other sizes (not between calls of the same).
- * in_features % 32 == 0; x and w rows 16-byte aligned, at most 4 MB apart; no more
- * than 2^35 results, less for sizes that leave 64 x 64 tiles part empty.
+ * sizes of a call choose its kernel, and with it the order of the sums: a row's float32
+ * sums may differ in their last bits between calls of other sizes (not between calls of
+ * the same).  In a 4-bit result such a difference can take a number that lies at a
+ * border to the next one, and a block whose largest lies at one to the next scale, by
+ * which all its numbers are rounded: what is made of it then depends on the number of
+ * rows in the call by as much as the format resolves.
+ * in_features % 32 == 0; x and w rows 16-byte aligned, at most 4 MB apart;
+ * num_tokens and out_features <= 2^28, no more than 2^35 results, less for sizes that
+ * leave 64 x 64 tiles part empty.
  */
 gr_status_t gr_linear_mxfp4(void* out, int64_t out_stride, uint8_t* out_scale, int64_t out_scale_stride, const void* x,
                             int64_t x_stride, const uint8_t* x_scale, int64_t x_scale_stride, const void* w,
@@ -71,13 +76,15 @@ gr_status_t gr_linear_mxfp4(void* out, int64_t out_stride, uint8_t* out_scale, i
  * [num_tokens, top_k] contiguous.  An id below 0 adds nothing (an expert of another
  * rank), one >= num_experts flags GR_DEV_BAD_EXPERT and adds nothing; an expert named
  * twice counts twice.  Sums are float32, the one over j too, which is in the order of j
- * and rounded once.  As for
- * gr_linear_mxfp4, a token's last bits may differ between calls of other sizes.
+ * and rounded once.  A token's result depends on its own row, choices and the experts
+ * alone: it has the same bits whatever other tokens the call has.
  * hidden % 32 == 0, ffn % 32 == 0; rows of x, and weights, 16-byte aligned; out rows
- * 8-byte aligned.  num_experts <= 1024, num_tokens < 2^23, num_tokens * hidden <
- * 2^32 - 2^24.  workspace: gr_expert_mlp_mxfp4_workspace_size bytes, 256-byte aligned,
- * no initial contents; one for more tokens does for fewer; calls that may overlap need
- * one each.
+ * 8-byte aligned.  num_experts <= 1024, hidden and ffn <= 2^21, num_tokens < 2^23,
+ * num_tokens * top_k <= 2^26, num_tokens * hidden <= 2^32 - 2^24, and fewer than 2^23 - 8
+ * workgroups: num_tokens * top_k over a tile's rows, plus one for each expert, times the
+ * larger of hidden and ffn over 64 (128 for tiles of 128 and 256 rows).
+ * workspace: gr_expert_mlp_mxfp4_workspace_size bytes, 256-byte aligned, no initial
+ * contents; one for more tokens does for fewer; calls that may overlap need one each.
  */
 size_t gr_expert_mlp_mxfp4_workspace_size(int num_tokens, int top_k, int num_experts, int hidden, int ffn);
 gr_status_t gr_expert_mlp_mxfp4(void* out, int64_t out_stride, const void* x, int64_t x_stride, const void* gate_up,

@@ -68,6 +68,13 @@ gr_status_t gr_linear_mxfp4(void* out, int64_t out_stride, uint8_t* out_scale, i
                             int out_features, int in_features, int swiglu, int out_dtype, hipStream_t stream);
 
 /*
+ * The tile that gr_linear_mxfp4 takes for these sizes: 1000 * rows + weight rows, with
+ * 1000000 * the tiles that share a CU (0: the few rows' kernel, of 16 rows); 0 for
+ * sizes that are not positive or above 2^28.
+ */
+int gr_linear_mxfp4_tile(int num_tokens, int out_features, int in_features, int swiglu, int out_dtype);
+
+/*
  * SwiGLU layers of the chosen experts with 4-bit weights:
  *   out[t] = sum_j weights[t, j] * down[e] q(silu(gate[e] q(x[t])) * (up[e] q(x[t]))),  e = ids[t, j]
  * with q as gr_quant_mxfp4.  x, out [num_tokens, hidden] fp16 or bf16 at their strides

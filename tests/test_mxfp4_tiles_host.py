@@ -32,3 +32,29 @@ def test_experts_tile_arguments(built_lib):
         assert built_lib.gr_expert_mlp_mxfp4_tile(*bad) == 0
     assert experts_tile(built_lib, *good) == (32, 3, 64)
     assert experts_tile(built_lib, 64, 8, 64, 2048, 768) == (32, 2, 256)
+
+
+def test_linear_tile_arguments(built_lib):
+    f = built_lib.gr_linear_mxfp4_tile
+    assert f(8, 64, 256, 0, 2) == 16016 and f(8, 64, 256, 1, 2) == 16032 and f(8, 64, 256, 0, 4) == 16032 and f(8, 64, 256, 1, 4) == 16064
+    for bad in ((0, 64, 256), (8, 0, 256), (8, 64, 0), (2 ** 28 + 1, 64, 256), (8, 2 ** 28 + 1, 256)):
+        assert f(*bad, 0, 2) == 0
+
+
+def test_every_form_is_tested(built_lib):
+    """The device tests name a size for each form that any size of a wide grid takes, and the form that it takes."""
+    from tests.test_gpu_mxfp4_tiles import EXPERT_TILES, TILES, tile
+    rows = [1, 2, 5, 9, 15, 17, 24, 33, 48, 64, 65, 90, 128, 129, 180, 256, 300, 400, 512, 700, 1000, 1500, 2048, 3000, 5000, 8192]
+    columns = [32, 96, 256, 512, 1024, 1536, 2048, 2592, 4096, 5120, 6144, 8192, 10240, 12288, 16384, 24576]
+    features = [32, 256, 512, 1024, 1536, 2048, 2592, 4096, 6144, 8192]
+    for mode, forms in TILES.items():
+        taken = {tile(mode, M, N, K) for M in rows for N in columns for K in features}
+        assert taken == set(forms), mode
+        for form, sizes in forms.items():
+            assert all(tile(mode, *s) == form for s in sizes), (mode, form)
+    f = built_lib.gr_expert_mlp_mxfp4_tile
+    taken = {f(T, k, E, H, F) for T in rows for E in (1, 4, 8, 16, 48, 64, 80, 128) for k in (1, 2, 8)
+             for H in (512, 1024, 2048, 2560, 4096) for F in (96, 256, 512, 768, 1024, 1536, 2048)}
+    assert taken == set(EXPERT_TILES)
+    for form, sizes in EXPERT_TILES.items():
+        assert all(f(T, k, E, H, F) == form for T, E, k, H, F in sizes), form

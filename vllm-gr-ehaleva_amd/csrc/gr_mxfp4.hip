@@ -107,17 +107,24 @@ int pick_mx(int M, int rows_w, int stages, bool quant) {
   return best;
 }
 
+// kMx' index, or below 0 the few rows' kernel of 16 (-1) or 32 (-2) columns.  Few rows, as long as the CUs hold all
+// workgroups at once: 8 x 4096 x 2048 3.7 us (64 x 64 tiles 5.0), 8 x 8192 x 6144 8.5 us in 32 columns a workgroup,
+// 9.5 in 16 (64 x 64 tiles 9.9; 32 x 8192 x 2048, twice that many, 7.4 and 5.2)
+int pick_linear_mx(int M, int N, int kbytes, bool gated, bool quant) {
+  const int64_t few = (int64_t)((M + 15) / 16) * ((N + 15) / 16);
+  if (few <= 256 && !quant) return -1;
+  if (few <= 512) return -2;
+  return pick_mx(M, gated ? 2 * N : N, (kbytes + 127) / 128, quant);
+}
+
 template <int MODE> void launch_linear_mx(const MxArgs& a, hipStream_t stream) {
   constexpr bool GATED = MODE == MM_SWIGLU || MODE == MM_SWIGLU_Q, QUANT = MODE == MM_SWIGLU_Q || MODE == MM_PLAIN_Q;
-  const int M = a.M, rows_w = GATED ? 2 * a.N : a.N;
-  // few rows, as long as the CUs hold all workgroups at once: 8 x 4096 x 2048 3.7 us (64 x 64 tiles 5.0), 8 x 8192 x
-  // 6144 8.5 us in 32 columns a workgroup, 9.5 in 16 (64 x 64 tiles 9.9; 32 x 8192 x 2048, twice that many, 7.4 and 5.2)
-  const int64_t few = (int64_t)((M + 15) / 16) * ((a.N + 15) / 16);
-  if constexpr (!QUANT) {
-    if (few <= 256) return launch_mx_few<1, 8, MODE>(a, stream);
-  }
-  if (few <= 512) return launch_mx_few<2, 8, MODE>(a, stream);
-  switch (pick_mx(M, rows_w, (a.kbytes + 127) / 128, QUANT)) {
+  const int M = a.M;
+  switch (pick_linear_mx(M, a.N, a.kbytes, GATED, QUANT)) {
+    case -1:
+      if constexpr (!QUANT) launch_mx_few<1, 8, MODE>(a, stream);
+      break;
+    case -2: launch_mx_few<2, 8, MODE>(a, stream); break;
     case 0:
       if constexpr (!QUANT) launch_mx<64, 64, 2, 2, 4, 4, MODE, false>(a, (M + 63) / 64, stream);
       break;
@@ -177,6 +184,13 @@ extern "C" gr_status_t gr_dequant_mxfp4(void* out, int64_t out_stride, const voi
   else if (dtype == GR_DTYPE_F16) go(mx_dequant_k<GR_DTYPE_F16>);
   else go(mx_dequant_k<GR_DTYPE_BF16>);
   return launch_status();
+}
+
+extern "C" int gr_linear_mxfp4_tile(int num_tokens, int out_features, int in_features, int swiglu, int out_dtype) {
+  if (num_tokens < 1 || out_features < 1 || in_features < 1 || num_tokens > (1 << 28) || out_features > (1 << 28)) return 0;
+  const int i = pick_linear_mx(num_tokens, out_features, in_features / 2, swiglu != 0, out_dtype == GR_DTYPE_MXFP4);
+  if (i < 0) return 16 * 1000 - 16 * i * (swiglu ? 2 : 1);
+  return 1000000 * kMx[i].per_cu + 1000 * kMx[i].bm + kMx[i].bn;
 }
 
 extern "C" gr_status_t gr_linear_mxfp4(void* out, int64_t out_stride, uint8_t* out_scale, int64_t out_scale_stride,

@@ -130,6 +130,7 @@ SIGNATURES = {
         _P, _L, _P, _L, _P, _L, _P, _L, # x, x_scale, w, w_scale, each with its stride
         _I, _I, _I, _I, _I, _P,         # tokens, out_features, in_features, swiglu, out_dtype, stream
     ]),
+    "gr_linear_mxfp4_tile": (_I, [_I, _I, _I, _I, _I]),
     "gr_expert_mlp_mxfp4_workspace_size": (_SZ, [_I, _I, _I, _I, _I]),
     "gr_expert_mlp_mxfp4_tile": (_I, [_I, _I, _I, _I, _I]),
     "gr_expert_mlp_mxfp4": (_I, [

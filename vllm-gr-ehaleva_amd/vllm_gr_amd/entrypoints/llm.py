@@ -96,7 +96,7 @@ class LLM:
     scales are served so in any case.  Sizes that these products do not take are
     refused here.  e4m3 halves the layers' memory; a step is faster with experts, not
     without.  4 bits take 27 % of it, and a step or a prefill of 2048-token prompts
-    16 to 44 % less time."""
+    16 to 43 % less time."""
 
     def __init__(self, cfg: DecoderConfig = SID_DECODER_1P7B, *, seed: int = 0, device="cuda",
                  num_blocks: int = 4096, block_size: int = 16, eos_token_id: int | None = None,

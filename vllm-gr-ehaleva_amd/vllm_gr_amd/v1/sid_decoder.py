@@ -22,7 +22,8 @@ elementwise stages are fused HIP kernels (include/gr_decoder.h): residual add
 + RMSNorm, per-head q/k RMSNorm + rotary + K/V cache write through the slot
 mapping, and the SiLU-gated product.  With weights from
 ``quantize_weights`` a layer's projections and experts are e4m3 in blocks of 128 x 128
-(include/gr_experts.h), their inputs quantised token by token.  Attention is
+(include/gr_experts.h) or 4-bit numbers in blocks of 32 of a row (include/gr_mxfp4.h),
+their inputs quantised token by token.  Attention is
 :class:`BeamAttentionImpl.forward`, the call vLLM's Attention layer makes
 (beam_attn.py:703-755), with the K/V already written (key/value None).
 Positions follow the reference's rule (a beam's j-th suffix token sits at prefix_len + j,

@@ -371,6 +371,8 @@ __global__ __launch_bounds__(64 * WM * WN * KG, (MxLds<BM, BN, WM, WN, KG, ST, C
           *reinterpret_cast<const u32x4_t*>(lds + r * PITCH + 16 * b);
       a.os4[row * a.os4_row + t.n0 / 32 + b] = scale[c];
     }
+  } else if constexpr (EXPERTS) {
+    M::template store<GR_DTYPE_F32>(a, t, acc, wt, wm, wn, lane, lds);
   } else {
     M::store_any(a, t, acc, wt, wm, wn, lane, lds);
   }
